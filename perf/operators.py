@@ -12,8 +12,8 @@ Definitions
   distill   loss_n = sum_j p_j (log p_j - log q_{i_j}), p = softmax of the teacher's values over T (the slots with an index
             in [0, V) alone), q = softmax of the student's row over T; a row without such a slot has loss 0 and gradient 0.
   draw      weights exp((z - max z) / T) of the top_k largest (ties: lowest index first), of those the smallest set whose
-            share reaches top_p, of those the ones with weight >= min_p; the label is the first whose running sum, in order
-            of the index, is over u times the total.  -1 where a row has nothing to draw.
+            share reaches top_p, of those the ones with weight >= min_p; the label is the first whose running sum, in the same
+            order of falling weight, is over u times the total.  -1 where a row has nothing to draw.
 """
 import math
 
@@ -248,10 +248,10 @@ def _draw_plain(s):
     before = p.cumsum(dim=1) - p
     p = torch.where((top_p >= 1) | (before < top_p * p.sum(dim=1, keepdim=True)) | (place == 0), p, 0.0)
     p = torch.where(p >= min_p, p, 0.0)
-    run_ = torch.zeros_like(p).scatter_(1, at, p).cumsum(dim=1)
-    label = (run_ <= s["u"].double()[:, None] * run_[:, -1:]).sum(dim=1, keepdim=True)
-    last = (run_ < run_[:, -1:]).sum(dim=1, keepdim=True)
-    return torch.where(some, torch.minimum(label, last), -1)[:, 0]
+    running = p.cumsum(dim=1)
+    place = (running <= s["u"].double()[:, None] * running[:, -1:]).sum(dim=1, keepdim=True)
+    last = (running < running[:, -1:]).sum(dim=1, keepdim=True)
+    return torch.where(some, at.gather(1, torch.minimum(place, last)), -1)[:, 0]
 
 
 def run(state):
@@ -344,7 +344,7 @@ def _exact_distill(s, case):
 
 
 def _exact_draw(s, case):
-    """Row by row over blocks of rows, by thresholds: a label is kept if it comes before the cut in (value, index) order."""
+    """Over blocks of rows, by every label's rank: a label is kept if it comes before the cut in (value, index) order."""
     z = s["logits"].double()
     out = []
     setting = {q: _column(s[q], z) for q in ("t", "top_k", "top_p", "min_p")}
@@ -359,10 +359,10 @@ def _exact_draw(s, case):
         share[:, 1:] = ranked.cumsum(1)[:, :-1]
         kept = (share.gather(1, rank) < tp * weight.sum(1, keepdim=True)) | (rank == 0) | (tp >= 1)
         weight = weight * kept * (weight >= mp)
-        running = weight.cumsum(1)
+        running = torch.zeros_like(weight).scatter_(1, rank, weight).cumsum(1)
         target = s["u"][rows].double()[:, None] * running[:, -1:]
-        label = torch.searchsorted(running, target, right=True)[:, 0]
-        out.append(torch.where(running[:, -1] > 0, label, -1))
+        place = torch.searchsorted(running, target, right=True)
+        out.append(torch.where(running[:, -1] > 0, (rank == place).to(torch.uint8).argmax(1), -1))
     return torch.cat(out)
 
 
