@@ -22,7 +22,7 @@
 extern "C" {
 #endif
 
-#define OBJNERF_ABI_VERSION 10
+#define OBJNERF_ABI_VERSION 11
 
 int objnerf_abi_version(void);
 const char* objnerf_last_error(void);
@@ -622,6 +622,52 @@ int objnerf_voxel_features(const objnerf_voxel_grid* grid, int C, const float* x
 int objnerf_pos_encode_block(const float* x, int64_t ldx, int64_t n, int C, int n_freqs, const float* freqs, float* out,
                              int64_t ldo, void* stream);
 int objnerf_repeat_rows(const float* src, int64_t lds, int64_t n_rows, int C, int repeat, float* out, int64_t ldo, void* stream);
+
+/* ---- label operators (ABI 11): rows of class / instance logits over the rays.  No reference file: the reference takes a ray's
+ * instance id from its dataset's masks (datasets/generic_dataset.py); these are what a label field over the rays learns from and
+ * answers with.  Strides are in elements of their tensor, the last dimension is contiguous, row offsets are 64-bit. ---- */
+#define OBJNERF_TYPE_F32 0
+#define OBJNERF_TYPE_BF16 1
+#define OBJNERF_TYPE_F16 2
+
+/* Distillation from a teacher's top logits.  Per row: p = softmax(teacher / T) over the slots whose index lies in [0, v) (any other
+ * index: an empty slot; so is a teacher value of -inf), q = softmax(student / T) over the v logits,
+ *   loss = sum_j p_j (log p_j - log q_{i_j}),    grad_v = (upstream / T) (q_v - sum_{j: i_j = v} p_j).
+ * A row without a filled slot has loss 0 and gradient 0 whatever its logits hold; otherwise NaN in the row, or no finite student
+ * logit, gives NaN; a student logit of -inf under a filled slot a loss of +inf.  An index may occur more than once.  loss or grad may
+ * be NULL; grad must not overlap student.  Sums in a fixed order: bit-reproducible.  fp32 statistics, grad rounded once. */
+typedef struct {
+  int64_t n;                 /* rows, < 2^31 */
+  int32_t v, k;              /* labels, slots: v >= 1, 1 <= k <= 1024 */
+  const void* student; int64_t student_stride; int32_t student_type;    /* (n, v) OBJNERF_TYPE_* */
+  int32_t teacher_type; const void* teacher; int64_t teacher_stride;    /* (n, k) OBJNERF_TYPE_* */
+  const void* index; int64_t index_stride; int32_t index_bytes;         /* (n, k) signed integers of 4 or 8 bytes */
+  int32_t _pad;
+  double temperature;        /* [1e-30, 1e30] */
+  float* loss;               /* (n) or NULL */
+  const float* upstream; int64_t upstream_stride;                       /* (n) gradient of the losses; stride 0 = one number */
+  void* grad; int64_t grad_stride;                                      /* (n, v) of the student's type, or NULL */
+} objnerf_distill_args;
+int objnerf_distill_top(const objnerf_distill_args* args, void* stream);
+
+/* One label per row at a given random number.  Weights w_v = exp((z_v - max z) / T); the order: falling z, equal ones by rising
+ * index; kept = the first top_k (0: all), of those the shortest prefix whose share reaches top_p (>= 1: all; at least one), of
+ * those the ones with w >= min_p (0: all); label = the first of the order whose running sum is over u * (sum of the kept).
+ * T <= 0 and top_k == 1: the first of the order.  NaN counts as -inf; a row of nothing but -inf: -1.  u outside [0, 1) is taken as
+ * the nearer end, NaN as 0.  Every setting is a number, or one per row where its pointer is not NULL (then not checked: a
+ * temperature that is not positive draws the first of the order, top_k < 0 counts as 0, NaN in top_p or min_p switches it off). */
+typedef struct {
+  int64_t n;                 /* rows, < 2^31 */
+  int32_t v, type;           /* labels >= 1; OBJNERF_TYPE_* */
+  const void* logits; int64_t logits_stride;
+  const float* u; int64_t u_stride;
+  const float* temperature_rows; double temperature;
+  const int32_t* top_k_rows; int64_t top_k;
+  const float* top_p_rows; double top_p;
+  const float* min_p_rows; double min_p;
+  int64_t* labels;           /* (n) */
+} objnerf_sample_args;
+int objnerf_sample_logits(const objnerf_sample_args* args, void* stream);
 
 /* ---- measurement hooks (bench.py): HIP-event timing of the MLP kernel on `stream` ---- */
 /* When enabled, objnerf_mlp_eval brackets its launch with hipEvents; objnerf_timing_read

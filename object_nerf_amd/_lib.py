@@ -12,7 +12,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # OBJNERF_LIB: developer hook for A/B-timing build variants (tools/); the product library is the in-tree one
 LIB_PATH = os.environ.get("OBJNERF_LIB") or os.path.join(_HERE, "libobjnerf_hip.so")
-ABI_VERSION = 10    # OBJNERF_ABI_VERSION of include/objnerf_hip.h these struct mirrors were written against
+ABI_VERSION = 11    # OBJNERF_ABI_VERSION of include/objnerf_hip.h these struct mirrors were written against
 
 c_float_p = C.POINTER(C.c_float)
 c_u8_p = C.POINTER(C.c_uint8)
@@ -174,6 +174,30 @@ class RenderMultiOut(C.Structure):
     ]
 
 
+class DistillArgs(C.Structure):
+    _fields_ = [
+        ("n", C.c_int64), ("v", C.c_int32), ("k", C.c_int32),
+        ("student", C.c_void_p), ("student_stride", C.c_int64), ("student_type", C.c_int32),
+        ("teacher_type", C.c_int32), ("teacher", C.c_void_p), ("teacher_stride", C.c_int64),
+        ("index", C.c_void_p), ("index_stride", C.c_int64), ("index_bytes", C.c_int32), ("_pad", C.c_int32),
+        ("temperature", C.c_double),
+        ("loss", C.c_void_p), ("upstream", C.c_void_p), ("upstream_stride", C.c_int64),
+        ("grad", C.c_void_p), ("grad_stride", C.c_int64),
+    ]
+
+
+class SampleArgs(C.Structure):
+    _fields_ = [
+        ("n", C.c_int64), ("v", C.c_int32), ("type", C.c_int32),
+        ("logits", C.c_void_p), ("logits_stride", C.c_int64), ("u", C.c_void_p), ("u_stride", C.c_int64),
+        ("temperature_rows", C.c_void_p), ("temperature", C.c_double),
+        ("top_k_rows", C.c_void_p), ("top_k", C.c_int64),
+        ("top_p_rows", C.c_void_p), ("top_p", C.c_double),
+        ("min_p_rows", C.c_void_p), ("min_p", C.c_double),
+        ("labels", C.c_void_p),
+    ]
+
+
 # every symbol include/objnerf_hip.h declares: (restype, argtypes)
 _VP = C.c_void_p
 SIGNATURES = {
@@ -242,6 +266,8 @@ SIGNATURES = {
     "objnerf_voxel_features": (C.c_int, [C.POINTER(VoxelGrid), C.c_int, _VP, C.c_int64, _VP, C.c_int64, _VP]),
     "objnerf_pos_encode_block": (C.c_int, [_VP, C.c_int64, C.c_int64, C.c_int, C.c_int, _VP, _VP, C.c_int64, _VP]),
     "objnerf_repeat_rows": (C.c_int, [_VP, C.c_int64, C.c_int64, C.c_int, C.c_int, _VP, C.c_int64, _VP]),
+    "objnerf_distill_top": (C.c_int, [C.POINTER(DistillArgs), _VP]),
+    "objnerf_sample_logits": (C.c_int, [C.POINTER(SampleArgs), _VP]),
     "objnerf_timing_enable": (C.c_int, [C.c_int]),
     "objnerf_timing_read": (C.c_int, [C.POINTER(C.c_int64), C.POINTER(C.c_double)]),
     "objnerf_train_timing_enable": (C.c_int, [C.c_int]),

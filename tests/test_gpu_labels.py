@@ -1,0 +1,321 @@
+"""GPU: the label operators against plain 64-bit forms, at the sizes, masks and strides where they can go wrong."""
+import math
+
+import pytest
+import torch
+
+import label_reference as R
+import object_nerf_amd as A
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _case(n, v, k, dtype, t_dtype, seed, spread=3.0):
+    g = _gen(seed)
+    z = (torch.randn(n, v, generator=g) * spread).to(dtype)
+    t = (torch.randn(n, k, generator=g) * 2).to(t_dtype)
+    i = torch.stack([torch.randperm(v, generator=g)[torch.arange(k) % v] for _ in range(n)])     # repeats where k > v
+    u = torch.rand(n, generator=g) + 0.25
+    return z, t, i, u
+
+
+def _check_distill(z, t, i, u, temperature, loss, grad=None):
+    """Bounds, with eps = 2^-24 the half step of fp32.  An exponent argument (z - m) c carries three roundings (difference, constant,
+    product), so exp is off by (3 d + 2) eps at distance d; terms with d > 25 weigh nothing in a sum of at least 1.  A sum of v terms
+    in chains of at least 256 threads adds (v / 256 + 16) eps.  loss = (mean of a - b) + log s - log A: the first is a mean of
+    numbers up to D = max |a - b| with the same relative error.  The gradient is the difference of q and p times upstream / T: each
+    term has that relative error (q at every distance: 3 d eps more), so the difference is off by it times their SUM, whatever
+    cancels, and is then rounded once to its type."""
+    eps = R.STEP[F32]
+    v = z.shape[1]
+    rl, rg, size = R.distill(z, t, i, u, temperature)
+    inf = torch.isinf(rl)
+    assert torch.equal(torch.isinf(loss.cpu()), inf), (loss.cpu(), rl)
+    part = (80 + v / 256 + 16 + t.shape[1] / 16) * eps
+    finite = z.float()[torch.isfinite(z.float())]
+    big = ((finite.max() - finite.min()).item() / temperature if finite.numel() else 0.0) + (t.float()[torch.isfinite(t.float())].abs().max().item() * 2 / temperature)
+    err = (loss.cpu().double() - rl)[~inf].abs()
+    assert err.numel() == 0 or err.max().item() <= part * (2 + big), (err.max().item(), part * (2 + big))
+    if grad is not None:
+        bound = R.STEP[z.dtype] * rg.abs() + (part + 3 * big * eps) * size + (2.0 ** -24 if z.dtype == F16 else 2.0 ** -126)
+        err = (grad.cpu().double() - rg).abs()
+        assert (err <= bound).all(), ((err - bound).max().item(), (err / bound).max().item())
+
+
+SIZES = [(3, 1, 1), (1, 2, 2), (5, 3, 8), (130, 63, 7), (33, 64, 8), (17, 65, 16), (9, 128, 17), (7, 129, 64), (6, 257, 5), (5, 1000, 65), (4, 1031, 64),
+         (3, 2048, 20), (3, 4097, 33), (2, 8200, 200), (3, 16385, 8), (2, 30011, 20), (2, 32768, 64), (2, 65537, 100), (1, 131072, 1024), (2, 140003, 9)]
+
+
+@pytest.mark.parametrize("n,v,k", SIZES)
+@pytest.mark.parametrize("dtype,t_dtype,i_dtype", [(F32, F32, torch.int64), (BF16, F32, torch.int32), (F16, BF16, torch.int64)])
+def test_distill_sizes_and_types(n, v, k, dtype, t_dtype, i_dtype):
+    z, t, i, u = _case(n, v, k, dtype, t_dtype, 7 * v + k)
+    i = i.to(i_dtype)
+    for temperature in (1.0, 2.5):
+        loss, grad = A.distill_top_logits_grad(z.to(DEV), t.to(DEV), i.to(DEV), u.to(DEV), temperature=temperature)
+        assert loss.dtype == F32 and grad.dtype == dtype and grad.shape == z.shape
+        _check_distill(z, t, i, u, temperature, loss, grad)
+        only = A.distill_top_logits(z.to(DEV), t.to(DEV), i.to(DEV), temperature=temperature)
+        assert torch.equal(only, loss)                    # one kernel, one order of sums
+
+
+@pytest.mark.parametrize("n,v,k", [(40, 64, 8), (12, 300, 20), (6, 5003, 70), (3, 70001, 16)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_distill_empty_slots_rows_and_masks(n, v, k, dtype):
+    z, t, i, u = _case(n, v, k, dtype, F32, 11)
+    g = _gen(3)
+    i[torch.rand(n, k, generator=g) < 0.3] = -1
+    i[0] = -7                                             # a row without a slot
+    z[0, 1] = math.nan                                    # whose logits are not looked at
+    i[1, :] = v                                           # beyond the labels: empty too
+    t[2, :] = -math.inf                                   # no weight: empty
+    i[2, 0] = 0
+    z[2] = -math.inf
+    t[:, 0] = torch.where(torch.arange(n) % 4 == 3, torch.tensor(-math.inf), t[:, 0])
+    low = torch.finfo(dtype).min
+    for r in range(3, n):                                 # masked labels that no slot names
+        free = [x for x in range(v) if x not in set(i[r].tolist())][:5]
+        z[r, free[:2]] = -math.inf
+        z[r, free[2:]] = low
+    loss, grad = A.distill_top_logits_grad(z.to(DEV), t.to(DEV), i.to(DEV), u.to(DEV))
+    assert torch.equal(loss[:3].cpu(), torch.zeros(3)) and torch.equal(grad[:3].cpu().float(), torch.zeros(3, v))
+    assert not torch.isnan(loss).any() and not torch.isnan(grad).any()
+    zz, zr = z.clone(), z[3:].float()
+    zz[:3] = 0
+    rl, rg, size = R.distill(zz, t, i, u, 1.0)
+    spread = 25.0
+    part = (80 + v / 256 + 16 + k / 16) * R.STEP[F32]
+    assert (loss.cpu().double() - rl).abs().max().item() <= part * (2 + spread)
+    bound = R.STEP[dtype] * rg.abs() + (part + 3 * spread * R.STEP[F32]) * size + (2.0 ** -24 if dtype == F16 else 2.0 ** -126)
+    assert ((grad.cpu().double() - rg).abs() <= bound).all()
+    assert (grad[3:].cpu().float()[zr == -math.inf] == 0).all()
+
+
+def test_distill_infinite_and_nan_rows():
+    z = torch.zeros(5, 70)
+    t, i = torch.zeros(5, 2), torch.tensor([[0, 1]] * 5)
+    z[0, 0] = -math.inf                                   # a slot that the student rules out
+    z[1, 5] = math.nan
+    z[2] = -math.inf
+    t[3, 0] = math.nan
+    z[4, 9] = -math.inf                                   # no slot names it
+    loss, grad = A.distill_top_logits_grad(z.to(DEV), t.to(DEV), i.to(DEV), torch.ones(5, device=DEV))
+    assert loss[0].item() == math.inf and all(math.isnan(loss[r].item()) for r in (1, 2, 3))
+    assert grad[0, 0].item() == -0.5 and torch.isnan(grad[1]).all() and torch.isnan(grad[2]).all()
+    assert math.isfinite(loss[4].item()) and grad[4, 9].item() == 0.0
+
+
+@pytest.mark.parametrize("v,k", [(40, 12), (700, 40), (9000, 300), (80001, 20)])
+def test_distill_repeated_index(v, k):
+    z, t, i, u = _case(6, v, k, F32, F32, 5)
+    i = i % max(2, k // 3)                                # every index about three times
+    i[1] = 3 % v
+    loss, grad = A.distill_top_logits_grad(z.to(DEV), t.to(DEV), i.to(DEV), u.to(DEV), temperature=0.5)
+    _check_distill(z, t, i, u, 0.5, loss, grad)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("v", [61, 1027, 40000])
+def test_distill_strides(dtype, v):
+    n, k = 5, 6
+    z, t, i, u = _case(n, v, k, dtype, F32, 2)
+    wide = torch.full((n, v + 11), 77.0, dtype=dtype, device=DEV)
+    wide[:, 3:3 + v] = z.to(DEV)
+    tw = torch.full((n, 2 * k), -5.0, device=DEV)
+    tw[:, 1:1 + k] = t.to(DEV)
+    iw = torch.zeros(k, n, dtype=torch.int64, device=DEV)
+    iw.copy_(i.t())
+    uw = torch.zeros(n, 3, device=DEV)
+    uw[:, 1] = u.to(DEV)
+    plain = A.distill_top_logits_grad(z.to(DEV), t.to(DEV), i.to(DEV), u.to(DEV))
+    views = A.distill_top_logits_grad(wide[:, 3:3 + v], tw[:, 1:1 + k], iw.t(), uw[:, 1])
+    columns = A.distill_top_logits_grad(z.to(DEV).t().contiguous().t(), t.to(DEV), i.to(DEV), u.to(DEV))
+    for got in (views, columns):
+        assert torch.equal(got[0], plain[0]) and torch.equal(got[1], plain[1])
+    same = A.distill_top_logits(z[:1].to(DEV).expand(n, v), t[:1].to(DEV).expand(n, k), i[:1].to(DEV).expand(n, k))
+    assert torch.equal(same, plain[0][:1].expand(n))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("v", [64, 3000, 40001])
+def test_distill_autograd(dtype, v):
+    n, k = 9, 7
+    z, t, i, u = _case(n, v, k, dtype, F32, 21)
+    leaf = z.to(DEV).requires_grad_()
+    args = (t.to(DEV), i.to(DEV))
+    loss = A.distill_top_logits(leaf, *args, temperature=2.0)
+    ref = A.distill_top_logits_grad(z.to(DEV), *args, u.to(DEV), temperature=2.0)
+    g, = torch.autograd.grad(loss, leaf, u.to(DEV), retain_graph=True)
+    assert torch.equal(loss.detach(), ref[0]) and torch.equal(g, ref[1])
+    g2, = torch.autograd.grad(loss.mean(), leaf, retain_graph=True)               # one number for every row, stride 0
+    assert torch.equal(g2, A.distill_top_logits_grad(z.to(DEV), *args, torch.full((n,), 1.0 / n, device=DEV), temperature=2.0)[1])
+    g3, = torch.autograd.grad(loss.double().sum(), leaf)
+    assert torch.equal(g3, A.distill_top_logits_grad(z.to(DEV), *args, torch.ones(n, device=DEV), temperature=2.0)[1])
+    with torch.no_grad():
+        assert not A.distill_top_logits(leaf, *args).requires_grad
+    with pytest.raises(ValueError, match="teacher"):
+        A.distill_top_logits(leaf, args[0].requires_grad_(), args[1])
+
+
+def test_distill_gradient_against_differences():
+    """Central differences of the operator's own fp32 losses with step h: truncation h^2 / 6 max |third derivative| (of a softmax
+    cross term: below 1) and 2 loss errors / 2 h."""
+    n, v, k, h = 4, 12, 3, 2.0 ** -5
+    z, t, i, _ = _case(n, v, k, F32, F32, 8, spread=1.0)
+    _, grad = A.distill_top_logits_grad(z.to(DEV), t.to(DEV), i.to(DEV), torch.ones(n, device=DEV))
+    moved = torch.cat([z[:, None] + h * torch.eye(v)[None], z[:, None] - h * torch.eye(v)[None]], 1).reshape(-1, v).to(DEV)
+    rep = lambda x: x[:, None].expand(-1, 2 * v, -1).reshape(-1, k).contiguous().to(DEV)                # noqa: E731
+    loss = A.distill_top_logits(moved, rep(t), rep(i)).reshape(n, 2, v).double().cpu()
+    num = (loss[:, 0] - loss[:, 1]) / (2 * h)
+    tol = h * h / 6 + 100 * R.STEP[F32] * 12 / h
+    assert (num - grad.cpu().double()).abs().max().item() <= tol
+
+
+def test_distill_offsets_past_32_bits():
+    v, k = 70, 3
+    z, t, i, u = _case(3, v, k, BF16, F32, 4)
+    stride = (1 << 30) + 3                                # the third row starts behind 2^31 elements
+    store = torch.empty(2 * stride + v, dtype=BF16, device=DEV)
+    rows = store.as_strided((3, v), (stride, 1))
+    rows.copy_(z.to(DEV))
+    far, near = (A.distill_top_logits_grad(x, t.to(DEV), i.to(DEV), u.to(DEV)) for x in (rows, z.to(DEV)))
+    assert torch.equal(far[0], near[0]) and torch.equal(far[1], near[1])
+    uu = torch.rand(3, generator=_gen(0)).to(DEV)
+    assert torch.equal(A.sample_logits(rows, uu), A.sample_logits(z.to(DEV), uu))
+
+
+def test_no_rows():
+    z, t, i, u = (torch.empty(0, 5, device=DEV), torch.empty(0, 2, device=DEV), torch.empty(0, 2, dtype=torch.int64, device=DEV), torch.empty(0, device=DEV))
+    loss, grad = A.distill_top_logits_grad(z, t, i, u)
+    assert loss.shape == (0,) and grad.shape == (0, 5) and A.sample_logits(z, u).shape == (0,)
+    leaf = z.requires_grad_()
+    A.distill_top_logits(leaf, t, i).sum().backward()
+    assert leaf.grad.shape == (0, 5)
+
+
+# ---- drawing a label ----
+
+FILTERS = [dict(), dict(temperature=0.6), dict(top_k=1), dict(top_k=5), dict(top_k=300), dict(top_p=0.9), dict(top_p=0.3, temperature=1.7), dict(min_p=0.05),
+           dict(temperature=0.8, top_k=40, top_p=0.95, min_p=0.01), dict(temperature=0.0), dict(top_p=0.0), dict(min_p=1.0), dict(top_k=700, top_p=0.999)]
+
+
+def _draw_check(z, u, **kw):
+    got = A.sample_logits(z.to(DEV), u.to(DEV), **{k: (x.to(DEV) if isinstance(x, torch.Tensor) else x) for k, x in kw.items()})
+    full = dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
+    full.update(kw)
+    want = R.sample(z, u, **full)
+    assert got.dtype == torch.int64 and torch.equal(got.cpu(), want), (kw, [(r, got[r].item(), want[r].item()) for r in range(len(want)) if got[r].item() != want[r].item()][:5])
+
+
+@pytest.mark.parametrize("kw", FILTERS, ids=str)
+@pytest.mark.parametrize("n,v,dtype", [(40, 1, F32), (60, 2, BF16), (70, 13, F16), (300, 64, F32), (130, 65, BF16), (90, 128, BF16), (50, 129, F32), (40, 1000, F16),
+                                       (25, 1025, F32), (12, 5003, BF16), (9, 30011, F16), (5, 32768, F32), (3, 70001, F32), (3, 131072, BF16)])
+def test_sample_sizes_types_and_filters(n, v, dtype, kw):
+    g = _gen(v)
+    _draw_check((torch.randn(n, v, generator=g) * 2.5).to(dtype), torch.rand(n, generator=g), **kw)
+
+
+@pytest.mark.parametrize("v", [3, 64, 100, 900, 3001, 66000])
+def test_sample_ties(v):
+    g = _gen(1)
+    z = torch.randint(0, 3, (12, v), generator=g).float()
+    z[0] = 1.5                                            # one value
+    z[1] = torch.where(torch.arange(v) % 2 == 0, 0.0, -0.0)        # equal numbers, other bits
+    z[2, : v // 2] = -math.inf
+    u = torch.rand(12, generator=g)
+    for kw in (dict(), dict(top_k=max(1, v // 3)), dict(top_p=0.5), dict(top_k=max(1, v // 2), top_p=0.25), dict(min_p=0.2)):
+        _draw_check(z, u, **kw)
+
+
+@pytest.mark.parametrize("v", [7, 64, 200, 5000, 70000])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_sample_masks_nan_and_infinities(v, dtype):
+    g = _gen(2)
+    z = (torch.randn(16, v, generator=g) * 2).to(dtype)
+    z[torch.rand(16, v, generator=g) < 0.5] = -math.inf
+    z[0] = -math.inf                                      # nothing to draw
+    z[1] = math.nan
+    z[2, ::2] = math.nan
+    z[3] = torch.finfo(dtype).min                         # a mask of the lowest value everywhere: equal weights
+    z[4] = torch.finfo(dtype).min
+    z[4, v // 2] = 0.25
+    z[5, 3] = math.inf                                    # certain
+    z[6, [1, 5]] = math.inf                               # two that are
+    z[7] = -math.inf
+    z[7, v - 1] = -3.0
+    z[8] = torch.finfo(dtype).max
+    z[8, 1] = torch.finfo(dtype).min
+    u = torch.rand(16, generator=g)
+    for kw in (dict(), dict(top_k=4), dict(top_p=0.7), dict(min_p=0.1), dict(top_k=6, top_p=0.8, min_p=0.05, temperature=0.5)):
+        _draw_check(z, u, **kw)
+
+
+def test_sample_random_numbers_at_the_ends():
+    z = torch.randn(6, 500, generator=_gen(5))
+    z[:, 400:] = -math.inf
+    u = torch.tensor([0.0, 1 - 2.0 ** -24, 1.0, 7.0, -1.0, math.nan])
+    got = A.sample_logits(z.to(DEV), u.to(DEV)).cpu()
+    want = R.sample(z, torch.tensor([0.0, 1 - 2.0 ** -24, 1.0, 1.0, 0.0, 0.0]), 1.0, 0, 1.0, 0.0)
+    assert torch.equal(got, want)
+
+
+def test_sample_settings_per_row():
+    n, v = 200, 700
+    g = _gen(9)
+    z, u = torch.randn(n, v, generator=g) * 2, torch.rand(n, generator=g)
+    kw = dict(temperature=torch.rand(n, generator=g) * 2, top_k=torch.randint(-1, 50, (n,), generator=g), top_p=torch.rand(n, generator=g) * 1.2, min_p=torch.rand(n, generator=g) * 0.2)
+    kw["temperature"][:5] = 0.0
+    kw["temperature"][5] = -1.0
+    _draw_check(z, u, **kw)
+    _draw_check(z, u, top_k=kw["top_k"].to(torch.int32), temperature=0.7)
+    with pytest.raises(TypeError):
+        A.sample_logits(z.to(DEV), u.to(DEV), top_k=kw["top_p"].to(DEV))
+    with pytest.raises(ValueError):
+        A.sample_logits(z.to(DEV), u.to(DEV), top_p=kw["top_p"][:5].to(DEV))
+    with pytest.raises(ValueError):
+        A.sample_logits(z.to(DEV), u)
+    for bad in (dict(temperature=-1.0), dict(temperature=math.nan), dict(top_k=-1), dict(top_p=-0.5), dict(min_p=2.0), dict(min_p=math.nan)):
+        with pytest.raises(ValueError):
+            A.sample_logits(z.to(DEV), u.to(DEV), **bad)
+
+
+def test_sample_strides():
+    n, v = 7, 333
+    z = torch.randn(n, v, generator=_gen(1)).to(torch.float16)
+    u = torch.rand(n, generator=_gen(2))
+    wide = torch.full((n, v + 9), 50.0, dtype=torch.float16, device=DEV)
+    wide[:, 5:5 + v] = z.to(DEV)
+    want = A.sample_logits(z.to(DEV), u.to(DEV), top_p=0.9)
+    assert torch.equal(A.sample_logits(wide[:, 5:5 + v], u.to(DEV), top_p=0.9), want)
+    assert torch.equal(A.sample_logits(z.to(DEV).t().contiguous().t(), u.to(DEV).double(), top_p=0.9), want)
+
+
+# ---- graphs and streams ----
+
+def test_replayed_graph_and_second_stream():
+    n, v, k = 33, 1500, 9
+    z, t, i, u = (x.to(DEV) for x in _case(n, v, k, BF16, F32, 13))
+    u = u - 0.25
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        A.distill_top_logits_grad(z, t, i, u)
+        A.sample_logits(z, u, top_p=0.9)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, grad = A.distill_top_logits_grad(z, t, i, u)
+        label = A.sample_logits(z, u, top_p=0.9)
+    for seed in range(4):
+        zz, tt, ii, uu = _case(n, v, k, BF16, F32, 100 + seed)
+        z.copy_(zz), t.copy_(tt), i.copy_(ii), u.copy_(uu - 0.25)
+        graph.replay()
+        want = A.distill_top_logits_grad(z, t, i, u)
+        assert torch.equal(loss, want[0]) and torch.equal(grad, want[1]) and torch.equal(label, A.sample_logits(z, u, top_p=0.9))
+        torch.cuda.synchronize()
