@@ -669,6 +669,39 @@ typedef struct {
 } objnerf_sample_args;
 int objnerf_sample_logits(const objnerf_sample_args* args, void* stream);
 
+/* Products in 8-bit floating point (OCP e4m3) with a scale for each block of 128.
+ * objnerf_fp8_quantize: x (rows, cols) -> values (rows, C') bytes, C' = cols filled up to a multiple of 128 with zeros, and scales
+ * (rows, B') bytes, B' = C' / 128 filled up to a multiple of 4 with 127; both without gaps between rows.  A block is 128 consecutive
+ * columns of one row (block_rows 1) or of 128 rows (128: their scale is repeated in every row); its scale is the power of two
+ * 2^(byte - 127), the smallest not below 2^-126 with max|block| / scale <= 448 (a block of zeros: byte 127); value = x / scale to
+ * nearest even.  Infinities and NaN set no scale and become NaN.
+ * values_t / scales_t: the same of x transposed, (cols, R') and (cols, BR') over the rows: blocks of 128 rows of one column
+ * (block_rows 1) or the same 128 x 128 blocks.  Either form may be NULL, not both.  column_sums (cols; optional, rows > 0): fp32 sums of x's
+ * columns in a fixed order, with workspace of objnerf_fp8_quantize_workspace_floats(). */
+typedef struct {
+  int64_t rows, cols;        /* < 2^31 each, rows * cols <= 2^40 */
+  const void* x; int64_t x_stride;
+  int32_t type, block_rows;  /* OBJNERF_TYPE_*; 1 or 128 */
+  uint8_t* values; uint8_t* scales;
+  uint8_t* values_t; uint8_t* scales_t;
+  float* column_sums; float* workspace;
+} objnerf_fp8_quantize_args;
+int64_t objnerf_fp8_quantize_workspace_floats(int64_t rows, int64_t cols);
+int objnerf_fp8_quantize(const objnerf_fp8_quantize_args* args, void* stream);
+/* C[M,N] = sum_k a[m][k] b[n][k] (+ bias[n]), then LeakyReLU(0.01) where `leaky`: both operands as objnerf_fp8_quantize writes them
+ * (K whole blocks, along the rows of both; strides in bytes), fp32 accumulation, C rounded once to its type.
+ * C in 16 bits: the 8-bit matrix instruction, which drops product bits more than 13 under the largest of eight before the fp32 sum;
+ * C in fp32: fp32 sums throughout. */
+typedef struct {
+  int64_t M, N, K;
+  const uint8_t* a; int64_t a_stride; const uint8_t* a_scale; int64_t a_scale_stride;
+  const uint8_t* b; int64_t b_stride; const uint8_t* b_scale; int64_t b_scale_stride;
+  const float* bias;         /* (N) or NULL */
+  int32_t leaky, c_type;     /* OBJNERF_TYPE_* */
+  void* c; int64_t c_stride;
+} objnerf_gemm_fp8_args;
+int objnerf_gemm_fp8(const objnerf_gemm_fp8_args* args, void* stream);
+
 /* ---- measurement hooks (bench.py): HIP-event timing of the MLP kernel on `stream` ---- */
 /* When enabled, objnerf_mlp_eval brackets its launch with hipEvents; objnerf_timing_read
  * synchronises those events and returns {launch count, total ms} since the last reset. */

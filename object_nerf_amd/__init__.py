@@ -9,7 +9,9 @@ from .nerf_model import ObjectNeRF  # noqa: F401
 from .embedding_helper import Embedding, EmbeddingVoxel  # noqa: F401
 from .code_library import CodeLibrary  # noqa: F401
 from .rendering import render_rays, sample_pdf  # noqa: F401
-from .label_ops import distill_top_logits, distill_top_logits_grad, sample_logits  # noqa: F401
+from .label_ops import (Fp8Matrix, quantize_fp8, matmul_fp8, linear_fp8, distill_top_logits,  # noqa: F401
+                        distill_top_logits_grad, sample_logits)
 
 __all__ = ["ObjectNeRF", "Embedding", "EmbeddingVoxel", "CodeLibrary", "render_rays", "sample_pdf",
-           "AttrDict", "default_model_config", "distill_top_logits", "distill_top_logits_grad", "sample_logits"]
+           "AttrDict", "default_model_config", "Fp8Matrix", "quantize_fp8", "matmul_fp8", "linear_fp8",
+           "distill_top_logits", "distill_top_logits_grad", "sample_logits"]

@@ -198,6 +198,23 @@ class SampleArgs(C.Structure):
     ]
 
 
+class Fp8QuantizeArgs(C.Structure):
+    _fields_ = [
+        ("rows", C.c_int64), ("cols", C.c_int64), ("x", C.c_void_p), ("x_stride", C.c_int64), ("type", C.c_int32), ("block_rows", C.c_int32),
+        ("values", C.c_void_p), ("scales", C.c_void_p), ("values_t", C.c_void_p), ("scales_t", C.c_void_p),
+        ("column_sums", C.c_void_p), ("workspace", C.c_void_p),
+    ]
+
+
+class GemmFp8Args(C.Structure):
+    _fields_ = [
+        ("M", C.c_int64), ("N", C.c_int64), ("K", C.c_int64),
+        ("a", C.c_void_p), ("a_stride", C.c_int64), ("a_scale", C.c_void_p), ("a_scale_stride", C.c_int64),
+        ("b", C.c_void_p), ("b_stride", C.c_int64), ("b_scale", C.c_void_p), ("b_scale_stride", C.c_int64),
+        ("bias", C.c_void_p), ("leaky", C.c_int32), ("c_type", C.c_int32), ("c", C.c_void_p), ("c_stride", C.c_int64),
+    ]
+
+
 # every symbol include/objnerf_hip.h declares: (restype, argtypes)
 _VP = C.c_void_p
 SIGNATURES = {
@@ -267,6 +284,9 @@ SIGNATURES = {
     "objnerf_pos_encode_block": (C.c_int, [_VP, C.c_int64, C.c_int64, C.c_int, C.c_int, _VP, _VP, C.c_int64, _VP]),
     "objnerf_repeat_rows": (C.c_int, [_VP, C.c_int64, C.c_int64, C.c_int, C.c_int, _VP, C.c_int64, _VP]),
     "objnerf_distill_top": (C.c_int, [C.POINTER(DistillArgs), _VP]),
+    "objnerf_fp8_quantize_workspace_floats": (C.c_int64, [C.c_int64, C.c_int64]),
+    "objnerf_fp8_quantize": (C.c_int, [C.POINTER(Fp8QuantizeArgs), _VP]),
+    "objnerf_gemm_fp8": (C.c_int, [C.POINTER(GemmFp8Args), _VP]),
     "objnerf_sample_logits": (C.c_int, [C.POINTER(SampleArgs), _VP]),
     "objnerf_timing_enable": (C.c_int, [C.c_int]),
     "objnerf_timing_read": (C.c_int, [C.POINTER(C.c_int64), C.POINTER(C.c_double)]),

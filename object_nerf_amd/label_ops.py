@@ -1,5 +1,8 @@
 """Label operators: what a label field over the rays forms its logits with, learns from and answers with.
 
+  linear_fp8                x @ weight.T + bias in 8-bit floating point with a scale for each block of 128, differentiable;
+                            quantize_fp8 / matmul_fp8: its two halves, for weights that are laid out once.  The fp32 product of the
+                            layer-wise training path (objnerf_gemm) at a quarter of its bytes
   distill_top_logits        loss of rows of student logits against a teacher's top logits (a 2-D segmenter of which only the largest
                             values per pixel are stored), differentiable; distill_top_logits_grad: loss and gradient in one pass
   sample_logits             one label per row at a given random number, behind temperature / top-k / top-p / min-p -- to logits what
@@ -11,12 +14,13 @@ a call can be captured in a graph.  Arguments of a wrong type raise TypeError, o
 failing launches RuntimeError.
 """
 import ctypes as C
+from typing import NamedTuple
 
 import torch
 
 from . import _lib
 
-__all__ = ["distill_top_logits", "distill_top_logits_grad", "sample_logits"]
+__all__ = ["Fp8Matrix", "quantize_fp8", "matmul_fp8", "linear_fp8", "distill_top_logits", "distill_top_logits_grad", "sample_logits"]
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # OBJNERF_TYPE_*
 MAX_SLOTS = 1024
@@ -54,6 +58,186 @@ def _call(fn, args, device, what):
     rc = fn(C.byref(args), C.c_void_p(torch.cuda.current_stream().cuda_stream))
     if rc:
         _lib.check(rc, what)
+
+
+# ---- products in 8-bit floating point ----
+
+BLOCK = 128
+
+
+class Fp8Matrix(NamedTuple):
+    """A matrix (R, cols) in e4m3 with a power-of-two scale for each block of 128 columns of a row.
+
+    data (R, C') float8_e4m3fn, C' = cols filled up to a multiple of 128 with zeros; scale (R, B') uint8, B' = C' / 128 filled up to a
+    multiple of 4: element [r, c] stands for data[r, c] * 2 ** (scale[r, c // 128] - 127)."""
+    data: torch.Tensor
+    scale: torch.Tensor
+    cols: int
+
+
+def _up(n, step):
+    return -(-n // step) * step
+
+
+def _empty_fp8(rows, cols, device):
+    width = _up(cols, BLOCK)
+    return Fp8Matrix(torch.empty(rows, width, dtype=torch.float8_e4m3fn, device=device),
+                     torch.empty(rows, _up(width // BLOCK, 4), dtype=torch.uint8, device=device), cols)
+
+
+def _quantize(x, block_rows, rows=True, columns=False, sums=False):
+    """(x by rows, x by columns, column sums) of a 2-D GPU tensor with contiguous rows, each where asked for, in one pass over x"""
+    r, c = x.shape
+    q = _empty_fp8(r, c, x.device) if rows else None
+    t = _empty_fp8(c, r, x.device) if columns else None
+    total = None
+    a = _lib.Fp8QuantizeArgs()
+    a.rows, a.cols, a.x, a.x_stride, a.type, a.block_rows = r, c, x.data_ptr(), x.stride(0), _TYPES[x.dtype], block_rows
+    if rows:
+        a.values, a.scales = q.data.data_ptr(), q.scale.data_ptr()
+    if columns:
+        a.values_t, a.scales_t = t.data.data_ptr(), t.scale.data_ptr()
+    if sums:
+        work = torch.empty(_up(r, BLOCK) // BLOCK * c, dtype=torch.float32, device=x.device)
+        total = torch.empty(c, dtype=torch.float32, device=x.device)
+        a.workspace, a.column_sums = work.data_ptr(), total.data_ptr()
+    if r and c:
+        _call(_lib.lib().objnerf_fp8_quantize, a, x.device, "fp8_quantize")
+    return q, t, total
+
+
+def _product(a, b, bias, leaky, out_dtype):
+    """(M, N) of two Fp8Matrix over the same columns"""
+    m, n, dev = a.data.shape[0], b.data.shape[0], a.data.device
+    out = torch.empty(m, n, dtype=out_dtype, device=dev)
+    g = _lib.GemmFp8Args()
+    g.M, g.N, g.K = m, n, a.data.shape[1]
+    g.a, g.a_stride, g.a_scale, g.a_scale_stride = a.data.data_ptr(), a.data.stride(0), a.scale.data_ptr(), a.scale.stride(0)
+    g.b, g.b_stride, g.b_scale, g.b_scale_stride = b.data.data_ptr(), b.data.stride(0), b.scale.data_ptr(), b.scale.stride(0)
+    if bias is not None:
+        g.bias = bias.data_ptr()
+    g.leaky, g.c_type, g.c, g.c_stride = int(leaky), _TYPES[out_dtype], out.data_ptr(), n
+    if m and n:
+        _call(_lib.lib().objnerf_gemm_fp8, g, dev, "gemm_fp8")
+    return out
+
+
+def _checked_fp8(x, name):
+    if not isinstance(x, Fp8Matrix):
+        raise TypeError("%s must be an Fp8Matrix (quantize_fp8), got %s" % (name, type(x).__name__))
+    d, s = x.data, x.scale
+    if d.dtype != torch.float8_e4m3fn or s.dtype != torch.uint8:
+        raise TypeError("%s: data must be float8_e4m3fn and scale uint8, got %s and %s" % (name, d.dtype, s.dtype))
+    width = _up(x.cols, BLOCK)
+    if d.dim() != 2 or s.dim() != 2 or d.shape[1] != width or tuple(s.shape) != (d.shape[0], _up(width // BLOCK, 4)):
+        raise ValueError("%s: data %s and scale %s do not hold %d columns in blocks of 128" % (name, tuple(d.shape), tuple(s.shape), x.cols))
+    if not d.is_cuda:
+        _lib.require_cuda(d, name)
+    if s.device != d.device:
+        raise ValueError("%s: data and scale must be on one device" % name)
+    if not (d.is_contiguous() and s.is_contiguous()) or d.data_ptr() % 16 or s.data_ptr() % 4:
+        raise ValueError("%s: data and scale must be contiguous and aligned to 16 and 4 bytes" % name)
+    return x
+
+
+def _checked_bias(bias, n, device):
+    if bias is None:
+        return None
+    if not isinstance(bias, torch.Tensor):
+        raise TypeError("bias must be a tensor, got %s" % type(bias).__name__)
+    return _column(bias.detach(), "bias", n, device)
+
+
+def quantize_fp8(x, block_rows=1, transpose=False):
+    """x (R, C) rounded to an Fp8Matrix: blocks of 128 columns of one row (block_rows 1: activations, gradients) or of 128 rows
+    (block_rows 128: weights).  A block's scale is the smallest power of two with max|block| / scale <= 448, so dividing by it is exact and
+    an element is rounded once, to nearest even; infinities and NaN become NaN and set no scale.  `transpose` rounds x.T -- its blocks run
+    along x's rows -- without forming it."""
+    if block_rows not in (1, BLOCK):
+        raise ValueError("block_rows must be 1 or 128, got %r" % (block_rows,))
+    q, t, _ = _quantize(_rows(x, "x").detach(), block_rows, not transpose, transpose)
+    return t if transpose else q
+
+
+def matmul_fp8(a, b, bias=None, activation=None, out_dtype=torch.bfloat16):
+    """a @ b.T (+ bias) of two Fp8Matrix (M, K) and (N, K): fp32 sums, rounded once to out_dtype (float32, bfloat16 or float16).
+    activation: None or "leaky_relu" (slope 0.01, the reference's layers).  Not differentiable (linear_fp8 is)."""
+    _checked_fp8(a, "a")
+    _checked_fp8(b, "b")
+    if a.cols != b.cols:
+        raise ValueError("a and b must have the same columns, got %d and %d" % (a.cols, b.cols))
+    if a.data.device != b.data.device:
+        raise ValueError("a and b must be on one device")
+    if activation not in (None, "leaky_relu"):
+        raise ValueError("activation must be None or 'leaky_relu', got %r" % (activation,))
+    if out_dtype not in _TYPES:
+        raise TypeError("out_dtype: %s is not supported" % (out_dtype,))
+    if bias is not None and isinstance(bias, torch.Tensor) and bias.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError("matmul_fp8 is inference-only: use linear_fp8 where a gradient is needed")
+    return _product(a, b, _checked_bias(bias, b.data.shape[0], a.data.device), activation is not None, out_dtype)
+
+
+class _LinearFp8Fn(torch.autograd.Function):
+    """y = X8 W8^T + b; dX = dY8 W8, dW = (dY^T)8 (X^T)8, db = column sums of dY.  Kept for the backward pass: both transposed operands in
+    their 8-bit form, written by the launches that round the forward's."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, out_dtype):
+        need_x, need_w, _, _ = ctx.needs_input_grad
+        xq, xt, _ = _quantize(x, 1, True, need_w)
+        wq, wt, _ = _quantize(weight, BLOCK, True, need_x)
+        ctx.save_for_backward(*((xt.data, xt.scale) if need_w else (None, None)), *((wt.data, wt.scale) if need_x else (None, None)))
+        ctx.types = x.dtype, weight.dtype, None if bias is None else bias.dtype
+        ctx.sizes = x.shape[0], weight.shape[0], x.shape[1]
+        return _product(xq, wq, _checked_bias(bias, weight.shape[0], x.device), False, out_dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        xt, sxt, wt, swt = ctx.saved_tensors
+        m, n, k = ctx.sizes
+        if dy.dtype not in _TYPES:
+            dy = dy.float()
+        dy = _rows(dy, "the gradient of y")
+        if m == 0:
+            db = torch.zeros(n, dtype=torch.float32, device=dy.device) if need_b else None
+            dq, dt, _ = _quantize(dy, 1, need_x, need_w)
+        else:
+            dq, dt, db = _quantize(dy, 1, need_x or not need_w, need_w, need_b)
+        dx = _product(dq, Fp8Matrix(wt, swt, n), None, False, ctx.types[0]) if need_x else None
+        dw = _product(dt, Fp8Matrix(xt, sxt, m), None, False, ctx.types[1]) if need_w else None
+        return dx, dw, None if db is None else db.to(ctx.types[2]), None
+
+
+def linear_fp8(x, weight, bias=None, out_dtype=None):
+    """x @ weight.T + bias, both factors rounded to 8-bit floating point with a scale for each block of 128 (x: 128 columns of a row,
+    weight: 128 x 128), (M, N) in out_dtype (default: x's type).
+
+    x (M, K); weight (N, K), a tensor -- rounded in every call, so that what an optimizer wrote is what counts -- or the Fp8Matrix that
+    quantize_fp8(weight, block_rows=128) laid out once, for inference; bias (N,).  Sizes need not be multiples of anything.  With a tensor
+    as weight it is differentiable: dX and dW are products of the same kind, of the gradient rounded along their own sums, in x's and
+    weight's types; the bias gradient is an fp32 sum."""
+    x = _rows(x, "x")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in _TYPES:
+        raise TypeError("out_dtype: %s is not supported" % (out_dtype,))
+    recording = torch.is_grad_enabled()
+    if isinstance(weight, Fp8Matrix):
+        _checked_fp8(weight, "weight")
+        if weight.cols != x.shape[1] or weight.data.device != x.device:
+            raise ValueError("x %s on %s does not fit a weight of %d columns on %s" % (tuple(x.shape), x.device, weight.cols, weight.data.device))
+        if recording and (x.requires_grad or (isinstance(bias, torch.Tensor) and bias.requires_grad)):
+            raise NotImplementedError("linear_fp8 with an Fp8Matrix is inference-only: pass the weight as a tensor where a gradient is needed")
+        return _product(_quantize(x, 1)[0], weight, _checked_bias(bias, weight.data.shape[0], x.device), False, out_dtype)
+    weight = _rows(weight, "weight")
+    if weight.shape[1] != x.shape[1] or weight.device != x.device:
+        raise ValueError("x %s on %s does not fit weight %s on %s" % (tuple(x.shape), x.device, tuple(weight.shape), weight.device))
+    if bias is not None:
+        _checked_bias(bias, weight.shape[0], x.device)
+    if recording and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        return _LinearFp8Fn.apply(x, weight, bias, out_dtype)
+    return _product(_quantize(x, 1)[0], _quantize(weight, BLOCK)[0], _checked_bias(bias, weight.shape[0], x.device), False, out_dtype)
 
 
 # ---- distillation ----

@@ -60,3 +60,27 @@ def sample(logits, u, temperature, top_k, top_p, min_p):
         last = int((run < run[-1]).sum())
         out.append(int(order[min(place, last)]))
     return torch.tensor(out)
+
+
+def fp8(x, block_rows):
+    """the values that x (R, C) stands for in e4m3 with a power-of-two scale per block of block_rows x 128, in float64, and the scale
+    bytes (R, blocks)"""
+    x = x.detach().cpu().double()
+    r, c = x.shape
+    out, scale = torch.zeros_like(x), torch.zeros(r, -(-c // 128), dtype=torch.int64)
+    for b in range(scale.shape[1]):
+        for top in range(0, r, block_rows):
+            blk = x[top:top + block_rows, b * 128:(b + 1) * 128]
+            mag = torch.where(torch.isfinite(blk), blk.abs(), torch.zeros_like(blk))
+            largest = float(mag.max())
+            e = 0
+            if largest > 0:
+                e = math.frexp(largest)[1] - 10
+                while largest > 448.0 * 2.0 ** e:
+                    e += 1
+                e = max(e, -126)
+            u = blk / 2.0 ** e
+            grid = 2.0 ** (torch.clamp(torch.frexp(u)[1] - 1, min=-6).double() - 3)
+            out[top:top + block_rows, b * 128:(b + 1) * 128] = torch.where(torch.isfinite(u), torch.round(u / grid) * grid * 2.0 ** e, torch.full_like(u, math.nan))
+            scale[top:top + block_rows, b] = 127 + e
+    return out, scale

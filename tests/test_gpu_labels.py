@@ -296,6 +296,217 @@ def test_sample_strides():
     assert torch.equal(A.sample_logits(z.to(DEV).t().contiguous().t(), u.to(DEV).double(), top_p=0.9), want)
 
 
+# ---- products in 8-bit floating point ----
+
+def _values(q):
+    return (q.data.cpu().double() * 2.0 ** (q.scale.cpu().double() - 127).repeat_interleave(128, 1)[:, :q.data.shape[1]])[:, :q.cols]
+
+
+def _same(got, want):
+    """equal numbers, NaN in the same places (one input of the float16 cases overflows to an infinity, which stands for NaN)"""
+    return torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+
+
+def _features(r, c, dtype, seed):
+    """rows of widely different sizes, blocks of zeros among them"""
+    g = _gen(seed)
+    x = torch.randn(r, c, generator=g) * torch.exp(2 * torch.randn(r, 1, generator=g)) * torch.exp(torch.randn(c, generator=g))
+    x[torch.rand(r, c, generator=g) < 0.1] = 0.0
+    x[0, :130] = 0.0
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("r,c", [(1, 1), (1, 128), (3, 127), (16, 129), (17, 256), (128, 64), (129, 130), (130, 520), (257, 1000), (5, 8191), (300, 3)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize_fp8(r, c, dtype, block_rows):
+    """equal to the definition, bit for bit: the scale is a power of two, so nothing but the rounding to e4m3 rounds"""
+    x = _features(r, c, dtype, r + c)
+    q = A.quantize_fp8(x.to(DEV), block_rows)
+    want, scale = R.fp8(x, block_rows)
+    assert _same(_values(q), want)
+    nb = -(-c // 128)
+    assert torch.equal(q.scale.cpu()[:, :nb].long(), scale) and (q.scale[:, nb:] == 127).all()
+    assert q.data.shape == (r, nb * 128) and (q.data[:, c:].float() == 0).all()
+    t = A.quantize_fp8(x.to(DEV), block_rows, transpose=True)
+    want, scale = R.fp8(x.t().contiguous(), block_rows)
+    assert _same(_values(t), want) and torch.equal(t.scale.cpu()[:, :scale.shape[1]].long(), scale)
+    assert (t.scale[:, scale.shape[1]:] == 127).all() and (t.data[:, r:].float() == 0).all()
+    wide = torch.full((r, c + 3), 1e4, dtype=dtype, device=DEV)
+    wide[:, 1:1 + c] = x.to(DEV)
+    for again in (A.quantize_fp8(wide[:, 1:1 + c], block_rows), A.quantize_fp8(x.to(DEV).t().contiguous().t(), block_rows)):
+        assert torch.equal(again.data.view(torch.uint8), q.data.view(torch.uint8)) and torch.equal(again.scale, q.scale)
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize_fp8_borders(block_rows):
+    """largest values at and next to 448 times a power of two, subnormal results, ties, the smallest and largest floats, infinities and NaN"""
+    up = lambda x: torch.nextafter(torch.tensor(x), torch.tensor(math.inf)).item()                 # noqa: E731
+    rows = [[448.0, 1.0, 2.0 ** -9, 2.0 ** -10, 3 * 2.0 ** -10, up(2.0 ** -10), 17.0, 19.0, 0.5 + 2.0 ** -5, -0.5 - 3 * 2.0 ** -5],
+            [up(448.0), 464.0, 1.0, -1.0, 0.3, 0.1, 1e-3, 0, 0, 0], [3.4e38, -3.3e38, 1.0, 1e30, 1e36, 0, 0, 0, 0, 0], [1e-45, -1e-44, 1e-40, 0, 0, 0, 0, 0, 0, 0],
+            [1e-38, 1e-40, 3e-39, 0, 0, 0, 0, 0, 0, 0], [2.0 ** -126 * 448, 2.0 ** -126, 1e-39, 0, 0, 0, 0, 0, 0, 0], [0.0] * 10]
+    x = torch.tensor(rows)
+    if block_rows == 1:
+        x = torch.cat([x, torch.tensor([[math.inf, 1.0, -math.inf, math.nan, 3.0, 0, 0, 0, 0, 0], [math.nan] * 10])])
+    for piece in ([x] if block_rows == 1 else x.split(1)):
+        q = A.quantize_fp8(piece.to(DEV), block_rows)
+        want, scale = R.fp8(piece, block_rows)
+        got = _values(q)
+        assert _same(got, want), (got, want)
+        assert torch.equal(q.scale.cpu()[:, :1].long(), scale)
+
+
+def _check_product(got, a, b, bias, leaky=False):
+    """Products of two e4m3 numbers are exact in fp32 (4 by 4 bits), scales are powers of two: what rounds is the sum of K terms in fp32, at
+    most K roundings (plus one for the bias), taken as a whole step each, of at most the sum of magnitudes, and the result's own
+    type, once.  Results in 16 bits come from the 8-bit matrix instruction, which adds eight products on a common exponent and drops what
+    lies more than 13 bits under their largest: each of the other seven loses less than 2^-13 of it, and the largest products of the
+    groups add up to no more than the sum of magnitudes."""
+    want = a @ b.t()
+    size = a.abs() @ b.abs().t()
+    if bias is not None:
+        want, size = want + bias.double(), size + bias.double().abs()
+    if leaky:
+        want = torch.where(want > 0, want, 0.01 * want)
+    tiny = 2.0 ** -24 if got.dtype == F16 else 2.0 ** -126
+    part = (a.shape[1] + 2) * 2 * R.STEP[F32] + (0 if got.dtype == F32 else 7 * 2.0 ** -13)
+    bound = R.STEP[got.dtype] * want.abs() + part * size * (1 + R.STEP[got.dtype]) + tiny
+    err = (got.cpu().double() - want).abs()
+    assert (err <= bound).all(), ((err - bound).max().item(), (err / bound.clamp(min=1e-300)).max().item())
+
+
+PRODUCTS = [(1, 1, 1), (1, 300, 256), (4, 1000, 130), (5, 33, 7), (16, 16, 128), (17, 129, 255), (33, 257, 256), (64, 64, 512), (65, 8, 100), (100, 4097, 64),
+            (128, 128, 128), (129, 1000, 1024), (257, 511, 640), (300, 2056, 520), (1000, 96, 256), (513, 260, 2100), (2048, 64, 256), (7, 40, 8000)]
+
+
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+@pytest.mark.parametrize("dtype,out", [(BF16, F32), (F32, BF16), (F16, F16)])
+def test_linear_fp8_sizes_and_types(m, n, k, dtype, out):
+    x = _features(m, k, dtype, m + k) * 0.125
+    w = (torch.randn(n, k, generator=_gen(n)) * k ** -0.5).to(dtype)
+    bias = torch.randn(n, generator=_gen(1)) if (m + n) % 2 else None
+    b = None if bias is None else bias.to(DEV)
+    y = A.linear_fp8(x.to(DEV), w.to(DEV), b, out_dtype=out)
+    assert y.shape == (m, n) and y.dtype == out
+    xq, wq = R.fp8(x, 1)[0], R.fp8(w, 128)[0]
+    _check_product(y, xq, wq, bias)
+    once = A.quantize_fp8(w.to(DEV), 128)
+    assert torch.equal(A.linear_fp8(x.to(DEV), once, b, out_dtype=out), y)
+    leaky = A.matmul_fp8(A.quantize_fp8(x.to(DEV)), once, b, activation="leaky_relu", out_dtype=out)
+    _check_product(leaky, xq, wq, bias, True)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (5, 33, 7), (130, 70, 300), (300, 129, 128), (257, 520, 64), (64, 1000, 256), (1500, 12, 40)])
+@pytest.mark.parametrize("dtype,w_dtype", [(BF16, BF16), (F32, F32), (BF16, F32), (F16, F16)])
+def test_linear_fp8_gradients(m, n, k, dtype, w_dtype):
+    x = (_features(m, k, dtype, 3) * 0.125).to(DEV).requires_grad_()
+    w = (torch.randn(n, k, generator=_gen(4)) * k ** -0.5).to(w_dtype).to(DEV).requires_grad_()
+    b = torch.randn(n, generator=_gen(5)).to(w_dtype).to(DEV).requires_grad_()
+    dy = (torch.randn(m, n, generator=_gen(6)) * m ** -0.5).to(dtype).to(DEV)
+    y = A.linear_fp8(x, w, b)
+    with torch.no_grad():
+        assert torch.equal(A.linear_fp8(x, w, b), y)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy, retain_graph=True)
+    assert dx.dtype == dtype and dw.dtype == w_dtype and db.dtype == w_dtype
+    d = dy.cpu()
+    _check_product(dx, R.fp8(d, 1)[0], R.fp8(w.t(), 128)[0], None)
+    _check_product(dw, R.fp8(d.t(), 1)[0], R.fp8(x.t(), 1)[0], None)
+    exact = d.double().sum(0)
+    bound = R.STEP[w_dtype] * exact.abs() + (m + 2) * R.STEP[F32] * d.double().abs().sum(0) * 1.01 + (2.0 ** -24 if w_dtype == F16 else 0)
+    assert ((db.cpu().double() - exact).abs() <= bound).all()
+    # each gradient alone, and again over the kept graph: the same bits
+    assert torch.equal(torch.autograd.grad(y, x, dy, retain_graph=True)[0], dx)
+    assert torch.equal(torch.autograd.grad(y, b, dy, retain_graph=True)[0], db)
+    assert torch.equal(torch.autograd.grad(y, w, dy)[0], dw)
+    alone = A.linear_fp8(x.detach(), w.detach(), b)
+    assert torch.equal(alone.detach(), y.detach()) and torch.equal(torch.autograd.grad(alone, b, dy)[0], db)
+
+
+def test_linear_fp8_gradient_against_differences():
+    """Where nothing is rounded (small whole numbers) the operator is a plain product: its gradients are its own differences, exactly."""
+    g = _gen(0)
+    x = torch.randint(-4, 5, (6, 40), generator=g).float().to(DEV).requires_grad_()
+    w = torch.randint(-4, 5, (9, 40), generator=g).float().to(DEV).requires_grad_()
+    dy = torch.randint(-2, 3, (6, 9), generator=g).float().to(DEV)
+    dx, dw = torch.autograd.grad(A.linear_fp8(x, w), (x, w), dy)
+    with torch.no_grad():
+        for r, c in ((0, 0), (3, 17), (5, 39)):
+            e = torch.zeros_like(x)
+            e[r, c] = 1.0
+            assert ((A.linear_fp8(x + e, w) - A.linear_fp8(x - e, w)) * dy).sum().item() / 2 == dx[r, c].item()
+        for r, c in ((0, 0), (4, 20), (8, 39)):
+            e = torch.zeros_like(w)
+            e[r, c] = 1.0
+            assert ((A.linear_fp8(x, w + e) - A.linear_fp8(x, w - e)) * dy).sum().item() / 2 == dw[r, c].item()
+
+
+def test_linear_fp8_nothing_to_do():
+    w, b = torch.randn(5, 7, device=DEV, requires_grad=True), torch.randn(5, device=DEV, requires_grad=True)
+    x = torch.empty(0, 7, device=DEV, requires_grad=True)
+    y = A.linear_fp8(x, w, b)
+    assert y.shape == (0, 5)
+    y.sum().backward()
+    assert torch.equal(w.grad, torch.zeros_like(w)) and torch.equal(b.grad, torch.zeros_like(b)) and x.grad.shape == (0, 7)
+    none = A.linear_fp8(torch.empty(3, 0, device=DEV), torch.empty(5, 0, device=DEV), b.detach())
+    assert torch.equal(none, b.detach().expand(3, 5))
+    assert A.linear_fp8(torch.empty(3, 7, device=DEV), torch.empty(0, 7, device=DEV)).shape == (3, 0)
+    poisoned = torch.randn(4, 300, device=DEV)
+    poisoned[2, 5] = math.inf
+    out = A.linear_fp8(poisoned, torch.randn(9, 300, device=DEV))
+    assert torch.isnan(out[2]).all() and torch.isfinite(out[[0, 1, 3]]).all()
+
+
+def test_fp8_refusals():
+    x, w = torch.randn(4, 256, device=DEV), torch.randn(8, 256, device=DEV)
+    q = A.quantize_fp8(w, 128)
+    for call in (lambda: A.quantize_fp8(x, 64), lambda: A.quantize_fp8(x[0]), lambda: A.matmul_fp8(A.quantize_fp8(x[:, :200]), q), lambda: A.linear_fp8(x[:, :200], w),
+                 lambda: A.linear_fp8(x, w, torch.zeros(7, device=DEV)), lambda: A.matmul_fp8(A.quantize_fp8(x), q, activation="relu"), lambda: A.linear_fp8(x, w.cpu().to("cpu")[:, :3].to(DEV)),
+                 lambda: A.matmul_fp8(A.Fp8Matrix(q.data, q.scale[:, :2], 256), q), lambda: A.matmul_fp8(A.Fp8Matrix(q.data[:, :128], q.scale, 128), q)):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: A.quantize_fp8(x.double()), lambda: A.matmul_fp8(x, q), lambda: A.linear_fp8(x, w, out_dtype=torch.float64), lambda: A.linear_fp8(x, w, 1.0),
+                 lambda: A.matmul_fp8(A.Fp8Matrix(q.data.view(torch.uint8), q.scale, 256), q)):
+        with pytest.raises(TypeError):
+            call()
+    with pytest.raises(RuntimeError, match="GPU"):
+        A.linear_fp8(x.cpu(), w)
+    with pytest.raises(NotImplementedError):
+        A.linear_fp8(x.clone().requires_grad_(), q)
+    with pytest.raises(NotImplementedError):
+        A.linear_fp8(x, q, torch.zeros(8, device=DEV, requires_grad=True))
+
+
+# ---- the operators together: a label head over rays, its training step and its answers ----
+
+def test_label_head_learns_and_answers():
+    """features of rays -> logits (8-bit product) -> distillation from a teacher's top logits -> gradients of features, weight and bias;
+    and logits -> a label per ray -> the object codes that render_rays takes"""
+    n, c, v, k = 300, 256, 64, 6
+    g = _gen(12)
+    feats = torch.randn(n, c, generator=g)
+    weight, bias = torch.randn(v, c, generator=g) * c ** -0.5, torch.randn(v, generator=g)
+    teacher, index = torch.randn(n, k, generator=g) * 2, torch.stack([torch.randperm(v, generator=g)[:k] for _ in range(n)])
+    index[::7, 3:] = -1
+    f, w, b = (x.to(DEV).requires_grad_() for x in (feats, weight, bias))
+    logits = A.linear_fp8(f, w, b)
+    loss = A.distill_top_logits(logits, teacher.to(DEV), index.to(DEV), temperature=2.0)
+    loss.mean().backward()
+    xq, wq = R.fp8(feats, 1)[0], R.fp8(weight, 128)[0]
+    _check_product(logits.detach(), xq, wq, bias)
+    _check_distill(logits.detach().cpu(), teacher, index, torch.full((n,), 1.0 / n), 2.0, loss.detach())
+    _, dz = A.distill_top_logits_grad(logits.detach(), teacher.to(DEV), index.to(DEV), torch.full((n,), 1.0 / n, device=DEV), temperature=2.0)
+    d = dz.cpu()
+    _check_product(f.grad, R.fp8(d, 1)[0], R.fp8(weight.t(), 128)[0], None)
+    _check_product(w.grad, R.fp8(d.t(), 1)[0], R.fp8(feats.t(), 1)[0], None)
+    assert (b.grad.cpu().double() - d.double().sum(0)).abs().max().item() <= (n + 2) * R.STEP[F32] * d.double().abs().sum(0).max().item()
+    u = torch.rand(n, generator=g)
+    ids = A.sample_logits(logits.detach(), u.to(DEV), temperature=0.7, top_k=8, top_p=0.95)
+    assert torch.equal(ids.cpu(), R.sample(logits.detach().cpu(), u, 0.7, 8, 0.95, 0.0))
+    codes = A.CodeLibrary(A.default_model_config()).to(DEV)
+    rows = codes({"instance_ids": ids})["embedding_instance"]
+    assert torch.equal(rows.detach(), codes.embedding_instance.weight.detach()[ids])
+
+
 # ---- graphs and streams ----
 
 def test_replayed_graph_and_second_stream():
@@ -307,15 +518,48 @@ def test_replayed_graph_and_second_stream():
     with torch.cuda.stream(side):
         A.distill_top_logits_grad(z, t, i, u)
         A.sample_logits(z, u, top_p=0.9)
+        A.linear_fp8(z, z[:100])
     torch.cuda.current_stream().wait_stream(side)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         loss, grad = A.distill_top_logits_grad(z, t, i, u)
         label = A.sample_logits(z, u, top_p=0.9)
+        y = A.linear_fp8(z, z[:100])
     for seed in range(4):
         zz, tt, ii, uu = _case(n, v, k, BF16, F32, 100 + seed)
         z.copy_(zz), t.copy_(tt), i.copy_(ii), u.copy_(uu - 0.25)
         graph.replay()
         want = A.distill_top_logits_grad(z, t, i, u)
         assert torch.equal(loss, want[0]) and torch.equal(grad, want[1]) and torch.equal(label, A.sample_logits(z, u, top_p=0.9))
+        assert torch.equal(y, A.linear_fp8(z, z[:100]))
+        torch.cuda.synchronize()
+
+
+def test_replayed_training_step():
+    """forward and backward of the head in one graph, replayed on changed data against the eager step"""
+    n, c, v, k = 200, 130, 90, 5
+    f, w, b = (torch.zeros(s, device=DEV, requires_grad=True) for s in ((n, c), (v, c), (v,)))
+    z, t, i, _ = _case(n, v, k, F32, F32, 3)
+    t, i = t.to(DEV), i.to(DEV)
+
+    def step():
+        loss = A.distill_top_logits(A.linear_fp8(f, w, b), t, i)
+        return (loss.detach(),) + torch.autograd.grad(loss.mean(), (f, w, b))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in range(3):
+        g = _gen(seed)
+        with torch.no_grad():
+            for p in (f, w, b):
+                p.copy_(torch.randn(p.shape, generator=g))
+        graph.replay()
+        for got, want in zip(out, step()):
+            assert torch.equal(got, want)
         torch.cuda.synchronize()
