@@ -7,12 +7,13 @@
 // With m = max z, s = sum exp((z - m) / T), a_j = (t_j - max t) / T, A = sum exp(a_j), b_j = (z_{i_j} - m) / T:
 //   loss = (1 / A) sum_j exp(a_j) (a_j - b_j) + log s - log A          (differences first: no large terms cancel)
 //
-// Bound by memory: z is read once for (m, s) and, where the gradient is asked for, once more while dz is written.  The statistics
-// are fp32, the sums in a fixed order (bit-reproducible).  The gradient's k special columns are not looked up while the row is
+// Bound by memory: a row up to 256 KB is read once and stays in registers until dz is written (longer ones are read twice).  The
+// statistics are fp32, the sums in a fixed order (bit-reproducible).  The gradient's k special columns are not looked up while the row is
 // written: the whole row is written as if p were 0, and behind a barrier the slots' own threads write their columns again.  The
 // first slot of an index owns its column and adds the shares of later slots with the same index in their order.
 #include "host_api.h"
 #include "label_ops.h"
+#include <type_traits>
 
 namespace objnerf {
 namespace {
@@ -45,137 +46,218 @@ __device__ __forceinline__ int slot_column(const DistillP& p, long row, int j) {
   return i >= 0 && i < p.v ? (int)i : -1;
 }
 
-template <int THREADS, class OP>
-__device__ __forceinline__ float block_reduce(float v, float* tmp) {
-  v = lanes_reduce<64, OP>(v);
-  if constexpr (THREADS > 64) {
-    const int wave = threadIdx.x >> 6;
-    __syncthreads();                            // tmp's last readers are done
-    if ((threadIdx.x & 63) == 0) tmp[wave] = v;
+// Reduction over the LANES threads that hold a row: within a wave, or over a workgroup through LDS (tmp: one float per wave, its own
+// for every call between two barriers of the caller).
+template <int LANES, class OP>
+__device__ __forceinline__ float row_reduce(float v, float* tmp) {
+  if constexpr (LANES <= 64) {
+    return lanes_reduce<LANES, OP>(v);
+  } else {
+    v = lanes_reduce<64, OP>(v);
+    if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = v;
     __syncthreads();
     v = tmp[0];
 #pragma unroll
-    for (int w = 1; w < THREADS / 64; ++w) v = OP::f(v, tmp[w]);
+    for (int w = 1; w < LANES / 64; ++w) v = OP::f(v, tmp[w]);
+    return v;
   }
-  return v;
 }
 
-// One workgroup per row.  The row is read in 16-byte pieces, four in flight per thread.
-template <class E, int THREADS>
-__global__ void __launch_bounds__(THREADS) distill_row_kernel(DistillP p) {
-  __shared__ float tmp[THREADS / 64], tmp2[THREADS / 64];
-  __shared__ int slot_i[kMaxSlots];
-  __shared__ float slot_e[kMaxSlots];
-  const long row = blockIdx.x;
-  const int tid = threadIdx.x;
-  const char* z = static_cast<const char*>(p.z) + row * p.ldz * E::kBytes;
-  const int pieces = p.v / E::kVec;
+// LANES threads per row (a row of 16 lanes, a wave, a workgroup).  PIECES > 0: the row stays in registers as it was read, LANES x PIECES
+// pieces of 16 bytes, and memory sees it once; 0: it is read again in each pass.
+template <class E, int LANES, int PIECES>
+__global__ void __launch_bounds__(LANES < 256 ? 256 : LANES, LANES < 1024 ? 6 : 4) distill_kernel(DistillP p) {
+  constexpr int kThreads = LANES < 256 ? 256 : LANES;
+  constexpr bool kGroups = LANES <= 64;                          // several rows per workgroup: one slot per thread at most
   constexpr float kInf = __builtin_inff();
+  __shared__ float tmp[6][kThreads / 64];
+  __shared__ int slot_i[kGroups ? kThreads : kMaxSlots];
+  __shared__ float slot_e[kGroups ? kThreads : kMaxSlots];
+  const int t = kGroups ? threadIdx.x & (LANES - 1) : threadIdx.x;
+  const long at = kGroups ? (long)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES : blockIdx.x;
+  const bool live = !kGroups || at < p.n;
+  const long row = live ? at : p.n - 1;
+  int* const my_i = slot_i + (kGroups ? threadIdx.x - t : 0);
+  float* const my_e = slot_e + (kGroups ? threadIdx.x - t : 0);
+  const char* z = static_cast<const char*>(p.z) + row * p.ldz * E::kBytes;
+  const int pieces = p.v / E::kVec, tail = p.v - pieces * E::kVec;
 
-  // running maximum and sum
-  float m = -kInf, s = 0.f;
-  for (int q = tid; q < pieces; q += THREADS * 4) {
-    u32x4 r[4];
+  // everything that does not wait for anything is asked for first: the row, the slots, the students' values under them
+  u32x4 r[PIECES > 0 ? PIECES : 1];
+  if constexpr (PIECES > 0)
 #pragma unroll
-    for (int u = 0; u < 4; ++u) r[u] = load16(z, (long)min(q + u * THREADS, pieces - 1) * 16);
+    for (int c = 0; c < PIECES; ++c)
+      if (t + c * LANES < pieces) r[c] = load16(z, (long)(t + c * LANES) * 16);
+  const float last = t < tail ? E::load(z, (long)pieces * E::kVec + t) : -kInf;
+  int i0 = t < p.k ? slot_column(p, row, t) : -1;
+  const float t0 = i0 >= 0 ? load_any(p.t, row * p.ldt + t, p.t_type) : -kInf;
+  if (t0 == -kInf) i0 = -1;                                      // a slot of -inf weighs nothing: empty
+  const float z0 = i0 >= 0 ? E::load(z, i0) : 0.f;
+
+  // largest of the row, of its teacher's values; is there a slot at all
+  float m = last, s = 0.f;
+  if constexpr (PIECES > 0) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (q + u * THREADS >= pieces) break;
-      float x[E::kVec];
-      E::unpack(r[u], x);
-      float mx = x[0];
+    for (int c = 0; c < PIECES; ++c)
+      if (t + c * LANES < pieces) {
+        float x[E::kVec];
+        E::unpack(r[c], x);
 #pragma unroll
-      for (int i = 1; i < E::kVec; ++i) mx = fmaxf(mx, x[i]);
-      if (mx > m) { s *= fast_exp2((m - mx) * p.c); m = mx; }
-      // a part of nothing but -inf adds nothing; NaN gets through either way
+        for (int i = 0; i < E::kVec; ++i) m = fmaxf(m, x[i]);
+      }
+  } else {
+    // running maximum and sum, four pieces in flight
+    for (int q = t; q < pieces; q += LANES * 4) {
+      u32x4 f[4];
 #pragma unroll
-      for (int i = 0; i < E::kVec; ++i) s += x[i] == -kInf ? 0.f : fast_exp2((x[i] - m) * p.c);
+      for (int u = 0; u < 4; ++u) f[u] = load16(z, (long)min(q + u * LANES, pieces - 1) * 16);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (q + u * LANES >= pieces) break;
+        float x[E::kVec];
+        E::unpack(f[u], x);
+        float mx = x[0];
+#pragma unroll
+        for (int i = 1; i < E::kVec; ++i) mx = fmaxf(mx, x[i]);
+        if (mx > m) { s *= fast_exp2((m - mx) * p.c); m = mx; }
+        // a part of nothing but -inf adds nothing; NaN gets through either way
+#pragma unroll
+        for (int i = 0; i < E::kVec; ++i) s += x[i] == -kInf ? 0.f : fast_exp2((x[i] - m) * p.c);
+      }
+    }
+    if (t < tail && last != -kInf) s += fast_exp2((last - m) * p.c);
+  }
+  float tm = t0, some = i0 >= 0 ? 1.f : 0.f;
+  if constexpr (!kGroups) {
+    if (t < p.k) { my_i[t] = i0; my_e[t] = t0; }
+    for (int j = t + LANES; j < p.k; j += LANES) {
+      int i = slot_column(p, row, j);
+      const float v = i >= 0 ? load_any(p.t, row * p.ldt + j, p.t_type) : -kInf;
+      if (v == -kInf) i = -1;
+      my_i[j] = i;
+      my_e[j] = v;
+      tm = fmaxf(tm, v);
+      if (i >= 0) some = 1.f;
     }
   }
-  for (int i = pieces * E::kVec + tid; i < p.v; i += THREADS) {
-    const float x = E::load(z, i);
-    if (x > m) { s *= fast_exp2((m - x) * p.c); m = x; }
-    s += x == -kInf ? 0.f : fast_exp2((x - m) * p.c);
-  }
-  {
-    const float mm = block_reduce<THREADS, OpMax>(m, tmp);
-    s = m == mm ? s : s * fast_exp2((m - mm) * p.c);
-    s = m == -kInf && !(s != s) ? 0.f : s;
-    m = mm;
-    s = block_reduce<THREADS, OpSum>(s, tmp2);
-    if (m == -kInf) s = __builtin_nanf("");     // a row of nothing but -inf has no softmax
-  }
+  const float own = m;
+  m = row_reduce<LANES, OpMax>(m, tmp[0]);
+  tm = row_reduce<LANES, OpMax>(tm, tmp[1]);
+  some = row_reduce<LANES, OpMax>(some, tmp[2]);
 
-  // the teacher's slots
-  float tm = -kInf, some = 0.f;
-  for (int j = tid; j < p.k; j += THREADS) {
-    const int i = slot_column(p, row, j);
-    const float t = i >= 0 ? load_any(p.t, row * p.ldt + j, p.t_type) : -kInf;
-    slot_i[j] = i >= 0 && t != -kInf ? i : -1;  // a slot of -inf weighs nothing: empty
-    slot_e[j] = t;
-    if (slot_i[j] >= 0) { tm = fmaxf(tm, t); some = 1.f; }
+  if constexpr (PIECES > 0) {
+    float part[2] = {t < tail ? fast_exp2((last - m) * p.c) : 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < PIECES; ++c)
+      if (t + c * LANES < pieces) {
+        float x[E::kVec];
+        E::unpack(r[c], x);
+#pragma unroll
+        for (int i = 0; i < E::kVec; ++i) part[i & 1] += fast_exp2((x[i] - m) * p.c);
+      }
+    s = part[0] + part[1];
+  } else {
+    // (own == -inf: this thread saw nothing else, s is 0 or NaN)
+    if (own != m && own != -kInf) s *= fast_exp2((own - m) * p.c);
   }
-  tm = block_reduce<THREADS, OpMax>(tm, tmp);
-  some = block_reduce<THREADS, OpMax>(some, tmp2);
-  float A = 0.f, W = 0.f;
-  for (int j = tid; j < p.k; j += THREADS) {
-    const int i = slot_i[j];
-    float e = 0.f;
-    if (i >= 0) {
-      const float a = (slot_e[j] - tm) * p.inv_t;
-      e = expf(a);
-      const float b = (E::load(z, i) - m) * p.inv_t;
+  float A = 0.f, W = 0.f;                                        // sum of exp(a_j), and of exp(a_j) (a_j - b_j)
+  if (i0 >= 0) {
+    const float a = (t0 - tm) * p.inv_t, e = expf(a), b = (z0 - m) * p.inv_t;
+    A = e;
+    if (e != 0.f) W = e * (a - b);
+    my_e[t] = e;
+  }
+  if constexpr (kGroups) my_i[t] = i0;
+  if constexpr (!kGroups)
+    for (int j = t + LANES; j < p.k; j += LANES) {
+      const int i = my_i[j];
+      if (i < 0) continue;
+      const float a = (my_e[j] - tm) * p.inv_t, e = expf(a), b = (E::load(z, i) - m) * p.inv_t;
       A += e;
       if (e != 0.f) W += e * (a - b);
+      my_e[j] = e;
     }
-    slot_e[j] = e;
-  }
-  A = block_reduce<THREADS, OpSum>(A, tmp);
-  W = block_reduce<THREADS, OpSum>(W, tmp2);
-  if (p.loss && tid == 0) p.loss[row] = some > 0.f ? W / A + (logf(s) - logf(A)) : 0.f;
+  s = row_reduce<LANES, OpSum>(s, tmp[3]);
+  A = row_reduce<LANES, OpSum>(A, tmp[4]);
+  W = row_reduce<LANES, OpSum>(W, tmp[5]);
+  if (m == -kInf) s = __builtin_nanf("");                        // a row of nothing but -inf has no softmax
+  if (p.loss && live && t == 0) p.loss[row] = some > 0.f ? W / A + (logf(s) - logf(A)) : 0.f;
   if (!p.dz) return;
 
   char* dz = static_cast<char*>(p.dz) + row * p.ldd * E::kBytes;
-  const float g = some > 0.f ? p.up[row * p.ldu] * p.inv_t : 0.f, coef = g / s;
-  if (!(some > 0.f)) {
-    const u32x4 zero = {0, 0, 0, 0};
-    for (int q = tid; q < pieces; q += THREADS) store16(dz, (long)q * 16, zero);
-    for (int i = pieces * E::kVec + tid; i < p.v; i += THREADS) E::store(dz, i, 0.f);
-    return;
-  }
-  for (int q = tid; q < pieces; q += THREADS * 4) {
-    u32x4 r[4];
+  const bool filled = some > 0.f;
+  const float g = filled ? p.up[row * p.ldu] * p.inv_t : 0.f, coef = filled ? g / s : 0.f;
+  if (live) {
+    auto piece = [&](int q, u32x4 f) {
+      u32x4 o = {0, 0, 0, 0};
+      if (filled) {
+        float x[E::kVec];
+        E::unpack(f, x);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) r[u] = load16(z, (long)min(q + u * THREADS, pieces - 1) * 16);
+        for (int i = 0; i < E::kVec; ++i) x[i] = coef * fast_exp2((x[i] - m) * p.c);
+        o = E::pack(x);
+      }
+      store16(dz, (long)q * 16, o);
+    };
+    if constexpr (PIECES > 0) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (q + u * THREADS >= pieces) break;
-      float x[E::kVec];
-      E::unpack(r[u], x);
+      for (int c = 0; c < PIECES; ++c)
+        if (t + c * LANES < pieces) piece(t + c * LANES, r[c]);
+    } else {
+      for (int q = t; q < pieces; q += LANES * 4) {
+        u32x4 f[4];
 #pragma unroll
-      for (int i = 0; i < E::kVec; ++i) x[i] = coef * fast_exp2((x[i] - m) * p.c);
-      store16(dz, (long)(q + u * THREADS) * 16, E::pack(x));
+        for (int u = 0; u < 4; ++u) f[u] = load16(z, (long)min(q + u * LANES, pieces - 1) * 16);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (q + u * LANES < pieces) piece(q + u * LANES, f[u]);
+      }
     }
+    if (t < tail) E::store(dz, (long)pieces * E::kVec + t, filled ? coef * fast_exp2((last - m) * p.c) : 0.f);
   }
-  for (int i = pieces * E::kVec + tid; i < p.v; i += THREADS) E::store(dz, i, coef * fast_exp2((E::load(z, i) - m) * p.c));
-  __syncthreads();                              // the row stands: the slots' columns are written over it
-  for (int j = tid; j < p.k; j += THREADS) {
-    const int i = slot_i[j];
+  __syncthreads();                                               // the row stands: the slots' columns are written over it
+  if (!live) return;
+  for (int j = t; j < p.k; j += LANES) {
+    const int i = my_i[j];
     if (i < 0) continue;
     float share = 0.f;
     bool first = true;
     for (int l = 0; l < p.k; ++l)
-      if (slot_i[l] == i) {
+      if (my_i[l] == i) {
         if (l < j) first = false;
-        share += slot_e[l];
+        share += my_e[l];
       }
-    if (first) E::store(dz, i, g * (fast_exp2((E::load(z, i) - m) * p.c) / s - share / A));
+    const float zi = j == t ? z0 : E::load(z, i);
+    if (first) E::store(dz, i, g * (fast_exp2((zi - m) * p.c) / s - share / A));
   }
 }
 
+// Threads per row: the fewest that hold it in registers at a few pieces each, and its slots at one each where rows share a
+// workgroup.
 template <class E>
 int launch_distill(const DistillP& p, hipStream_t s) {
-  hipLaunchKernelGGL((distill_row_kernel<E, 256>), dim3((unsigned)p.n), dim3(256), 0, s, p);
+  const int pieces = p.v / E::kVec;
+  auto run = [&](auto lanes, auto held) {
+    constexpr int L = decltype(lanes)::value, P = decltype(held)::value;
+    constexpr int threads = L < 256 ? 256 : L;
+    hipLaunchKernelGGL((distill_kernel<E, L, P>), dim3((unsigned)((p.n + threads / L - 1) / (threads / L))), dim3(threads), 0, s, p);
+  };
+  using std::integral_constant;
+#define OBJ_ROWS(L, P) run(integral_constant<int, L>{}, integral_constant<int, P>{})
+  if (p.k <= 16 && pieces <= 16) OBJ_ROWS(16, 1);
+  else if (p.k <= 16 && pieces <= 32) OBJ_ROWS(16, 2);
+  else if (p.k <= 16 && pieces <= 64) OBJ_ROWS(16, 4);
+  else if (p.k <= 64 && pieces <= 64) OBJ_ROWS(64, 1);
+  else if (p.k <= 64 && pieces <= 128) OBJ_ROWS(64, 2);
+  else if (p.k <= 64 && pieces <= 256) OBJ_ROWS(64, 4);
+  else if (p.k <= 64 && pieces <= 512) OBJ_ROWS(64, 8);
+  else if (pieces <= 1024) OBJ_ROWS(256, 4);
+  else if (pieces <= 2048) OBJ_ROWS(256, 8);
+  else if (pieces <= 4096) OBJ_ROWS(512, 8);
+  else if (pieces <= 8192) OBJ_ROWS(1024, 8);
+  else if (pieces <= 16384) OBJ_ROWS(1024, 16);
+  else OBJ_ROWS(1024, 0);
+#undef OBJ_ROWS
   return check_launch("distill_top");
 }
 
