@@ -78,9 +78,9 @@ __device__ __forceinline__ float load_any(const void* p, long i, int type) {
 struct OpSum { template <class T> static __device__ __forceinline__ T f(T a, T b) { return a + b; } };
 struct OpMax {
   static __device__ __forceinline__ float f(float a, float b) { return fmaxf(a, b); }
-  static __device__ __forceinline__ unsigned f(unsigned a, unsigned b) { return a > b ? a : b; }
+  template <class T> static __device__ __forceinline__ T f(T a, T b) { return a > b ? a : b; }
 };
-struct OpMin { static __device__ __forceinline__ unsigned f(unsigned a, unsigned b) { return a < b ? a : b; } };
+struct OpMin { template <class T> static __device__ __forceinline__ T f(T a, T b) { return a < b ? a : b; } };
 
 template <int CTRL> __device__ __forceinline__ unsigned dpp_u32(unsigned v) {
   return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
