@@ -248,79 +248,241 @@ struct GemmP {
   const float* bias;
   int leaky;
   void* c; long ldc;
+  float* partial;                          // (splits, M, N) sums of a run of blocks each, or null
+  long blocks_per_split;
 };
 
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+typedef __attribute__((address_space(3))) uint8_t lds_byte;
+typedef const __attribute__((address_space(1))) uint8_t global_byte;
 
-__device__ __forceinline__ i32x8 fragment(const uint8_t* p) {
-  const u32x4 lo = *reinterpret_cast<const u32x4*>(p), hi = *reinterpret_cast<const u32x4*>(p + 16);
-  return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
-}
-// 8 elements times their block's scale: exact (4 bits, and bf16 has fp32's exponents)
-__device__ __forceinline__ bf16x8 widened(const uint8_t* p, float scale) {
-  const uint2 v = *reinterpret_cast<const uint2*>(p);
-  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v.x, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v.x, scale, true);
-  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v.y, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v.y, scale, true);
+// 8 elements (two dwords) times their block's scale: exact (4 bits, and bf16 has fp32's exponents)
+__device__ __forceinline__ bf16x8 widened(int lo, int hi, float scale) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 __device__ __forceinline__ float scale_of(unsigned byte) { return __uint_as_float(byte << 23); }
-template <int SEL> __device__ __forceinline__ f32x4 mfma(i32x8 a, i32x8 b, f32x4 c, int sa, int sb) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, SEL, sa, SEL, sb);
+__device__ __forceinline__ float finished(float v, const GemmP& p, float bias) {
+  v += bias;
+  return p.leaky ? fmaxf(v, 0.01f * v) : v;
 }
 
-// A workgroup of four waves per 64 x 64 of C, a wave per 16 rows of C; fragments straight from memory.  The instruction's "A" is b's rows
-// and its "B" a's, so that a lane's four results are four neighbouring columns of one row of C.
-template <class E, bool WIDE>
-__global__ void __launch_bounds__(256) gemm_fp8_kernel(GemmP p) {
-  const long nb = (p.N + 63) / 64;
-  const long m0 = (blockIdx.x / nb) * 64 + (threadIdx.x >> 6) * 16, n0 = (blockIdx.x % nb) * 64;
-  const int lane = threadIdx.x & 63, i = lane & 15, h = lane >> 4;
-  const long m = min(m0 + i, p.M - 1);
-  f32x4 acc[4] = {};
-  for (long k = 0; k < p.K; k += kBlock) {
-    const unsigned sa = p.sa[m * p.ldsa + k / kBlock];
+// Four neighbouring columns of one row of C.
+template <class E> __device__ __forceinline__ void store4(const GemmP& p, long m, long n, f32x4 v) {
+  char* c = static_cast<char*>(p.c) + (m * p.ldc + n) * E::kBytes;
+  if (n + 4 <= p.N) {
+    if (E::kBytes == 4) {
+      *reinterpret_cast<u32x4e*>(c) = u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+    } else {
+      float x[8] = {v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f};
+      const u32x4 o = E::pack(x);
+      typedef unsigned u32x2e __attribute__((ext_vector_type(2), aligned(2)));
+      *reinterpret_cast<u32x2e*>(c) = u32x2e{o[0], o[1]};
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (n + r < p.N) E::store(c, r, v[r]);
+  }
+}
+
+// BM x BN of C per workgroup of WM x WN waves.  A step is one block of 128: BM + BN rows of 128 bytes, moved from memory straight
+// into LDS one step ahead (two slots, one barrier a step).  The 16-byte pieces of a row are permuted by its row number on the way
+// (piece c of row r lies at c ^ (r / 2 mod 8)), so that the 16 rows a fragment is read from fall on different banks; the permutation is
+// done on the addresses the lanes read from, since LDS is filled in order.  The instruction's "A" is b's rows and its "B" a's: a
+// lane's four results are four neighbouring columns of one row of C.
+// A lane's 32 bytes of a fragment are one 32-wide run of the block, in the 8-bit form as in the widened one (whose four
+// instructions take 8 bytes of every lane each: another order of the same sum).
+template <class E, bool WIDE, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 2) gemm_fp8_kernel(GemmP p) {
+  constexpr int kWaves = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, RA = BM / kWaves / 8, RB = BN / kWaves / 8;
+  constexpr int kSlot = (BM + BN) * kBlock;
+  __shared__ __align__(16) uint8_t ring[2 * kSlot + 2 * (BM + BN) * 4];      // one object: the copies' waits stay with the barrier
+  const long mt = (p.M + BM - 1) / BM, nt = (p.N + BN - 1) / BN, tiles = mt * nt;
+  // workgroups go round the 8 XCDs: each XCD takes one run of tiles, in panels of 8 tile rows, so that its L2 serves neighbours
+  long tile = blockIdx.x;
+  {
+    const long xcd = tile % 8, per = tiles / 8, more = tiles % 8;
+    tile = xcd * per + min(xcd, more) + tile / 8;
+  }
+  const long panel = tile / (8 * nt), rows = min(mt - panel * 8, 8l), in = tile - panel * 8 * nt;
+  const long m0 = (panel * 8 + in % rows) * BM, n0 = in / rows * BN;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, h = lane >> 4;
+  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+  const long first = blockIdx.y * p.blocks_per_split, steps = min(p.blocks_per_split, p.K / kBlock - first);
+
+  // this lane's part of the copies: row lane / 8 of every 8, piece lane % 8 of LDS
+  const long arow = min(m0 + wave * RA * 8, p.M - 1), brow = min(n0 + wave * RB * 8, p.N - 1);
+  const uint8_t* abase = p.a + arow * p.lda + first * kBlock;
+  const uint8_t* bbase = p.b + brow * p.ldb + first * kBlock;
+  unsigned aoff[RA], boff[RB];
+#pragma unroll
+  for (int c = 0; c < RA; ++c) {
+    const int r = wave * RA * 8 + c * 8 + lane / 8;
+    aoff[c] = (unsigned)((min(m0 + r, p.M - 1) - arow) * p.lda) + (((lane & 7) ^ (r >> 1 & 7)) << 4);
+  }
+#pragma unroll
+  for (int c = 0; c < RB; ++c) {
+    const int r = wave * RB * 8 + c * 8 + lane / 8;
+    boff[c] = (unsigned)((min(n0 + r, p.N - 1) - brow) * p.ldb) + (((lane & 7) ^ (r >> 1 & 7)) << 4);
+  }
+  lds_byte* const lds = (lds_byte*)ring;
+  auto copy = [&](long step) {
+    lds_byte* slot = lds + (step & 1) * kSlot + wave * RA * 1024;
+#pragma unroll
+    for (int c = 0; c < RA; ++c)
+      __builtin_amdgcn_global_load_lds((global_byte*)(abase + step * kBlock + aoff[c]), (__attribute__((address_space(3))) void*)(slot + c * 1024), 16, 0, 0);
+    slot = lds + (step & 1) * kSlot + BM * kBlock + wave * RB * 1024;
+#pragma unroll
+    for (int c = 0; c < RB; ++c)
+      __builtin_amdgcn_global_load_lds((global_byte*)(bbase + step * kBlock + boff[c]), (__attribute__((address_space(3))) void*)(slot + c * 1024), 16, 0, 0);
+  };
+  // scales: a dword of each row, four steps' worth, two slots behind the rows'; a wave copies those of 64 rows
+  constexpr int kScaleWaves = (BM + BN) / 64;
+  static_assert(kScaleWaves <= kWaves, "one copy per wave");
+  const bool of_a = wave < BM / 64;
+  const long srow = of_a ? min(m0 + wave * 64 + lane, p.M - 1) : min(n0 + (wave - BM / 64) * 64 + lane, p.N - 1);
+  const uint8_t* const sfrom = of_a ? p.sa + srow * p.ldsa : p.sb + srow * p.ldsb;
+  auto scales = [&](long step) {
+    const long group = (first + step) >> 2;
+    if (wave < kScaleWaves)
+      __builtin_amdgcn_global_load_lds((global_byte*)(sfrom + group * 4), (__attribute__((address_space(3))) void*)(lds + 2 * kSlot + ((group & 1) * (BM + BN) + wave * 64) * 4), 4, 0, 0);
+  };
+  auto fragment = [&](const lds_byte* rows_, int r) {
+    const int key = r >> 1 & 7;
+    const u32x4 lo = *(const __attribute__((address_space(3))) u32x4*)(rows_ + r * kBlock + ((h * 2 ^ key) << 4));
+    const u32x4 hi = *(const __attribute__((address_space(3))) u32x4*)(rows_ + r * kBlock + ((h * 2 + 1 ^ key) << 4));
+    return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+  };
+
+  f32x4 acc[TM][TN] = {};
+  if (steps > 0) {
+    copy(0);
+    scales(0);
+  }
+  for (long step = 0; step < steps; ++step) {
+    __syncthreads();                                             // the step's rows have landed; the other slot has been read
+    const int turn = (int)((first + step) & 3);
+    if (step + 1 < steps) {
+      copy(step + 1);
+      if (turn == 3) scales(step + 1);
+    }
+    const lds_byte* const scale_a = lds + 2 * kSlot + (((first + step) >> 2 & 1) * (BM + BN) + wm + i) * 4 + turn;
+    const lds_byte* const scale_b = scale_a + (BM + wn - wm) * 4;
+    int sa[TM];
+#pragma unroll
+    for (int t = 0; t < TM; ++t) sa[t] = scale_a[t * 64];
+    const lds_byte* rows_a = lds + (step & 1) * kSlot + wm * kBlock;
+    const lds_byte* rows_b = lds + (step & 1) * kSlot + (BM + wn) * kBlock;
+    i32x8 fa[TM];
+#pragma unroll
+    for (int t = 0; t < TM; ++t) fa[t] = fragment(rows_a, t * 16 + i);
     if constexpr (WIDE) {
+      i32x8 fb[TN];
+#pragma unroll
+      for (int t = 0; t < TN; ++t) fb[t] = fragment(rows_b, t * 16 + i);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const bf16x8 fa = widened(p.a + m * p.lda + k + q * 32 + h * 8, scale_of(sa));
+        bf16x8 xa[TM];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const long n = min(n0 + t * 16 + i, p.N - 1);
-          const bf16x8 fb = widened(p.b + n * p.ldb + k + q * 32 + h * 8, scale_of(p.sb[n * p.ldsb + k / kBlock]));
-          acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb, fa, acc[t], 0, 0, 0);
+        for (int t = 0; t < TM; ++t) xa[t] = widened(fa[t][2 * q], fa[t][2 * q + 1], scale_of(sa[t]));
+#pragma unroll
+        for (int t = 0; t < TN; ++t) {
+          const bf16x8 xb = widened(fb[t][2 * q], fb[t][2 * q + 1], scale_of(scale_b[t * 64]));
+#pragma unroll
+          for (int u = 0; u < TM; ++u) acc[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb, xa[u], acc[u][t], 0, 0, 0);
         }
       }
     } else {
-      const i32x8 fa = fragment(p.a + m * p.lda + k + h * 32);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const long n = min(n0 + t * 16 + i, p.N - 1);
-        acc[t] = mfma<0>(fragment(p.b + n * p.ldb + k + h * 32), fa, acc[t], (int)p.sb[n * p.ldsb + k / kBlock], (int)sa);
+      for (int t = 0; t < TN; ++t) {
+        const i32x8 fb = fragment(rows_b, t * 16 + i);
+        const int s = scale_b[t * 64];
+#pragma unroll
+        for (int u = 0; u < TM; ++u)
+          acc[u][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb, fa[u], acc[u][t], 0, 0, 0, s, 0, sa[u]);
       }
     }
   }
-  if (m0 + i >= p.M) return;
-  char* c = static_cast<char*>(p.c) + (m0 + i) * p.ldc * E::kBytes;
+
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < TN; ++t) {
+    const long n = n0 + wn + t * 16 + h * 4;
+    if (n >= p.N) continue;
+    float bias[4] = {0.f, 0.f, 0.f, 0.f};
+    if (p.bias && !p.partial)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const long n = n0 + t * 16 + h * 4 + r;
-      if (n >= p.N) continue;
-      float v = acc[t][r] + (p.bias ? p.bias[n] : 0.f);
-      if (p.leaky) v = fmaxf(v, 0.01f * v);
-      E::store(c, n, v);
+      for (int r = 0; r < 4; ++r) bias[r] = n + r < p.N ? p.bias[n + r] : 0.f;
+#pragma unroll
+    for (int u = 0; u < TM; ++u) {
+      const long m = m0 + wm + u * 16 + i;
+      if (m >= p.M) continue;
+      if (p.partial) {
+        float* o = p.partial + ((long)blockIdx.y * p.M + m) * p.N + n;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (n + r < p.N) o[r] = acc[u][t][r];
+        continue;
+      }
+      f32x4 v;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = finished(acc[u][t][r], p, bias[r]);
+      store4<E>(p, m, n, v);
     }
+  }
+}
+
+// C from the partial sums of the splits, in their order
+template <class E>
+__global__ void __launch_bounds__(256) join_splits_kernel(GemmP p, int splits) {
+  const long groups = (p.N + 3) / 4, at = (long)blockIdx.x * 256 + threadIdx.x;
+  if (at >= p.M * groups) return;
+  const long m = at / groups, n = (at - m * groups) * 4;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < splits; ++s) {
+    const float* o = p.partial + ((long)s * p.M + m) * p.N + n;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (n + r < p.N) v[r] += o[r];
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v[r] = finished(v[r], p, p.bias && n + r < p.N ? p.bias[n + r] : 0.f);
+  store4<E>(p, m, n, v);
+}
+
+// Tile and split of a product.  256 x 256 per workgroup (one per CU, 128 KB of LDS) where such tiles fill the card and the sum is long
+// enough to run behind its copies; else 128 x 128 (two per CU), with the sum split where there are fewer tiles than places.
+struct Plan { bool big; int splits; long blocks; };
+inline Plan plan_of(long M, long N, long K, bool wide) {
+  const long blocks = K / kBlock;
+  if (!wide && blocks >= 8 && ((M + 255) / 256) * ((N + 255) / 256) >= 224) return Plan{true, 1, blocks};
+  const long tiles = ((M + 127) / 128) * ((N + 127) / 128);
+  long splits = tiles >= 256 ? 1 : 512 / tiles;                  // two workgroups per CU
+  splits = splits < blocks / 4 ? splits : blocks / 4;            // of at least four blocks each
+  if (splits < 2) return Plan{false, 1, blocks};
+  const long per = (blocks + splits - 1) / splits;
+  return Plan{false, (int)((blocks + per - 1) / per), per};
 }
 
 template <class E>
-int launch_gemm_fp8(const GemmP& p, hipStream_t s) {
-  const long tiles = ((p.M + 63) / 64) * ((p.N + 63) / 64);
-  hipLaunchKernelGGL((gemm_fp8_kernel<E, E::kBytes == 4>), dim3((unsigned)tiles), dim3(256), 0, s, p);
+int launch_gemm_fp8(GemmP p, float* workspace, hipStream_t s) {
+  constexpr bool wide = E::kBytes == 4;
+  const Plan plan = plan_of(p.M, p.N, p.K, wide);
+  p.blocks_per_split = plan.blocks;
+  p.partial = plan.splits > 1 ? workspace : nullptr;
+  if (plan.big) {
+    if constexpr (!wide)
+      hipLaunchKernelGGL((gemm_fp8_kernel<E, false, 256, 256, 2, 4>), dim3((unsigned)(((p.M + 255) / 256) * ((p.N + 255) / 256))), dim3(512), 0, s, p);
+  } else {
+    hipLaunchKernelGGL((gemm_fp8_kernel<E, wide, 128, 128, 2, 2>), dim3((unsigned)(((p.M + 127) / 128) * ((p.N + 127) / 128)), (unsigned)plan.splits), dim3(256), 0, s, p);
+  }
+  if (plan.splits > 1)
+    hipLaunchKernelGGL((join_splits_kernel<E>), dim3((unsigned)((p.M * ((p.N + 3) / 4) + 255) / 256)), dim3(256), 0, s, p, plan.splits);
   return check_launch("gemm_fp8");
 }
 
-constexpr int64_t kMaxSize = 1ll << 31;
+constexpr int64_t kMaxSize = 1ll << 31, kMaxK = 1ll << 26;     // 32 rows of kMaxK bytes: 32-bit offsets in a wave's copies
 
 }  // namespace
 }  // namespace objnerf
@@ -356,20 +518,27 @@ int objnerf_fp8_quantize(const objnerf_fp8_quantize_args* a, void* stream) {
                                         : launch_quantize<ElemF16>(p, square, a->column_sums, s);
 }
 
+int64_t objnerf_gemm_fp8_workspace_floats(int64_t M, int64_t N, int64_t K, int c_type) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const Plan plan = plan_of(M, N, K, c_type == OBJNERF_TYPE_F32);
+  return plan.splits > 1 ? plan.splits * M * N : 0;
+}
+
 int objnerf_gemm_fp8(const objnerf_gemm_fp8_args* a, void* stream) {
   if (!a) return set_error(-1, "gemm_fp8: no arguments");
-  if (a->M < 0 || a->N < 0 || a->K < 0 || a->M >= kMaxSize || a->N >= kMaxSize || a->K >= kMaxSize || a->K % kBlock)
-    return set_error(-1, "gemm_fp8: bad sizes (M, N, K < 2^31, K a multiple of 128)");
+  if (a->M < 0 || a->N < 0 || a->K < 0 || a->M >= kMaxSize || a->N >= kMaxSize || a->K > kMaxK || a->K % kBlock)
+    return set_error(-1, "gemm_fp8: bad sizes (M, N < 2^31, K <= 2^26, K a multiple of 128)");
   if (!label_type_ok(a->c_type)) return set_error(-1, "gemm_fp8: unknown element type");
-  if ((a->K && (a->a_stride < a->K || a->b_stride < a->K || a->a_stride % 16 || a->b_stride % 16)) || a->c_stride < a->N)
-    return set_error(-1, "gemm_fp8: bad strides (operands: multiples of 16, at least K)");
+  if ((a->K && (a->a_stride < a->K || a->b_stride < a->K || a->a_stride % 16 || a->b_stride % 16 || a->a_stride > kMaxK || a->b_stride > kMaxK)) || a->c_stride < a->N)
+    return set_error(-1, "gemm_fp8: bad strides (operands: multiples of 16, at least K, at most 2^26)");
   const int64_t nb = a->K / kBlock;
   if (a->K && (a->a_scale_stride < nb || a->b_scale_stride < nb || a->a_scale_stride % 4 || a->b_scale_stride % 4))
     return set_error(-1, "gemm_fp8: bad scale strides (multiples of 4, at least K / 128)");
   if (((uintptr_t)a->a | (uintptr_t)a->b) & 15 || ((uintptr_t)a->a_scale | (uintptr_t)a->b_scale) & 3)
     return set_error(-1, "gemm_fp8: operands must be 16-byte, scales 4-byte aligned");
   if (a->M == 0 || a->N == 0) return 0;
-  if (((a->M + 63) / 64) > INT32_MAX / ((a->N + 63) / 64)) return set_error(-1, "gemm_fp8: more than 2^31 tiles");
+  if (((a->M + 127) / 128) > (1 << 30) / ((a->N + 127) / 128)) return set_error(-1, "gemm_fp8: more than 2^30 tiles");
+  if (objnerf_gemm_fp8_workspace_floats(a->M, a->N, a->K, a->c_type) && !a->workspace) return set_error(-1, "gemm_fp8: a workspace is needed");
   if (!a->c || (a->K && (!a->a || !a->b || !a->a_scale || !a->b_scale))) return set_error(-1, "gemm_fp8: a needed buffer is missing");
   GemmP p;
   p.M = a->M; p.N = a->N; p.K = a->K;
@@ -377,9 +546,10 @@ int objnerf_gemm_fp8(const objnerf_gemm_fp8_args* a, void* stream) {
   p.b = a->b; p.ldb = a->b_stride; p.sb = a->b_scale; p.ldsb = a->b_scale_stride;
   p.bias = a->bias; p.leaky = a->leaky;
   p.c = a->c; p.ldc = a->c_stride;
+  p.partial = nullptr; p.blocks_per_split = 0;
   hipStream_t s = (hipStream_t)stream;
-  return a->c_type == OBJNERF_TYPE_F32 ? launch_gemm_fp8<ElemF32>(p, s)
-         : a->c_type == OBJNERF_TYPE_BF16 ? launch_gemm_fp8<ElemBf16>(p, s) : launch_gemm_fp8<ElemF16>(p, s);
+  return a->c_type == OBJNERF_TYPE_F32 ? launch_gemm_fp8<ElemF32>(p, a->workspace, s)
+         : a->c_type == OBJNERF_TYPE_BF16 ? launch_gemm_fp8<ElemBf16>(p, a->workspace, s) : launch_gemm_fp8<ElemF16>(p, a->workspace, s);
 }
 
 }  // extern "C"

@@ -117,8 +117,13 @@ def _product(a, b, bias, leaky, out_dtype):
     if bias is not None:
         g.bias = bias.data_ptr()
     g.leaky, g.c_type, g.c, g.c_stride = int(leaky), _TYPES[out_dtype], out.data_ptr(), n
+    lib = _lib.lib()
+    floats = lib.objnerf_gemm_fp8_workspace_floats(m, n, g.K, g.c_type)
+    if floats:
+        work = torch.empty(floats, dtype=torch.float32, device=dev)
+        g.workspace = work.data_ptr()
     if m and n:
-        _call(_lib.lib().objnerf_gemm_fp8, g, dev, "gemm_fp8")
+        _call(lib.objnerf_gemm_fp8, g, dev, "gemm_fp8")
     return out
 
 
