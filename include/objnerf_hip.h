@@ -666,7 +666,10 @@ typedef struct {
   const float* top_p_rows; double top_p;
   const float* min_p_rows; double min_p;
   int64_t* labels;           /* (n) */
+  void* workspace;           /* objnerf_sample_logits_workspace_bytes() (0: may be NULL), 8-byte aligned: few long rows are spread
+                              * over several workgroups; not to be shared by calls that may run at the same time */
 } objnerf_sample_args;
+int64_t objnerf_sample_logits_workspace_bytes(int64_t n, int32_t v, int type);
 int objnerf_sample_logits(const objnerf_sample_args* args, void* stream);
 
 /* Products in 8-bit floating point (OCP e4m3) with a scale for each block of 128.

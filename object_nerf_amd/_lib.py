@@ -194,7 +194,7 @@ class SampleArgs(C.Structure):
         ("top_k_rows", C.c_void_p), ("top_k", C.c_int64),
         ("top_p_rows", C.c_void_p), ("top_p", C.c_double),
         ("min_p_rows", C.c_void_p), ("min_p", C.c_double),
-        ("labels", C.c_void_p),
+        ("labels", C.c_void_p), ("workspace", C.c_void_p),
     ]
 
 
@@ -289,6 +289,7 @@ SIGNATURES = {
     "objnerf_fp8_quantize": (C.c_int, [C.POINTER(Fp8QuantizeArgs), _VP]),
     "objnerf_gemm_fp8_workspace_floats": (C.c_int64, [C.c_int64, C.c_int64, C.c_int64, C.c_int]),
     "objnerf_gemm_fp8": (C.c_int, [C.POINTER(GemmFp8Args), _VP]),
+    "objnerf_sample_logits_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int32, C.c_int]),
     "objnerf_sample_logits": (C.c_int, [C.POINTER(SampleArgs), _VP]),
     "objnerf_timing_enable": (C.c_int, [C.c_int]),
     "objnerf_timing_read": (C.c_int, [C.POINTER(C.c_int64), C.POINTER(C.c_double)]),

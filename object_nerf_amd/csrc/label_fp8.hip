@@ -20,6 +20,7 @@
 // number of blocks filled up to a multiple of 4 (with 127): one aligned dword holds four blocks' scales, the instruction's op_sel
 // picks the byte.  Blocks of 128 x 128 repeat their scale in 128 rows: a 128th of the values' bytes buys one form for all.
 #include "host_api.h"
+#include "device_math.h"
 #include "label_ops.h"
 
 namespace objnerf {
@@ -27,7 +28,6 @@ namespace {
 
 constexpr int kBlock = 128;
 using i32x8 = __attribute__((ext_vector_type(8))) int;
-using f32x4 = __attribute__((ext_vector_type(4))) float;
 
 // largest finite |x| of a block -> its scale byte
 __device__ __forceinline__ unsigned scale_byte(float largest) {
@@ -268,18 +268,26 @@ __device__ __forceinline__ float finished(float v, const GemmP& p, float bias) {
   return p.leaky ? fmaxf(v, 0.01f * v) : v;
 }
 
+// Where piece c of a row lies in LDS: at c ^ piece_key(row).  Rows are 32 banks apart, so that 16 rows of a fragment need their eight pairs
+// on eight different pieces; and the hardware serves a 16-byte read not in runs of 16 lanes but, e.g., lanes 0-3, 12-15 and 20-27
+// together: rows 0-3 and 12-15 of piece c with rows 4-11 of piece c + 2.  Keys 0 2 | 1 3 5 7 | 4 6 keep both apart.
+__device__ __forceinline__ int piece_key(int row) { return 0x64753120 >> ((row >> 1 & 7) * 4) & 7; }
+
 // Four neighbouring columns of one row of C.
+template <class E> __device__ __forceinline__ void write4(char* c, f32x4 v) {
+  if (E::kBytes == 4) {
+    *reinterpret_cast<u32x4e*>(c) = u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+  } else {
+    float x[8] = {v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f};
+    const u32x4 o = E::pack(x);
+    typedef unsigned u32x2e __attribute__((ext_vector_type(2), aligned(2)));
+    *reinterpret_cast<u32x2e*>(c) = u32x2e{o[0], o[1]};
+  }
+}
 template <class E> __device__ __forceinline__ void store4(const GemmP& p, long m, long n, f32x4 v) {
   char* c = static_cast<char*>(p.c) + (m * p.ldc + n) * E::kBytes;
   if (n + 4 <= p.N) {
-    if (E::kBytes == 4) {
-      *reinterpret_cast<u32x4e*>(c) = u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
-    } else {
-      float x[8] = {v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f};
-      const u32x4 o = E::pack(x);
-      typedef unsigned u32x2e __attribute__((ext_vector_type(2), aligned(2)));
-      *reinterpret_cast<u32x2e*>(c) = u32x2e{o[0], o[1]};
-    }
+    write4<E>(c, v);
   } else {
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -287,101 +295,176 @@ template <class E> __device__ __forceinline__ void store4(const GemmP& p, long m
   }
 }
 
-// BM x BN of C per workgroup of WM x WN waves.  A step is one block of 128: BM + BN rows of 128 bytes, moved from memory straight
-// into LDS one step ahead (two slots, one barrier a step).  The 16-byte pieces of a row are permuted by its row number on the way
-// (piece c of row r lies at c ^ (r / 2 mod 8)), so that the 16 rows a fragment is read from fall on different banks; the permutation is
-// done on the addresses the lanes read from, since LDS is filled in order.  The instruction's "A" is b's rows and its "B" a's: a
-// lane's four results are four neighbouring columns of one row of C.
-// A lane's 32 bytes of a fragment are one 32-wide run of the block, in the 8-bit form as in the widened one (whose four
-// instructions take 8 bytes of every lane each: another order of the same sum).
-template <class E, bool WIDE, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 2) gemm_fp8_kernel(GemmP p) {
-  constexpr int kWaves = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, RA = BM / kWaves / 8, RB = BN / kWaves / 8;
-  constexpr int kSlot = (BM + BN) * kBlock;
-  __shared__ __align__(16) uint8_t ring[2 * kSlot + 2 * (BM + BN) * 4];      // one object: the copies' waits stay with the barrier
+// Which BM x BN of C a workgroup has.  Workgroups go round the 8 XCDs: each XCD takes one run of tiles, in panels of 8 tile rows, so that
+// its L2 serves neighbours.
+template <int BM, int BN> __device__ __forceinline__ void tile_of(const GemmP& p, long& m0, long& n0) {
   const long mt = (p.M + BM - 1) / BM, nt = (p.N + BN - 1) / BN, tiles = mt * nt;
-  // workgroups go round the 8 XCDs: each XCD takes one run of tiles, in panels of 8 tile rows, so that its L2 serves neighbours
-  long tile = blockIdx.x;
-  {
-    const long xcd = tile % 8, per = tiles / 8, more = tiles % 8;
-    tile = xcd * per + min(xcd, more) + tile / 8;
-  }
+  const long xcd = blockIdx.x % 8, per = tiles / 8, more = tiles % 8;
+  const long tile = xcd * per + min(xcd, more) + blockIdx.x / 8;
   const long panel = tile / (8 * nt), rows = min(mt - panel * 8, 8l), in = tile - panel * 8 * nt;
-  const long m0 = (panel * 8 + in % rows) * BM, n0 = in / rows * BN;
+  m0 = (panel * 8 + in % rows) * BM;
+  n0 = in / rows * BN;
+}
+
+// The copies of a workgroup's rows from memory straight into LDS.  A step is one block of 128: BM + BN rows of 128 bytes into one of two
+// slots.  The 16-byte pieces of a row are permuted (piece_key) on the addresses the lanes read from, since LDS is filled in order.  Scales:
+// a dword of each row, four steps' worth, into two slots of their own; a wave copies those of 64 rows.
+template <int BM, int BN, int WAVES> struct Copies {
+  static constexpr int kSlot = (BM + BN) * kBlock, kBytes = 2 * kSlot + 2 * (BM + BN) * 4;
+  static constexpr int RA = BM / WAVES / 8, RB = BN / WAVES / 8, kScaleCopies = (BM + BN) / 64 / WAVES;
+  static_assert((BM + BN) / 64 % WAVES == 0, "whole copies of 64 rows' scales per wave");
+  const uint8_t *abase, *bbase, *sbase[kScaleCopies];
+  unsigned aoff[RA], boff[RB];
+  long first;
+  lds_byte* lds;
+  __device__ __forceinline__ Copies(const GemmP& p, long m0, long n0, long first_block, lds_byte* ring) : first(first_block), lds(ring) {
+    const int lane = threadIdx.x & 63, wave = uni((int)(threadIdx.x >> 6));
+    // this lane's part: row lane / 8 of every 8, piece lane % 8 of LDS
+    const long arow = min(m0 + wave * RA * 8, p.M - 1), brow = min(n0 + wave * RB * 8, p.N - 1);
+    abase = p.a + arow * p.lda + first * kBlock;
+    bbase = p.b + brow * p.ldb + first * kBlock;
+#pragma unroll
+    for (int c = 0; c < RA; ++c) {
+      const int r = wave * RA * 8 + c * 8 + lane / 8;
+      aoff[c] = (unsigned)((min(m0 + r, p.M - 1) - arow) * p.lda) + (((lane & 7) ^ piece_key(r)) << 4);
+    }
+#pragma unroll
+    for (int c = 0; c < RB; ++c) {
+      const int r = wave * RB * 8 + c * 8 + lane / 8;
+      boff[c] = (unsigned)((min(n0 + r, p.N - 1) - brow) * p.ldb) + (((lane & 7) ^ piece_key(r)) << 4);
+    }
+#pragma unroll
+    for (int c = 0; c < kScaleCopies; ++c) {
+      const int r = (wave * kScaleCopies + c) * 64 + lane;
+      sbase[c] = r < BM ? p.sa + min(m0 + r, p.M - 1) * p.ldsa : p.sb + min(n0 + r - BM, p.N - 1) * p.ldsb;
+    }
+  }
+  __device__ __forceinline__ void rows(long step) const {
+    const int wave = uni((int)(threadIdx.x >> 6));
+    lds_byte* slot = lds + (int)(step & 1) * kSlot + wave * RA * 1024;
+    const uint8_t* from = abase + step * kBlock;
+#pragma unroll
+    for (int c = 0; c < RA; ++c)
+      __builtin_amdgcn_global_load_lds((global_byte*)(from + aoff[c]), (__attribute__((address_space(3))) void*)(slot + c * 1024), 16, 0, 0);
+    slot = lds + (int)(step & 1) * kSlot + BM * kBlock + wave * RB * 1024;
+    from = bbase + step * kBlock;
+#pragma unroll
+    for (int c = 0; c < RB; ++c)
+      __builtin_amdgcn_global_load_lds((global_byte*)(from + boff[c]), (__attribute__((address_space(3))) void*)(slot + c * 1024), 16, 0, 0);
+  }
+  __device__ __forceinline__ void scales(long step) const {
+    const int wave = uni((int)(threadIdx.x >> 6));
+    const long group = (first + step) >> 2;
+#pragma unroll
+    for (int c = 0; c < kScaleCopies; ++c)
+      __builtin_amdgcn_global_load_lds((global_byte*)(sbase[c] + group * 4), (__attribute__((address_space(3))) void*)(lds + 2 * kSlot + ((int)(group & 1) * (BM + BN) + (wave * kScaleCopies + c) * 64) * 4), 4, 0, 0);
+  }
+  // scale byte of row 0 of the tile in this step; rows are 4 bytes apart, b's rows behind a's
+  __device__ __forceinline__ const lds_byte* scale_at(long step) const {
+    const long at = first + step;
+    return lds + 2 * kSlot + ((int)(at >> 2 & 1) * (BM + BN)) * 4 + (int)(at & 3);
+  }
+};
+// a lane's 32 bytes of a fragment: row i of the 16 rows at `rows`, the h-th run of 32 of the block
+__device__ __forceinline__ i32x8 fragment(const lds_byte* rows, int i, int h) {
+  const int key = piece_key(i);
+  const u32x4 lo = *(const __attribute__((address_space(3))) u32x4*)(rows + i * kBlock + ((h * 2 ^ key) << 4));
+  const u32x4 hi = *(const __attribute__((address_space(3))) u32x4*)(rows + i * kBlock + (((h * 2 + 1) ^ key) << 4));
+  return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+}
+__device__ __forceinline__ f32x4 mfma8(i32x8 b, i32x8 a, f32x4 c, int sb, int sa) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, 0, 0, 0, sb, 0, sa);
+}
+
+// A wave's TM x TN tiles of 16 x 16 to memory: lane (i, h) holds columns 4 h .. 4 h + 3 of row i of each.
+template <class E, int TM, int TN>
+__device__ __forceinline__ void write_tile(const GemmP& p, long m0, long n0, bool whole, const f32x4 (&acc)[TM][TN]) {
+  const int i = threadIdx.x & 15, h = threadIdx.x >> 4 & 3;
+  if (!p.partial && whole) {                                     // no questions
+    char* c = static_cast<char*>(p.c) + ((m0 + i) * p.ldc + n0 + h * 4) * E::kBytes;
+    const long down = 16 * p.ldc * E::kBytes;
+#pragma unroll
+    for (int u = 0; u < TM; ++u, c += down)
+#pragma unroll
+      for (int t = 0; t < TN; ++t) {
+        float bias[4] = {0.f, 0.f, 0.f, 0.f};
+        if (p.bias)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) bias[r] = p.bias[n0 + t * 16 + h * 4 + r];
+        f32x4 v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = finished(acc[u][t][r], p, bias[r]);
+        write4<E>(c + t * 16 * E::kBytes, v);
+      }
+    return;
+  }
+#pragma unroll
+  for (int t = 0; t < TN; ++t) {
+    const long n = n0 + t * 16 + h * 4;
+    if (n >= p.N) continue;
+    float bias[4] = {0.f, 0.f, 0.f, 0.f};
+    if (p.bias && !p.partial)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) bias[r] = n + r < p.N ? p.bias[n + r] : 0.f;
+#pragma unroll
+    for (int u = 0; u < TM; ++u) {
+      const long m = m0 + u * 16 + i;
+      if (m >= p.M) continue;
+      if (p.partial) {
+        float* o = p.partial + ((long)blockIdx.y * p.M + m) * p.N + n;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (n + r < p.N) o[r] = acc[u][t][r];
+        continue;
+      }
+      f32x4 v;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = finished(acc[u][t][r], p, bias[r]);
+      store4<E>(p, m, n, v);
+    }
+  }
+}
+
+// BM x BN of C per workgroup of WM x WN waves, rows copied one step ahead, one barrier a step.  The instruction's "A" is b's rows and its
+// "B" a's: a lane's four results are four neighbouring columns of one row of C.  In the widened form the four instructions of a
+// block take 8 bytes of every lane's 32 each: another order of the same sum.
+template <class E, bool WIDE, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(WM * WN * 64, 2) gemm_fp8_kernel(GemmP p) {
+  using Copy = Copies<BM, BN, WM * WN>;
+  constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
+  __shared__ __align__(16) uint8_t ring[Copy::kBytes];           // one object: the copies' waits stay with the barrier
+  long m0, n0;
+  tile_of<BM, BN>(p, m0, n0);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, h = lane >> 4;
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
   const long first = blockIdx.y * p.blocks_per_split, steps = min(p.blocks_per_split, p.K / kBlock - first);
-
-  // this lane's part of the copies: row lane / 8 of every 8, piece lane % 8 of LDS
-  const long arow = min(m0 + wave * RA * 8, p.M - 1), brow = min(n0 + wave * RB * 8, p.N - 1);
-  const uint8_t* abase = p.a + arow * p.lda + first * kBlock;
-  const uint8_t* bbase = p.b + brow * p.ldb + first * kBlock;
-  unsigned aoff[RA], boff[RB];
-#pragma unroll
-  for (int c = 0; c < RA; ++c) {
-    const int r = wave * RA * 8 + c * 8 + lane / 8;
-    aoff[c] = (unsigned)((min(m0 + r, p.M - 1) - arow) * p.lda) + (((lane & 7) ^ (r >> 1 & 7)) << 4);
-  }
-#pragma unroll
-  for (int c = 0; c < RB; ++c) {
-    const int r = wave * RB * 8 + c * 8 + lane / 8;
-    boff[c] = (unsigned)((min(n0 + r, p.N - 1) - brow) * p.ldb) + (((lane & 7) ^ (r >> 1 & 7)) << 4);
-  }
-  lds_byte* const lds = (lds_byte*)ring;
-  auto copy = [&](long step) {
-    lds_byte* slot = lds + (step & 1) * kSlot + wave * RA * 1024;
-#pragma unroll
-    for (int c = 0; c < RA; ++c)
-      __builtin_amdgcn_global_load_lds((global_byte*)(abase + step * kBlock + aoff[c]), (__attribute__((address_space(3))) void*)(slot + c * 1024), 16, 0, 0);
-    slot = lds + (step & 1) * kSlot + BM * kBlock + wave * RB * 1024;
-#pragma unroll
-    for (int c = 0; c < RB; ++c)
-      __builtin_amdgcn_global_load_lds((global_byte*)(bbase + step * kBlock + boff[c]), (__attribute__((address_space(3))) void*)(slot + c * 1024), 16, 0, 0);
-  };
-  // scales: a dword of each row, four steps' worth, two slots behind the rows'; a wave copies those of 64 rows
-  constexpr int kScaleWaves = (BM + BN) / 64;
-  static_assert(kScaleWaves <= kWaves, "one copy per wave");
-  const bool of_a = wave < BM / 64;
-  const long srow = of_a ? min(m0 + wave * 64 + lane, p.M - 1) : min(n0 + (wave - BM / 64) * 64 + lane, p.N - 1);
-  const uint8_t* const sfrom = of_a ? p.sa + srow * p.ldsa : p.sb + srow * p.ldsb;
-  auto scales = [&](long step) {
-    const long group = (first + step) >> 2;
-    if (wave < kScaleWaves)
-      __builtin_amdgcn_global_load_lds((global_byte*)(sfrom + group * 4), (__attribute__((address_space(3))) void*)(lds + 2 * kSlot + ((group & 1) * (BM + BN) + wave * 64) * 4), 4, 0, 0);
-  };
-  auto fragment = [&](const lds_byte* rows_, int r) {
-    const int key = r >> 1 & 7;
-    const u32x4 lo = *(const __attribute__((address_space(3))) u32x4*)(rows_ + r * kBlock + ((h * 2 ^ key) << 4));
-    const u32x4 hi = *(const __attribute__((address_space(3))) u32x4*)(rows_ + r * kBlock + ((h * 2 + 1 ^ key) << 4));
-    return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
-  };
+  const Copy copy(p, m0, n0, first, (lds_byte*)ring);
 
   f32x4 acc[TM][TN] = {};
   if (steps > 0) {
-    copy(0);
-    scales(0);
+    copy.rows(0);
+    copy.scales(0);
   }
   for (long step = 0; step < steps; ++step) {
     __syncthreads();                                             // the step's rows have landed; the other slot has been read
-    const int turn = (int)((first + step) & 3);
     if (step + 1 < steps) {
-      copy(step + 1);
-      if (turn == 3) scales(step + 1);
+      copy.rows(step + 1);
+      if (((first + step) & 3) == 3) copy.scales(step + 1);
     }
-    const lds_byte* const scale_a = lds + 2 * kSlot + (((first + step) >> 2 & 1) * (BM + BN) + wm + i) * 4 + turn;
-    const lds_byte* const scale_b = scale_a + (BM + wn - wm) * 4;
+    const lds_byte* const rows_a = copy.lds + (step & 1) * Copy::kSlot + wm * kBlock;
+    const lds_byte* const rows_b = copy.lds + (step & 1) * Copy::kSlot + (BM + wn) * kBlock;
+    const lds_byte* const scale_a = copy.scale_at(step) + (wm + i) * 4;
+    const lds_byte* const scale_b = copy.scale_at(step) + (BM + wn + i) * 4;
+    i32x8 fa[TM];
     int sa[TM];
 #pragma unroll
     for (int t = 0; t < TM; ++t) sa[t] = scale_a[t * 64];
-    const lds_byte* rows_a = lds + (step & 1) * kSlot + wm * kBlock;
-    const lds_byte* rows_b = lds + (step & 1) * kSlot + (BM + wn) * kBlock;
-    i32x8 fa[TM];
 #pragma unroll
-    for (int t = 0; t < TM; ++t) fa[t] = fragment(rows_a, t * 16 + i);
+    for (int t = 0; t < TM; ++t) fa[t] = fragment(rows_a + t * 16 * kBlock, i, h);
     if constexpr (WIDE) {
       i32x8 fb[TN];
 #pragma unroll
-      for (int t = 0; t < TN; ++t) fb[t] = fragment(rows_b, t * 16 + i);
+      for (int t = 0; t < TN; ++t) fb[t] = fragment(rows_b + t * 16 * kBlock, i, h);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         bf16x8 xa[TM];
@@ -397,40 +480,14 @@ __global__ void __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 2) gemm_fp8_k
     } else {
 #pragma unroll
       for (int t = 0; t < TN; ++t) {
-        const i32x8 fb = fragment(rows_b, t * 16 + i);
-        const int s = scale_b[t * 64];
+        const i32x8 fb = fragment(rows_b + t * 16 * kBlock, i, h);
+        const int sb = scale_b[t * 64];
 #pragma unroll
-        for (int u = 0; u < TM; ++u)
-          acc[u][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb, fa[u], acc[u][t], 0, 0, 0, s, 0, sa[u]);
+        for (int u = 0; u < TM; ++u) acc[u][t] = mfma8(fb, fa[u], acc[u][t], sb, sa[u]);
       }
     }
   }
-
-#pragma unroll
-  for (int t = 0; t < TN; ++t) {
-    const long n = n0 + wn + t * 16 + h * 4;
-    if (n >= p.N) continue;
-    float bias[4] = {0.f, 0.f, 0.f, 0.f};
-    if (p.bias && !p.partial)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) bias[r] = n + r < p.N ? p.bias[n + r] : 0.f;
-#pragma unroll
-    for (int u = 0; u < TM; ++u) {
-      const long m = m0 + wm + u * 16 + i;
-      if (m >= p.M) continue;
-      if (p.partial) {
-        float* o = p.partial + ((long)blockIdx.y * p.M + m) * p.N + n;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (n + r < p.N) o[r] = acc[u][t][r];
-        continue;
-      }
-      f32x4 v;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = finished(acc[u][t][r], p, bias[r]);
-      store4<E>(p, m, n, v);
-    }
-  }
+  write_tile<E, TM, TN>(p, m0 + wm, n0 + wn, m0 + BM <= p.M && n0 + BN <= p.N, acc);
 }
 
 // C from the partial sums of the splits, in their order

@@ -69,8 +69,8 @@ struct Weight {
   double zmax, c;                         // c = log2(e) / T
   int shift;
   const double* table;                    // 2^(i / 32)
-  __device__ __forceinline__ uint64_t of(unsigned bits) const {
-    const double z = (double)value_of(bits);
+  __device__ __forceinline__ uint64_t of(float logit) const {
+    const double z = (double)logit;
     const double t = fmax((z - zmax) * c, -2000.0);
     const double n = rint(t * 32.0);
     const double r = fma(n, -1.0 / 32.0, t);
@@ -102,9 +102,7 @@ __device__ __forceinline__ uint64_t position_of(float u, uint64_t kept) {
 }
 // -log2(min_p): what a label may lie below the largest in units of log2(e) / T; the strongest label always stays
 __device__ __forceinline__ double reach_of(double min_p) { return min_p > 0.0 ? fmax(-log2(min_p), 0.0) : __builtin_inf(); }
-__device__ __forceinline__ bool is_strong(const Weight& w, unsigned bits, double reach) {
-  return !((w.zmax - (double)value_of(bits)) * w.c > reach);
-}
+__device__ __forceinline__ bool is_strong(const Weight& w, float logit, double reach) { return !((w.zmax - (double)logit) * w.c > reach); }
 
 // ---- rows of up to LANES x PER labels: a sorting network in registers ----
 // The key as a double, so that a comparison is one instruction: sign 0, exponent field in [0x400, 0x5ff] (never NaN), order bits, then
@@ -254,10 +252,10 @@ __global__ void __launch_bounds__(256) sample_sorted_kernel(SampleP p) {
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const bool in = x[i] != 0.0 && (set.top_k <= 0 || t * PER + i < set.top_k);
-    const unsigned b = sorted_bits(x[i]);
-    sum += in ? w.of(b) : 0;
+    const float logit = value_of(sorted_bits(x[i]));
+    sum += in ? w.of(logit) : 0;
     run[i] = sum;
-    if (in && is_strong(w, b, reach)) strong |= 1u << i;
+    if (in && is_strong(w, logit, reach)) strong |= 1u << i;
   }
   const uint64_t before = lanes_scan<LANES>(sum) - sum;
   const uint64_t all = lanes_reduce<LANES, OpSum>(sum);
@@ -314,65 +312,83 @@ __device__ __forceinline__ T block_all(T v, Shared<THREADS>& sh) {
   return r;
 }
 
-// The row: each(f) calls f(order bits, index) for the labels of this thread, four pieces of 16 bytes in flight.  It is read again in
-// every pass: the first comes from memory, the others from the L2 it left the row in.
+// The row, or a part of it: each(f) calls f(logit, index) for the labels of this thread, four pieces of 16 bytes in flight.  It is read
+// again in every pass: the first comes from memory, the others from the caches it left the row in.
 template <class E, int THREADS>
 struct RowInMemory {
   const char* z;
   int v;
+  int from = 0, to = -1;                  // in pieces; -1: to the row's end
   template <class F> __device__ __forceinline__ void each(F f) const {
-    const int pieces = v / E::kVec;
-    for (int q = threadIdx.x; q < pieces; q += THREADS * 4) {
+    const int pieces = v / E::kVec, end = to < 0 ? pieces : to;
+    for (int q = from + threadIdx.x; q < end; q += THREADS * 4) {
       u32x4 r[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) r[u] = load16(z, (long)min(q + u * THREADS, pieces - 1) * 16);
+      for (int u = 0; u < 4; ++u) r[u] = load16(z, (long)min(q + u * THREADS, end - 1) * 16);
 #pragma unroll 1
       for (int u = 0; u < 4; ++u) {
         const int at = q + u * THREADS;
-        if (at >= pieces) break;
+        if (at >= end) break;
         float x[E::kVec];
-        const u32x4 now = u == 0 ? r[0] : u == 1 ? r[1] : u == 2 ? r[2] : r[3];
-        E::unpack(now, x);
+        E::unpack(r[0], x);
+        r[0] = r[1];
+        r[1] = r[2];
+        r[2] = r[3];
 #pragma unroll
-        for (int i = 0; i < E::kVec; ++i) f(order_bits(x[i]), at * E::kVec + i);
+        for (int i = 0; i < E::kVec; ++i) f(x[i], at * E::kVec + i);
       }
     }
     const int i = pieces * E::kVec + threadIdx.x;
-    if (i < v) f(order_bits(E::load(z, i)), i);
+    if (to < 0 && i < v) f(E::load(z, i), i);
   }
 };
 
-// A histogram of the labels with low <= key <= high: by equal steps of the value (step > 0) or of the key (2^bits).
+// Steps of a histogram over the labels with low <= key <= high: equal steps of the value (step > 0) or of the key (2^bits).
 struct Steps {
   uint64_t low, high;
   float top, step;
   int bits;
-  __device__ __forceinline__ bool has(uint64_t k) const { return k >= low && k <= high; }
-  __device__ __forceinline__ int bin(unsigned b, uint64_t k) const {
-    return step > 0.f ? (int)fminf((top - value_of(b)) * step, (float)(kBins - 1)) : (int)((high - k) >> bits);
+  __device__ __forceinline__ bool has(unsigned b, int i) const {
+    const unsigned lo = (unsigned)(low >> 32);
+    if (b - lo > (unsigned)(high >> 32) - lo) return false;      // 32 bits decide all but the ends
+    const uint64_t k = key_of(b, i);
+    return k >= low && k <= high;
+  }
+  __device__ __forceinline__ int bin(float x, uint64_t k) const {
+    return step > 0.f ? (int)fminf((top - x) * step, (float)(kBins - 1)) : (int)((high - k) >> bits);
+  }
+  __device__ __forceinline__ void fit_bits() {
+    const uint64_t span = high - low;
+    bits = 0;
+    while ((span >> bits) >= (uint64_t)kBins) ++bits;
   }
 };
-
 // steps of the value over `span` below the largest; 0 (steps of the key) where there is no such span
 __device__ __forceinline__ float step_of(float span) {
   const float step = span > 0.f && span < 1e30f ? (float)(kBins - 1) / span : 0.f;
   return step < 1e30f ? step : 0.f;
 }
 
+// also returns this thread's share of the weight of the strong labels
 template <bool COUNT, int THREADS, class ROW>
-__device__ __forceinline__ void histogram(const ROW& row, const Weight& w, const Steps& st, Shared<THREADS>& sh) {
+__device__ __forceinline__ uint64_t histogram(const ROW& row, const Weight& w, const Steps& st, double reach, Shared<THREADS>& sh) {
   for (int i = threadIdx.x; i < kBins; i += THREADS) { sh.count[i] = 0; sh.mass[i] = 0; }
   __syncthreads();
-  row.each([&](unsigned b, int i) {
-    const uint64_t k = key_of(b, i);
-    if (!st.has(k)) return;
-    const uint64_t m = COUNT ? 1 : w.of(b);
+  uint64_t strong = 0;
+  row.each([&](float x, int i) {
+    const unsigned b = order_bits(x);
+    if (!st.has(b, i)) return;
+    const uint64_t m = COUNT ? 1 : w.of(x);
     if (m == 0) return;                                          // no position can fall on it
-    const int at = st.bin(b, k);
+    const int at = st.bin(x, key_of(b, i));
     atomicAdd(&sh.count[at], 1u);
-    if (!COUNT) atomicAdd((unsigned long long*)&sh.mass[at], (unsigned long long)m);
+    if (!COUNT) {
+      atomicAdd((unsigned long long*)&sh.mass[at], (unsigned long long)m);
+      if (is_strong(w, x, reach)) strong += m;
+    }
   });
   __syncthreads();
+  return strong;
 }
 
 // The label on which position `want` falls, by count (COUNT: the want-th of the order, from 0) or by weight (the first whose running sum
@@ -387,9 +403,10 @@ __device__ Found find(const ROW& row, const Weight& w, Steps st, unsigned member
   for (int round = 0; members > (unsigned)kList && round < 10; ++round) {      // 64 bits of key, at least 10 a round
     if (bin >= 0) {                                              // the bin's own range of keys, in equal steps of the key
       uint64_t lo = ~0ull, hi = 0;
-      row.each([&](unsigned b, int i) {
+      row.each([&](float x, int i) {
+        const unsigned b = order_bits(x);
         const uint64_t k = key_of(b, i);
-        if (!st.has(k) || st.bin(b, k) != bin) return;
+        if (!st.has(b, i) || st.bin(x, k) != bin) return;
         lo = k < lo ? k : lo;
         hi = k > hi ? k : hi;
       });
@@ -399,10 +416,8 @@ __device__ Found find(const ROW& row, const Weight& w, Steps st, unsigned member
     }
     if (!ready || bin >= 0) {
       ready = bin < 0;
-      const uint64_t span = st.high - st.low;
-      st.bits = 0;
-      while ((span >> st.bits) >= (uint64_t)kBins) ++st.bits;
-      histogram<COUNT, THREADS>(row, w, st, sh);
+      st.fit_bits();
+      histogram<COUNT, THREADS>(row, w, st, 0.0, sh);
     }
     // the bin in which the running sum crosses `want`
     constexpr int PER = kBins / THREADS;
@@ -439,10 +454,11 @@ __device__ Found find(const ROW& row, const Weight& w, Steps st, unsigned member
   __syncthreads();
   if (tid == 0) sh.listed = 0;
   __syncthreads();
-  row.each([&](unsigned b, int i) {
+  row.each([&](float x, int i) {
+    const unsigned b = order_bits(x);
     const uint64_t k = key_of(b, i);
-    if (!st.has(k) || (bin >= 0 && st.bin(b, k) != bin)) return;
-    const uint64_t m = COUNT ? 1 : w.of(b);
+    if (!st.has(b, i) || (bin >= 0 && st.bin(x, k) != bin)) return;
+    const uint64_t m = COUNT ? 1 : w.of(x);
     if (m == 0) return;
     const unsigned at = atomicAdd(&sh.listed, 1u);
     if (at < (unsigned)kList) {
@@ -455,8 +471,8 @@ __device__ Found find(const ROW& row, const Weight& w, Steps st, unsigned member
   for (int e = tid; e < n; e += THREADS) {
     const uint64_t k = sh.list_key[e];
     uint64_t before = COUNT ? base_c : base_m;
-    for (int l = 0; l < n; ++l)
-      if (sh.list_key[l] > k) before += sh.list_mass[l];
+#pragma unroll 4
+    for (int l = 0; l < n; ++l) before += sh.list_key[l] > k ? sh.list_mass[l] : 0;
     const uint64_t upto = before + sh.list_mass[e];
     if (before <= want && want < upto) sh.found = Found{k, upto};
   }
@@ -476,8 +492,14 @@ __device__ __forceinline__ void draw_from_list(const Weight& w, const Settings& 
     const int e = tid + h * THREADS;
     key[h] = e < n ? sh.list_key[e] : 0;
     unsigned rank = 0;
+    before[h] = 0;
     if (e < n)
-      for (int l = 0; l < n; ++l) rank += sh.list_key[l] > key[h];
+#pragma unroll 4
+      for (int l = 0; l < n; ++l) {
+        const bool better = sh.list_key[l] > key[h];
+        rank += better;
+        before[h] += better ? sh.list_mass[l] : 0;
+      }
     own[h] = e < n && rank < (unsigned)set.top_k ? sh.list_mass[e] : 0;
     if (own[h] == 0) key[h] = 0;
     sum += own[h];
@@ -487,13 +509,8 @@ __device__ __forceinline__ void draw_from_list(const Weight& w, const Settings& 
   const double reach = reach_of(set.min_p);
   uint64_t kept = 0;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    before[h] = 0;
-    if (key[h] == 0) continue;
-    for (int l = 0; l < n; ++l)
-      if (sh.list_key[l] > key[h]) before[h] += sh.list_mass[l];
-    if (before[h] <= border && is_strong(w, (unsigned)(key[h] >> 32), reach)) kept = max(kept, before[h] + own[h]);
-  }
+  for (int h = 0; h < 2; ++h)
+    if (key[h] && before[h] <= border && is_strong(w, value_of((unsigned)(key[h] >> 32)), reach)) kept = max(kept, before[h] + own[h]);
   kept = block_all<THREADS, OpMax>(kept, sh);
   const uint64_t want = position_of(set.u, kept);
 #pragma unroll
@@ -501,117 +518,426 @@ __device__ __forceinline__ void draw_from_list(const Weight& w, const Settings& 
     if (key[h] && before[h] <= want && want < before[h] + own[h]) *out = (int64_t)(0xffffffffu - (unsigned)key[h]);
 }
 
+__device__ __forceinline__ Weight weight_of(const SampleP& p, const Settings& set, unsigned top, const double* table) {
+  Weight w;
+  w.zmax = (double)value_of(top);
+  w.c = 1.4426950408889634 / set.t;
+  w.shift = p.shift;
+  w.table = table;
+  return w;
+}
+// All labels of a row whose largest has order bits `top`, in steps down to where a weight is 0 as an integer, or to the least label that
+// counts as one (-1e30: what lies lower masks) where that is known.
+__device__ __forceinline__ float span_of(const Weight& w) { return (float)((w.shift + 1) / w.c); }
+__device__ __forceinline__ float least_of(float least, float x) { return x > -1e30f ? fminf(least, x) : least; }
+__device__ __forceinline__ Steps all_steps(const Weight& w, unsigned top, float least) {
+  Steps st;
+  st.low = key_of(kNothing + 1, 0x7fffffff);
+  st.high = key_of(top, 0);
+  st.top = (float)w.zmax;
+  st.step = step_of(fminf(span_of(w), st.top - least));
+  st.fit_bits();
+  return st;
+}
+__device__ __forceinline__ bool is_single(const Settings& set) { return !(set.t > 0.0) || set.top_k == 1; }
+
 template <class E, int THREADS>
-__global__ void __launch_bounds__(THREADS) sample_row_kernel(SampleP p) {
-  __shared__ Shared<THREADS> sh;
-  const long r = blockIdx.x;
+__device__ void draw_row(const SampleP& p, long r, Shared<THREADS>& sh) {
   const RowInMemory<E, THREADS> row{static_cast<const char*>(p.z) + r * p.ldz * E::kBytes, p.v};
   const Settings set = settings_of(p, r);
   fill_table(sh.table);
 
-  uint64_t best = 0;
-  unsigned lowest = 0xffffffffu, some = 0;
-  row.each([&](unsigned b, int i) {
-    if (b == kNothing) return;
-    const uint64_t k = key_of(b, i);
-    best = k > best ? k : best;
-    lowest = b < lowest ? b : lowest;
-    ++some;
-  });
-  const uint64_t mine = best;
-  best = block_all<THREADS, OpMax>(best, sh);
-  if (best == 0 || !(set.t > 0.0) || set.top_k == 1) {           // nothing to draw; or the first alone
-    if (threadIdx.x == 0) p.out[r] = best == 0 ? -1 : (int64_t)(0xffffffffu - (unsigned)best);
+  float most = -__builtin_inff();
+  row.each([&](float x, int) { most = fmaxf(most, x); });
+  const unsigned mine = order_bits(most), top = block_all<THREADS, OpMax>(mine, sh);
+  if (top == kNothing) {
+    if (threadIdx.x == 0) p.out[r] = -1;
     return;
   }
-  some = block_all<THREADS, OpSum>(some, sh);
-  Weight w;
-  w.zmax = (double)value_of((unsigned)(best >> 32));
-  w.c = 1.4426950408889634 / set.t;
-  w.shift = p.shift;
-  w.table = sh.table;
-  Steps st;
-  st.low = key_of(kNothing + 1, 0x7fffffff);
-  st.high = best;
-  st.bits = 0;
-
-  if (set.top_k > 0 && (unsigned)set.top_k < some && set.top_k <= kPrune) {
-    // a label under the top_k-th largest of 256 groups' maxima has top_k better ones: it is out
-    constexpr int kGroups = 256, kGroup = THREADS / kGroups;
-    static_assert(kGroup == 1 || kGroup == 4, "a thread or a quad");
-    uint64_t* maxima = sh.mass;
-    uint64_t group = mine;
-    if constexpr (kGroup == 4) {
-      group = max(group, lane_step<0xB1>(group));
-      group = max(group, lane_step<0x4E>(group));
-    }
-    if (threadIdx.x % kGroup == 0) maxima[threadIdx.x / kGroup] = group;
-    if (threadIdx.x == 0) { sh.listed = 0; sh.found.key = 0; }
-    __syncthreads();
-    if (threadIdx.x < kGroups) {
-      const uint64_t me = maxima[threadIdx.x];
-      int better = 0;
-#pragma unroll 8
-      for (int l = 0; l < kGroups; ++l) better += maxima[l] > me;
-      if (me && better == set.top_k - 1) sh.found.key = me;
-    }
-    __syncthreads();
-    const uint64_t bound = max(sh.found.key, st.low);            // fewer groups with a label than top_k: no bound
-    row.each([&](unsigned b, int i) {
-      const uint64_t k = key_of(b, i);
-      if (k < bound) return;
-      const unsigned at = atomicAdd(&sh.listed, 1u);
-      if (at < (unsigned)kList) {
-        sh.list_key[at] = k;
-        sh.list_mass[at] = w.of(b);
-      }
+  if (is_single(set)) {
+    unsigned at = 0xffffffffu;
+    row.each([&](float x, int i) {
+      if (order_bits(x) == top) at = min(at, (unsigned)i);
     });
-    __syncthreads();
-    if (sh.listed <= (unsigned)kList) {
-      draw_from_list<THREADS>(w, set, (int)sh.listed, p.out + r, sh);
-      return;
+    at = block_all<THREADS, OpMin>(at, sh);
+    if (threadIdx.x == 0) p.out[r] = at;
+    return;
+  }
+  const Weight w = weight_of(p, set, top, sh.table);
+  Steps st = all_steps(w, top, -__builtin_inff());
+  unsigned members = (unsigned)p.v;
+
+  if (set.top_k > 0 && set.top_k < p.v) {
+    if (set.top_k <= kPrune) {
+      // a label under the top_k-th largest of 256 groups' maxima has top_k better ones: it is out
+      constexpr int kGroups = 256, kGroup = THREADS / kGroups;
+      static_assert(kGroup == 1 || kGroup == 2, "a thread or a pair");
+      unsigned* const maxima = sh.count;
+      unsigned group = mine;
+      if constexpr (kGroup == 2) group = max(group, lane_step<0xB1>(group));
+      if (threadIdx.x % kGroup == 0) maxima[threadIdx.x / kGroup] = group;
+      if (threadIdx.x == 0) { sh.listed = 0; sh.bin = (int)kNothing; }
+      __syncthreads();
+      if (threadIdx.x < kGroups) {
+        const unsigned me = maxima[threadIdx.x];
+        int better = 0, equal = 0;
+#pragma unroll 8
+        for (int l = 0; l < kGroups; ++l) {
+          better += maxima[l] > me;
+          equal += maxima[l] == me;
+        }
+        if (better < set.top_k && set.top_k <= better + equal) sh.bin = (int)me;        // (equal ones write the same)
+      }
+      __syncthreads();
+      const float bound = value_of((unsigned)sh.bin);            // -inf: fewer groups with a label than top_k
+      row.each([&](float x, int i) {
+        if (!(x >= bound) || x == -__builtin_inff()) return;
+        const unsigned at = atomicAdd(&sh.listed, 1u);
+        if (at < (unsigned)kList) {
+          sh.list_key[at] = key_of(order_bits(x), i);
+          sh.list_mass[at] = w.of(x);
+        }
+      });
+      __syncthreads();
+      if (sh.listed <= (unsigned)kList) {
+        draw_from_list<THREADS>(w, set, (int)sh.listed, p.out + r, sh);
+        return;
+      }
+      __syncthreads();                                           // sh.listed has been read
     }
-    __syncthreads();                                             // sh.listed has been read
+    unsigned some = 0;
+    float least = (float)w.zmax;
+    row.each([&](float x, int) {
+      if (!(x > -__builtin_inff())) return;
+      ++some;
+      least = fminf(least, x);
+    });
+    some = block_all<THREADS, OpSum>(some, sh);
+    least = value_of(block_all<THREADS, OpMin>(order_bits(least), sh));
+    members = some;
+    if ((unsigned)set.top_k < some) {
+      Steps by = st;
+      by.step = step_of((float)w.zmax - fmaxf(least, -1e30f));
+      bool ready = false;
+      st.low = find<true, THREADS>(row, w, by, some, (uint64_t)(set.top_k - 1), ready, sh).key;
+      st.fit_bits();
+      members = (unsigned)set.top_k;
+    }
   }
-  lowest = block_all<THREADS, OpMin>(lowest, sh);
-  const float top = (float)w.zmax;
-  const float reach = top - fmaxf(value_of(lowest), -1e30f);
-  st.top = top;
-  if (set.top_k > 0 && (unsigned)set.top_k < some) {
-    st.step = step_of(reach);
-    bool ready = false;
-    st.low = find<true, THREADS>(row, w, st, some, (uint64_t)(set.top_k - 1), ready, sh).key;
-    some = (unsigned)set.top_k;
+  if (span_of(w) > 64.f) {                                       // a high temperature: steps of the labels' own range
+    float least = (float)w.zmax;
+    row.each([&](float x, int) { least = least_of(least, x); });
+    const uint64_t low = st.low;
+    st = all_steps(w, top, value_of(block_all<THREADS, OpMin>(order_bits(least), sh)));
+    st.low = low;
+    st.fit_bits();
   }
-  // weights more than 2^-52 below the largest are 0 as integers: the steps are spent above that
-  st.step = step_of(fminf(reach, (float)(52.0 / w.c)));
-  const uint64_t range = st.high - st.low;
-  while ((range >> st.bits) >= (uint64_t)kBins) ++st.bits;
   const double weak = reach_of(set.min_p);
-  histogram<false, THREADS>(row, w, st, sh);
+  const uint64_t strong = block_all<THREADS, OpSum>(histogram<false, THREADS>(row, w, st, weak, sh), sh);
   bool ready = true;
-  uint64_t all = 0, strong = 0;
+  uint64_t all = 0;
   for (int i = threadIdx.x; i < kBins; i += THREADS) all += sh.mass[i];
   all = block_all<THREADS, OpSum>(all, sh);
-  uint64_t kept = all;
-  if (weak < __builtin_inf()) {
-    row.each([&](unsigned b, int i) {
-      if (st.has(key_of(b, i)) && is_strong(w, b, weak)) strong += w.of(b);
-    });
-    kept = block_all<THREADS, OpSum>(strong, sh);
-  }
-  if (set.top_p < 1.0) {
-    const uint64_t upto = find<false, THREADS>(row, w, st, some, border_of(set.top_p, all), ready, sh).upto;
-    kept = upto < kept ? upto : kept;
-  }
-  const Found f = find<false, THREADS>(row, w, st, some, position_of(set.u, kept), ready, sh);
+  uint64_t kept = strong;
+  if (set.top_p < 1.0) kept = min(kept, find<false, THREADS>(row, w, st, members, border_of(set.top_p, all), ready, sh).upto);
+  const Found f = find<false, THREADS>(row, w, st, members, position_of(set.u, kept), ready, sh);
   if (threadIdx.x == 0) p.out[r] = (int64_t)(0xffffffffu - (unsigned)f.key);
 }
 
-// Up to 512 labels: the sorting network (16 lanes where 8 labels each are enough).  Above: a workgroup per row, of 1,024 threads for
-// long rows and where there are too few rows to fill the card with smaller ones.
+template <class E, int THREADS>
+__global__ void __launch_bounds__(THREADS, 4) sample_row_kernel(SampleP p) {
+  __shared__ Shared<THREADS> sh;
+  draw_row<E, THREADS>(p, blockIdx.x, sh);
+}
+
+// ---- few long rows: a row's passes spread over several workgroups, one kernel per pass ----
+// 1: maxima of the parts.  2: the histogram of weights relative to the largest (integer atomics: the same bits in any order), and the
+// sum of the strong ones.  3: from the histogram, which bins the answers lie in; their labels into a list.  4: one workgroup per row
+// looks up the answers in the list.  Where the list overflows (equal logits in masses, a temperature of extremes) it draws the row
+// by itself.
+constexpr int kSplitThreads = 512, kSplitList = 4096;
+struct SplitRow {
+  uint64_t mass[kBins];
+  uint64_t strong;
+  uint64_t list[kSplitList];
+  unsigned count[kBins];
+  unsigned listed, first;                 // first: the lowest index of the largest logit, where one label alone is kept
+};
+struct SplitP {
+  SplitRow* rows;
+  unsigned* top;                          // (n, parts): order bits of the parts' largest, and the least
+  float* least;
+  int parts, per;                         // pieces of 16 bytes per part
+};
+template <class E> __device__ __forceinline__ RowInMemory<E, kSplitThreads> part_of(const SampleP& p, const SplitP& sp, long r) {
+  const int part = blockIdx.x, pieces = p.v / E::kVec;
+  RowInMemory<E, kSplitThreads> row{static_cast<const char*>(p.z) + r * p.ldz * E::kBytes, p.v};
+  row.from = min(part * sp.per, pieces);
+  row.to = part == sp.parts - 1 ? -1 : min((part + 1) * sp.per, pieces);
+  return row;
+}
+__device__ __forceinline__ unsigned top_of(const SplitP& sp, long r) {       // by every wave for itself
+  unsigned top = 0;
+  for (int i = threadIdx.x & 63; i < sp.parts; i += 64) top = max(top, sp.top[r * sp.parts + i]);
+  return lanes_reduce<64, OpMax>(top);
+}
+__device__ __forceinline__ float least_label(const SplitP& sp, long r) {
+  float least = __builtin_inff();
+  for (int i = threadIdx.x & 63; i < sp.parts; i += 64) least = fminf(least, sp.least[r * sp.parts + i]);
+  return -lanes_reduce<64, OpMax>(-least);
+}
+// labels of a list that lie in one bin of `st`
+struct RowInList {
+  const uint64_t* keys;
+  int n, bin;
+  Steps st;
+  template <class F> __device__ __forceinline__ void each(F f) const {
+    for (int e = threadIdx.x; e < n; e += kSplitThreads) {
+      const uint64_t k = keys[e];
+      const float x = value_of((unsigned)(k >> 32));
+      if (st.bin(x, k) == bin) f(x, (int)(0xffffffffu - (unsigned)k));
+    }
+  }
+};
+
 template <class E>
-int launch_sample(const SampleP& p, hipStream_t s) {
+__global__ void __launch_bounds__(kSplitThreads, 4) split_best_kernel(SampleP p, SplitP sp) {
+  __shared__ float red[2][kSplitThreads / 64];
+  const long r = blockIdx.y;
+  float most = -__builtin_inff(), least = __builtin_inff();
+  part_of<E>(p, sp, r).each([&](float x, int) {
+    most = fmaxf(most, x);
+    least = least_of(least, x);
+  });
+  most = lanes_reduce<64, OpMax>(most);
+  least = -lanes_reduce<64, OpMax>(-least);
+  if ((threadIdx.x & 63) == 0) { red[0][threadIdx.x >> 6] = most; red[1][threadIdx.x >> 6] = least; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < kSplitThreads / 64; ++i) { most = fmaxf(most, red[0][i]); least = fminf(least, red[1][i]); }
+    sp.top[r * sp.parts + blockIdx.x] = order_bits(most);
+    sp.least[r * sp.parts + blockIdx.x] = least;
+  }
+  SplitRow& sr = sp.rows[r];                                     // cleared for the kernels behind this one
+  for (int i = blockIdx.x * kSplitThreads + threadIdx.x; i < kBins; i += sp.parts * kSplitThreads) {
+    sr.mass[i] = 0;
+    sr.count[i] = 0;
+    if (i == 0) { sr.strong = 0; sr.listed = 0; sr.first = 0xffffffffu; }
+  }
+}
+
+template <class E>
+__global__ void __launch_bounds__(kSplitThreads, 4) split_histogram_kernel(SampleP p, SplitP sp) {
+  __shared__ Shared<kSplitThreads> sh;
+  const long r = blockIdx.y;
+  const Settings set = settings_of(p, r);
+  const unsigned top = top_of(sp, r);
+  SplitRow& sr = sp.rows[r];
+  const auto row = part_of<E>(p, sp, r);
+  if (top == kNothing) return;
+  if (is_single(set)) {
+    row.each([&](float x, int i) {
+      if (order_bits(x) == top) atomicMin(&sr.first, (unsigned)i);
+    });
+    return;
+  }
+  fill_table(sh.table);
+  const Weight w = weight_of(p, set, top, sh.table);
+  uint64_t strong = histogram<false, kSplitThreads>(row, w, all_steps(w, top, least_label(sp, r)), reach_of(set.min_p), sh);
+  for (int i = threadIdx.x; i < kBins; i += kSplitThreads)
+    if (sh.count[i]) {
+      atomicAdd(&sr.count[i], sh.count[i]);
+      atomicAdd((unsigned long long*)&sr.mass[i], (unsigned long long)sh.mass[i]);
+    }
+  strong = block_all<kSplitThreads, OpSum>(strong, sh);
+  if (threadIdx.x == 0 && strong) atomicAdd((unsigned long long*)&sr.strong, (unsigned long long)strong);
+}
+
+// What the histogram says of a row: with a top_k that cuts, the labels of bins 0 .. last_k are the candidates; else the border of
+// top_p lies in bin_p and u's position in one of bins low_u .. high_u.  sh.mass: the weight in front of each bin.
+struct Places {
+  uint64_t all, strong;
+  int last_k, bin_p, low_u, high_u;
+};
+template <int THREADS>
+__device__ Places places_of(const SplitRow& sr, const Settings& set, Shared<THREADS>& sh) {
+  constexpr int PER = kBins / THREADS;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  uint64_t m[PER], sum = 0;
+  unsigned c[PER], count = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    m[i] = sr.mass[tid * PER + i];
+    c[i] = sr.count[tid * PER + i];
+    sum += m[i];
+    count += c[i];
+  }
+  const uint64_t mi = lanes_scan<64>(sum);
+  const unsigned ci = (unsigned)lanes_scan<64>((uint64_t)count);
+  if (lane == 63) { sh.part_m[wave] = mi; sh.part_c[wave] = ci; }
+  int* const found = reinterpret_cast<int*>(&sh.count[0]);       // last_k, bin_p, low_u, high_u
+  uint64_t* const border_bin = &sh.list_mass[0];                 // weight in front of bin_p, and with it
+  if (tid == 0) found[0] = -1;
+  __syncthreads();
+  uint64_t before = mi - sum, all = 0;
+  unsigned before_c = ci - count;
+  for (int x = 0; x < THREADS / 64; ++x) {
+    if (x < wave) { before += sh.part_m[x]; before_c += sh.part_c[x]; }
+    all += sh.part_m[x];
+  }
+  Places pl;
+  pl.all = all;
+  pl.strong = sr.strong;
+  const bool cut = set.top_p < 1.0;
+  const uint64_t border = cut ? border_of(set.top_p, all) : all - 1;
+  uint64_t mb = before;
+  unsigned cb = before_c;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (set.top_k > 0 && cb < (unsigned)set.top_k && (unsigned)set.top_k <= cb + c[i]) found[0] = tid * PER + i;
+    if (mb <= border && border < mb + m[i]) { found[1] = tid * PER + i; border_bin[0] = mb; border_bin[1] = mb + m[i]; }
+    sh.mass[tid * PER + i] = mb;
+    mb += m[i];
+    cb += c[i];
+  }
+  __syncthreads();
+  pl.last_k = found[0];
+  pl.bin_p = cut ? found[1] : -1;
+  const uint64_t least = cut ? border_bin[0] + 1 : all, most = cut ? border_bin[1] : all;
+  const uint64_t low = position_of(set.u, min(least, pl.strong)), high = position_of(set.u, min(most, pl.strong));
+  mb = before;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (mb <= low && low < mb + m[i]) found[2] = tid * PER + i;
+    if (mb <= high && high < mb + m[i]) found[3] = tid * PER + i;
+    mb += m[i];
+  }
+  __syncthreads();
+  pl.low_u = found[2];
+  pl.high_u = found[3];
+  __syncthreads();
+  return pl;
+}
+
+template <class E>
+__global__ void __launch_bounds__(kSplitThreads, 4) split_collect_kernel(SampleP p, SplitP sp) {
+  __shared__ Shared<kSplitThreads> sh;
+  const long r = blockIdx.y;
+  const Settings set = settings_of(p, r);
+  const unsigned top = top_of(sp, r);
+  if (top == kNothing || is_single(set)) return;
+  const Weight w = weight_of(p, set, top, sh.table);             // (no weight is formed: the table stays empty)
+  const Steps st = all_steps(w, top, least_label(sp, r));
+  SplitRow& sr = sp.rows[r];
+  const Places pl = places_of<kSplitThreads>(sr, set, sh);
+  const int from = pl.last_k >= 0 ? 0 : pl.low_u, to = pl.last_k >= 0 ? pl.last_k : pl.high_u, also = pl.last_k >= 0 ? -1 : pl.bin_p;
+  part_of<E>(p, sp, r).each([&](float x, int i) {
+    if (!(x > -__builtin_inff())) return;
+    const unsigned b = order_bits(x);
+    const uint64_t k = key_of(b, i);
+    const int bin = st.bin(x, k);
+    if ((bin < from || bin > to) && bin != also) return;
+    const unsigned at = atomicAdd(&sr.listed, 1u);
+    if (at < (unsigned)kSplitList) sr.list[at] = k;
+  });
+}
+
+template <class E>
+__global__ void __launch_bounds__(kSplitThreads, 4) split_draw_kernel(SampleP p, SplitP sp) {
+  __shared__ Shared<kSplitThreads> sh;
+  const long r = blockIdx.x;
+  const int tid = threadIdx.x;
+  const Settings set = settings_of(p, r);
+  const unsigned top = top_of(sp, r);
+  const SplitRow& sr = sp.rows[r];
+  if (top == kNothing || is_single(set)) {
+    if (tid == 0) p.out[r] = top == kNothing ? -1 : (int64_t)sr.first;
+    return;
+  }
+  const int n = (int)min(sr.listed, (unsigned)kSplitList);
+  fill_table(sh.table);
+  const Weight w = weight_of(p, set, top, sh.table);
+  const Steps st = all_steps(w, top, least_label(sp, r));
+  const Places pl = places_of<kSplitThreads>(sr, set, sh);
+  if (sr.listed > (unsigned)(pl.last_k >= 0 ? kList : kSplitList)) {
+    __syncthreads();
+    draw_row<E, kSplitThreads>(p, r, sh);
+    return;
+  }
+  if (pl.last_k >= 0) {
+    for (int e = tid; e < n; e += kSplitThreads) {
+      const uint64_t k = sr.list[e];
+      sh.list_key[e] = k;
+      sh.list_mass[e] = w.of(value_of((unsigned)(k >> 32)));
+    }
+    __syncthreads();
+    draw_from_list<kSplitThreads>(w, set, n, p.out + r, sh);
+    return;
+  }
+  // the label of one bin on which a position falls
+  auto look_up = [&](int bin, uint64_t front, uint64_t want) {
+    const RowInList row{sr.list, n, bin, st};
+    Steps in = st;
+    in.step = 0.f;
+    uint64_t lo = ~0ull, hi = 0;
+    row.each([&](float x, int i) {
+      const uint64_t k = key_of(order_bits(x), i);
+      lo = min(lo, k);
+      hi = max(hi, k);
+    });
+    in.low = block_all<kSplitThreads, OpMin>(lo, sh);
+    in.high = block_all<kSplitThreads, OpMax>(hi, sh);
+    bool ready = false;
+    Found f = find<false, kSplitThreads>(row, w, in, (unsigned)n, want - front, ready, sh);
+    f.upto += front;
+    return f;
+  };
+  // what stands in front of the bins that matter; find has its own use for sh.mass
+  uint64_t kept = pl.strong;
+  const uint64_t front_p = pl.bin_p >= 0 ? sh.mass[pl.bin_p] : 0;
+  const int bins_u = pl.high_u - pl.low_u;
+  uint64_t front_u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) front_u[i] = sh.mass[min(pl.low_u + i, kBins - 1)];
+  const bool near = bins_u < 4;                                  // u's position moves over a few bins at most; else search again
+  __syncthreads();
+  if (pl.bin_p >= 0) kept = min(kept, look_up(pl.bin_p, front_p, border_of(set.top_p, pl.all)).upto);
+  const uint64_t want = position_of(set.u, kept);
+  int bin = pl.low_u;
+  uint64_t front = front_u[0];
+  if (near) {
+#pragma unroll
+    for (int i = 1; i < 4; ++i)
+      if (i <= bins_u && front_u[i] <= want) { bin = pl.low_u + i; front = front_u[i]; }
+  } else {
+    front = 0;
+    for (int i = 0; i <= pl.high_u; ++i) {
+      const uint64_t m = sr.mass[i];
+      if (front + m > want) { bin = i; break; }
+      front += m;
+    }
+  }
+  const Found f = look_up(bin, front, want);
+  if (tid == 0) p.out[r] = (int64_t)(0xffffffffu - (unsigned)f.key);
+}
+
+struct SplitPlan { int parts, per; };
+// A row is spread where there are too few rows to fill the card: 1,024 workgroups in all, of at least 4,096 labels each.
+inline SplitPlan split_plan(long n, int v, int vec) {
+  const int pieces = v / vec;
+  long parts = n > 0 ? 1024 / n : 0;
+  if (parts > v / 4096) parts = v / 4096;
+  if (n > 512 || parts < 2) return SplitPlan{1, pieces};
+  const int per = (int)((pieces + parts - 1) / parts);
+  return SplitPlan{(pieces + per - 1) / per, per};
+}
+inline int64_t split_bytes(long n, const SplitPlan& plan) {
+  return plan.parts < 2 ? 0 : n * (int64_t)sizeof(SplitRow) + n * plan.parts * 8;
+}
+
+// Up to 512 labels: the sorting network (16 lanes where 8 labels each are enough).  Above: a workgroup per row, or several.
+template <class E>
+int launch_sample(const SampleP& p, void* workspace, hipStream_t s) {
   auto sorted = [&](auto lanes, auto per) {
     constexpr int L = decltype(lanes)::value, P = decltype(per)::value;
     hipLaunchKernelGGL((sample_sorted_kernel<E, L, P>), dim3((unsigned)((p.n + 256 / L - 1) / (256 / L))), dim3(256), 0, s, p);
@@ -624,8 +950,26 @@ int launch_sample(const SampleP& p, hipStream_t s) {
   else if (p.v <= 128) OBJ_SORTED(16, 8);
   else if (p.v <= 256) OBJ_SORTED(64, 4);
   else if (p.v <= 512) OBJ_SORTED(64, 8);
-  else if (p.v <= 16384 && p.n > 512) hipLaunchKernelGGL((sample_row_kernel<E, 256>), dim3((unsigned)p.n), dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((sample_row_kernel<E, 1024>), dim3((unsigned)p.n), dim3(1024), 0, s, p);
+  else {
+    const SplitPlan plan = split_plan(p.n, p.v, E::kVec);
+    if (plan.parts > 1) {
+      SplitP sp;
+      sp.rows = static_cast<SplitRow*>(workspace);
+      sp.top = reinterpret_cast<unsigned*>(sp.rows + p.n);
+      sp.least = reinterpret_cast<float*>(sp.top + p.n * plan.parts);
+      sp.parts = plan.parts;
+      sp.per = plan.per;
+      const dim3 grid((unsigned)plan.parts, (unsigned)p.n), block(kSplitThreads);
+      hipLaunchKernelGGL((split_best_kernel<E>), grid, block, 0, s, p, sp);
+      hipLaunchKernelGGL((split_histogram_kernel<E>), grid, block, 0, s, p, sp);
+      hipLaunchKernelGGL((split_collect_kernel<E>), grid, block, 0, s, p, sp);
+      hipLaunchKernelGGL((split_draw_kernel<E>), dim3((unsigned)p.n), block, 0, s, p, sp);
+    } else if (p.v <= 4096) {
+      hipLaunchKernelGGL((sample_row_kernel<E, 256>), dim3((unsigned)p.n), dim3(256), 0, s, p);
+    } else {
+      hipLaunchKernelGGL((sample_row_kernel<E, 512>), dim3((unsigned)p.n), dim3(512), 0, s, p);
+    }
+  }
 #undef OBJ_SORTED
   return check_launch("sample_logits");
 }
@@ -634,6 +978,11 @@ int launch_sample(const SampleP& p, hipStream_t s) {
 }  // namespace objnerf
 
 using namespace objnerf;
+
+extern "C" int64_t objnerf_sample_logits_workspace_bytes(int64_t n, int32_t v, int type) {
+  if (n <= 0 || v <= 512 || !label_type_ok(type)) return 0;
+  return split_bytes(n, split_plan(n, v, 16 / label_type_bytes(type)));
+}
 
 extern "C" int objnerf_sample_logits(const objnerf_sample_args* a, void* stream) {
   if (!a) return set_error(-1, "sample_logits: no arguments");
@@ -646,6 +995,8 @@ extern "C" int objnerf_sample_logits(const objnerf_sample_args* a, void* stream)
   if (!a->min_p_rows && !(a->min_p >= 0.0 && a->min_p <= 1.0)) return set_error(-1, "sample_logits: min_p must lie in [0, 1]");
   if (a->n == 0) return 0;
   if (!a->logits || !a->u || !a->labels) return set_error(-1, "sample_logits: a needed buffer is missing");
+  if (objnerf_sample_logits_workspace_bytes(a->n, a->v, a->type) && (!a->workspace || (uintptr_t)a->workspace & 7))
+    return set_error(-1, "sample_logits: a workspace (8-byte aligned) is needed");
   SampleP p;
   p.n = a->n; p.v = a->v;
   p.z = a->logits; p.ldz = a->logits_stride;
@@ -659,6 +1010,6 @@ extern "C" int objnerf_sample_logits(const objnerf_sample_args* a, void* stream)
   p.shift = 62 - log_v < 51 ? 62 - log_v : 51;
   p.out = a->labels;
   hipStream_t s = (hipStream_t)stream;
-  return a->type == OBJNERF_TYPE_F32 ? launch_sample<ElemF32>(p, s)
-         : a->type == OBJNERF_TYPE_BF16 ? launch_sample<ElemBf16>(p, s) : launch_sample<ElemF16>(p, s);
+  return a->type == OBJNERF_TYPE_F32 ? launch_sample<ElemF32>(p, a->workspace, s)
+         : a->type == OBJNERF_TYPE_BF16 ? launch_sample<ElemBf16>(p, a->workspace, s) : launch_sample<ElemF16>(p, a->workspace, s);
 }

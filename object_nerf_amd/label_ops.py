@@ -380,6 +380,11 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         a.min_p = min_p
     labels = torch.empty(n, dtype=torch.int64, device=dev)
     a.labels = labels.data_ptr()
+    lib = _lib.lib()
+    room = lib.objnerf_sample_logits_workspace_bytes(n, v, a.type) if v > 512 else 0
+    if room:
+        work = torch.empty(room, dtype=torch.uint8, device=dev)
+        a.workspace = work.data_ptr()
     if n:
-        _call(_lib.lib().objnerf_sample_logits, a, dev, "sample_logits")
+        _call(lib.objnerf_sample_logits, a, dev, "sample_logits")
     return labels
