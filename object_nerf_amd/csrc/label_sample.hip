@@ -24,7 +24,7 @@
 namespace objnerf {
 namespace {
 
-constexpr int kBins = 2048, kList = 512, kPrune = 128;
+constexpr int kList = 512, kPrune = 128;
 
 struct SampleP {
   long n;
@@ -283,12 +283,14 @@ __global__ void __launch_bounds__(256) sample_sorted_kernel(SampleP p) {
 // ---- longer rows: a workgroup each ----
 
 struct Found { uint64_t key, upto; };     // the label's key; weight of the order up to it, itself included
+struct __align__(16) Entry { uint64_t key, mass; };
 
 template <int THREADS>
 struct Shared {
+  static constexpr int kBins = 8 * THREADS;
   unsigned count[kBins];
   uint64_t mass[kBins];
-  uint64_t list_key[kList], list_mass[kList];
+  Entry list[kList];
   double table[32];
   uint64_t red[THREADS / 64];
   uint64_t part_m[THREADS / 64];
@@ -347,7 +349,7 @@ struct RowInMemory {
 struct Steps {
   uint64_t low, high;
   float top, step;
-  int bits;
+  int bits, last;                         // last: the last bin's number
   __device__ __forceinline__ bool has(unsigned b, int i) const {
     const unsigned lo = (unsigned)(low >> 32);
     if (b - lo > (unsigned)(high >> 32) - lo) return false;      // 32 bits decide all but the ends
@@ -355,24 +357,24 @@ struct Steps {
     return k >= low && k <= high;
   }
   __device__ __forceinline__ int bin(float x, uint64_t k) const {
-    return step > 0.f ? (int)fminf((top - x) * step, (float)(kBins - 1)) : (int)((high - k) >> bits);
+    return step > 0.f ? (int)fminf((top - x) * step, (float)last) : (int)((high - k) >> bits);
   }
   __device__ __forceinline__ void fit_bits() {
     const uint64_t span = high - low;
     bits = 0;
-    while ((span >> bits) >= (uint64_t)kBins) ++bits;
+    while ((span >> bits) > (uint64_t)last) ++bits;
+  }
+  // steps of the value over `span` below the largest; 0 (steps of the key) where there is no such span
+  __device__ __forceinline__ void fit_step(float span) {
+    step = span > 0.f && span < 1e30f ? (float)last / span : 0.f;
+    if (!(step < 1e30f)) step = 0.f;
   }
 };
-// steps of the value over `span` below the largest; 0 (steps of the key) where there is no such span
-__device__ __forceinline__ float step_of(float span) {
-  const float step = span > 0.f && span < 1e30f ? (float)(kBins - 1) / span : 0.f;
-  return step < 1e30f ? step : 0.f;
-}
 
 // also returns this thread's share of the weight of the strong labels
 template <bool COUNT, int THREADS, class ROW>
 __device__ __forceinline__ uint64_t histogram(const ROW& row, const Weight& w, const Steps& st, double reach, Shared<THREADS>& sh) {
-  for (int i = threadIdx.x; i < kBins; i += THREADS) { sh.count[i] = 0; sh.mass[i] = 0; }
+  for (int i = threadIdx.x; i < Shared<THREADS>::kBins; i += THREADS) { sh.count[i] = 0; sh.mass[i] = 0; }
   __syncthreads();
   uint64_t strong = 0;
   row.each([&](float x, int i) {
@@ -420,7 +422,7 @@ __device__ Found find(const ROW& row, const Weight& w, Steps st, unsigned member
       histogram<COUNT, THREADS>(row, w, st, 0.0, sh);
     }
     // the bin in which the running sum crosses `want`
-    constexpr int PER = kBins / THREADS;
+    constexpr int PER = Shared<THREADS>::kBins / THREADS;
     unsigned c = 0;
     uint64_t m = 0;
 #pragma unroll
@@ -461,46 +463,52 @@ __device__ Found find(const ROW& row, const Weight& w, Steps st, unsigned member
     const uint64_t m = COUNT ? 1 : w.of(x);
     if (m == 0) return;
     const unsigned at = atomicAdd(&sh.listed, 1u);
-    if (at < (unsigned)kList) {
-      sh.list_key[at] = k;
-      sh.list_mass[at] = m;
-    }
+    if (at < (unsigned)kList) sh.list[at] = Entry{k, m};
   });
   __syncthreads();
   const int n = (int)min(sh.listed, (unsigned)kList);
   for (int e = tid; e < n; e += THREADS) {
-    const uint64_t k = sh.list_key[e];
+    const Entry me = sh.list[e];
     uint64_t before = COUNT ? base_c : base_m;
-#pragma unroll 4
-    for (int l = 0; l < n; ++l) before += sh.list_key[l] > k ? sh.list_mass[l] : 0;
-    const uint64_t upto = before + sh.list_mass[e];
-    if (before <= want && want < upto) sh.found = Found{k, upto};
+#pragma unroll 8
+    for (int l = 0; l < n; ++l) {
+      const Entry o = sh.list[l];
+      before += o.key > me.key ? o.mass : 0;
+    }
+    if (before <= want && want < before + me.mass) sh.found = Found{me.key, before + me.mass};
   }
   __syncthreads();
   return sh.found;
+}
+
+// weights of the list's labels (here and not where they are found: every lane has one to work on)
+template <int THREADS> __device__ __forceinline__ void weigh_list(const Weight& w, int n, Shared<THREADS>& sh) {
+  for (int e = threadIdx.x; e < n; e += THREADS) sh.list[e].mass = w.of(value_of((unsigned)(sh.list[e].key >> 32)));
+  __syncthreads();
 }
 
 // The whole draw among the n labels of the list, of which the top_k count.
 template <int THREADS>
 __device__ __forceinline__ void draw_from_list(const Weight& w, const Settings& set, int n, int64_t* out, Shared<THREADS>& sh) {
   const int tid = threadIdx.x;
-  static_assert(kList <= 2 * THREADS, "two labels per thread");
-  uint64_t key[2], own[2], before[2];
+  constexpr int H = kList / THREADS > 0 ? kList / THREADS : 1;     // labels per thread
+  uint64_t key[H], own[H], before[H];
   uint64_t sum = 0;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < H; ++h) {
     const int e = tid + h * THREADS;
-    key[h] = e < n ? sh.list_key[e] : 0;
+    key[h] = e < n ? sh.list[e].key : 0;
     unsigned rank = 0;
     before[h] = 0;
     if (e < n)
-#pragma unroll 4
+#pragma unroll 8
       for (int l = 0; l < n; ++l) {
-        const bool better = sh.list_key[l] > key[h];
+        const Entry o = sh.list[l];
+        const bool better = o.key > key[h];
         rank += better;
-        before[h] += better ? sh.list_mass[l] : 0;
+        before[h] += better ? o.mass : 0;
       }
-    own[h] = e < n && rank < (unsigned)set.top_k ? sh.list_mass[e] : 0;
+    own[h] = e < n && rank < (unsigned)set.top_k ? sh.list[e].mass : 0;
     if (own[h] == 0) key[h] = 0;
     sum += own[h];
   }
@@ -509,12 +517,12 @@ __device__ __forceinline__ void draw_from_list(const Weight& w, const Settings& 
   const double reach = reach_of(set.min_p);
   uint64_t kept = 0;
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int h = 0; h < H; ++h)
     if (key[h] && before[h] <= border && is_strong(w, value_of((unsigned)(key[h] >> 32)), reach)) kept = max(kept, before[h] + own[h]);
   kept = block_all<THREADS, OpMax>(kept, sh);
   const uint64_t want = position_of(set.u, kept);
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
+  for (int h = 0; h < H; ++h)
     if (key[h] && before[h] <= want && want < before[h] + own[h]) *out = (int64_t)(0xffffffffu - (unsigned)key[h]);
 }
 
@@ -530,16 +538,127 @@ __device__ __forceinline__ Weight weight_of(const SampleP& p, const Settings& se
 // counts as one (-1e30: what lies lower masks) where that is known.
 __device__ __forceinline__ float span_of(const Weight& w) { return (float)((w.shift + 1) / w.c); }
 __device__ __forceinline__ float least_of(float least, float x) { return x > -1e30f ? fminf(least, x) : least; }
-__device__ __forceinline__ Steps all_steps(const Weight& w, unsigned top, float least) {
+template <int THREADS> __device__ __forceinline__ Steps all_steps(const Weight& w, unsigned top, float least) {
   Steps st;
+  st.last = Shared<THREADS>::kBins - 1;
   st.low = key_of(kNothing + 1, 0x7fffffff);
   st.high = key_of(top, 0);
   st.top = (float)w.zmax;
-  st.step = step_of(fminf(span_of(w), st.top - least));
+  st.fit_step(fminf(span_of(w), st.top - least));
   st.fit_bits();
   return st;
 }
 __device__ __forceinline__ bool is_single(const Settings& set) { return !(set.t > 0.0) || set.top_k == 1; }
+
+// What the histogram says of a row: with a top_k that cuts, the labels of bins 0 .. last_k are the candidates; else the border of
+// top_p lies in bin_p and u's position in one of bins low_u .. high_u.  Afterwards sh.mass holds the weight in front of each bin, and
+// sh.list is free.
+struct Places {
+  uint64_t all, strong;
+  int last_k, bin_p, low_u, high_u;
+};
+template <int THREADS>
+__device__ Places places_of(const uint64_t* mass, const unsigned* counts, uint64_t strong, const Settings& set, Shared<THREADS>& sh) {
+  constexpr int PER = Shared<THREADS>::kBins / THREADS;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  uint64_t m[PER], sum = 0;
+  unsigned c[PER], count = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    m[i] = mass[tid * PER + i];
+    c[i] = counts[tid * PER + i];
+    sum += m[i];
+    count += c[i];
+  }
+  const uint64_t mi = lanes_scan<64>(sum);
+  const unsigned ci = (unsigned)lanes_scan<64>((uint64_t)count);
+  if (lane == 63) { sh.part_m[wave] = mi; sh.part_c[wave] = ci; }
+  int* const found = reinterpret_cast<int*>(&sh.list[0]);        // last_k, bin_p, low_u, high_u
+  uint64_t* const border_bin = &sh.list[1].key;                  // weight in front of bin_p, and with it
+  if (tid == 0) found[0] = -1;
+  __syncthreads();                                               // (and mass / counts have been read, where they are sh's)
+  uint64_t before = mi - sum, all = 0;
+  unsigned before_c = ci - count;
+  for (int x = 0; x < THREADS / 64; ++x) {
+    if (x < wave) { before += sh.part_m[x]; before_c += sh.part_c[x]; }
+    all += sh.part_m[x];
+  }
+  Places pl;
+  pl.all = all;
+  pl.strong = strong;
+  const bool cut = set.top_p < 1.0;
+  const uint64_t border = cut ? border_of(set.top_p, all) : all - 1;
+  uint64_t mb = before;
+  unsigned cb = before_c;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (set.top_k > 0 && cb < (unsigned)set.top_k && (unsigned)set.top_k <= cb + c[i]) found[0] = tid * PER + i;
+    if (mb <= border && border < mb + m[i]) { found[1] = tid * PER + i; border_bin[0] = mb; border_bin[1] = mb + m[i]; }
+    sh.mass[tid * PER + i] = mb;
+    mb += m[i];
+    cb += c[i];
+  }
+  __syncthreads();
+  pl.last_k = found[0];
+  pl.bin_p = cut ? found[1] : -1;
+  const uint64_t least = cut ? border_bin[0] + 1 : all, most = cut ? border_bin[1] : all;
+  const uint64_t low = position_of(set.u, min(least, pl.strong)), high = position_of(set.u, min(most, pl.strong));
+  mb = before;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (mb <= low && low < mb + m[i]) found[2] = tid * PER + i;
+    if (mb <= high && high < mb + m[i]) found[3] = tid * PER + i;
+    mb += m[i];
+  }
+  __syncthreads();
+  pl.low_u = found[2];
+  pl.high_u = found[3];
+  __syncthreads();
+  return pl;
+}
+
+// The draw from the list of all labels of the bins that `pl` names, n <= kList of them.  In front of a label stand the better ones of
+// the list, and what lies in front of its bin less the listed bins there.
+template <int THREADS>
+__device__ __forceinline__ void finish_from_list(const Settings& set, const Steps& st, const Places& pl, int n, int64_t* out, Shared<THREADS>& sh) {
+  const int tid = threadIdx.x;
+  constexpr int H = kList / THREADS > 0 ? kList / THREADS : 1;
+  Entry me[H];
+  uint64_t ahead[H];
+  int bin[H];
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    const int e = tid + h * THREADS;
+    bin[h] = -1;
+    ahead[h] = 0;
+    me[h] = Entry{0, 0};
+    if (e >= n) continue;
+    me[h] = sh.list[e];
+    const int at = st.bin(value_of((unsigned)(me[h].key >> 32)), me[h].key);
+    bin[h] = at;
+    ahead[h] = sh.mass[at];
+    if (at > pl.low_u) ahead[h] -= sh.mass[min(at, pl.high_u + 1)] - sh.mass[pl.low_u];
+    if (pl.bin_p >= 0 && pl.bin_p < at && (pl.bin_p < pl.low_u || pl.bin_p > pl.high_u)) ahead[h] -= sh.mass[pl.bin_p + 1] - sh.mass[pl.bin_p];
+#pragma unroll 8
+    for (int l = 0; l < n; ++l) {
+      const Entry o = sh.list[l];
+      ahead[h] += o.key > me[h].key ? o.mass : 0;
+    }
+  }
+  uint64_t kept = pl.strong;
+  if (pl.bin_p >= 0) {
+    const uint64_t border = border_of(set.top_p, pl.all);
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+      if (bin[h] == pl.bin_p && ahead[h] <= border && border < ahead[h] + me[h].mass) sh.base_m = ahead[h] + me[h].mass;
+    __syncthreads();
+    kept = min(kept, sh.base_m);
+  }
+  const uint64_t want = position_of(set.u, kept);
+#pragma unroll
+  for (int h = 0; h < H; ++h)
+    if (bin[h] >= 0 && ahead[h] <= want && want < ahead[h] + me[h].mass) *out = (int64_t)(0xffffffffu - (unsigned)me[h].key);
+}
 
 template <class E, int THREADS>
 __device__ void draw_row(const SampleP& p, long r, Shared<THREADS>& sh) {
@@ -564,17 +683,18 @@ __device__ void draw_row(const SampleP& p, long r, Shared<THREADS>& sh) {
     return;
   }
   const Weight w = weight_of(p, set, top, sh.table);
-  Steps st = all_steps(w, top, -__builtin_inff());
+  Steps st = all_steps<THREADS>(w, top, -__builtin_inff());
   unsigned members = (unsigned)p.v;
 
   if (set.top_k > 0 && set.top_k < p.v) {
     if (set.top_k <= kPrune) {
       // a label under the top_k-th largest of 256 groups' maxima has top_k better ones: it is out
       constexpr int kGroups = 256, kGroup = THREADS / kGroups;
-      static_assert(kGroup == 1 || kGroup == 2, "a thread or a pair");
+      static_assert(kGroup == 1 || kGroup == 2 || kGroup == 4, "a thread, a pair or a quad");
       unsigned* const maxima = sh.count;
       unsigned group = mine;
-      if constexpr (kGroup == 2) group = max(group, lane_step<0xB1>(group));
+      if constexpr (kGroup >= 2) group = max(group, lane_step<0xB1>(group));
+      if constexpr (kGroup == 4) group = max(group, lane_step<0x4E>(group));
       if (threadIdx.x % kGroup == 0) maxima[threadIdx.x / kGroup] = group;
       if (threadIdx.x == 0) { sh.listed = 0; sh.bin = (int)kNothing; }
       __syncthreads();
@@ -582,9 +702,13 @@ __device__ void draw_row(const SampleP& p, long r, Shared<THREADS>& sh) {
         const unsigned me = maxima[threadIdx.x];
         int better = 0, equal = 0;
 #pragma unroll 8
-        for (int l = 0; l < kGroups; ++l) {
-          better += maxima[l] > me;
-          equal += maxima[l] == me;
+        for (int l = 0; l < kGroups / 4; ++l) {
+          const u32x4 o = reinterpret_cast<const u32x4*>(maxima)[l];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            better += o[i] > me;
+            equal += o[i] == me;
+          }
         }
         if (better < set.top_k && set.top_k <= better + equal) sh.bin = (int)me;        // (equal ones write the same)
       }
@@ -593,13 +717,11 @@ __device__ void draw_row(const SampleP& p, long r, Shared<THREADS>& sh) {
       row.each([&](float x, int i) {
         if (!(x >= bound) || x == -__builtin_inff()) return;
         const unsigned at = atomicAdd(&sh.listed, 1u);
-        if (at < (unsigned)kList) {
-          sh.list_key[at] = key_of(order_bits(x), i);
-          sh.list_mass[at] = w.of(x);
-        }
+        if (at < (unsigned)kList) sh.list[at] = Entry{key_of(order_bits(x), i), 0};
       });
       __syncthreads();
       if (sh.listed <= (unsigned)kList) {
+        weigh_list<THREADS>(w, (int)sh.listed, sh);
         draw_from_list<THREADS>(w, set, (int)sh.listed, p.out + r, sh);
         return;
       }
@@ -617,7 +739,7 @@ __device__ void draw_row(const SampleP& p, long r, Shared<THREADS>& sh) {
     members = some;
     if ((unsigned)set.top_k < some) {
       Steps by = st;
-      by.step = step_of((float)w.zmax - fmaxf(least, -1e30f));
+      by.fit_step((float)w.zmax - fmaxf(least, -1e30f));
       bool ready = false;
       st.low = find<true, THREADS>(row, w, by, some, (uint64_t)(set.top_k - 1), ready, sh).key;
       st.fit_bits();
@@ -628,18 +750,34 @@ __device__ void draw_row(const SampleP& p, long r, Shared<THREADS>& sh) {
     float least = (float)w.zmax;
     row.each([&](float x, int) { least = least_of(least, x); });
     const uint64_t low = st.low;
-    st = all_steps(w, top, value_of(block_all<THREADS, OpMin>(order_bits(least), sh)));
+    st = all_steps<THREADS>(w, top, value_of(block_all<THREADS, OpMin>(order_bits(least), sh)));
     st.low = low;
     st.fit_bits();
   }
   const double weak = reach_of(set.min_p);
   const uint64_t strong = block_all<THREADS, OpSum>(histogram<false, THREADS>(row, w, st, weak, sh), sh);
-  bool ready = true;
-  uint64_t all = 0;
-  for (int i = threadIdx.x; i < kBins; i += THREADS) all += sh.mass[i];
-  all = block_all<THREADS, OpSum>(all, sh);
-  uint64_t kept = strong;
-  if (set.top_p < 1.0) kept = min(kept, find<false, THREADS>(row, w, st, members, border_of(set.top_p, all), ready, sh).upto);
+  Places pl = places_of<THREADS>(sh.mass, sh.count, strong, set, sh);
+  if (threadIdx.x == 0) sh.listed = 0;
+  __syncthreads();
+  row.each([&](float x, int i) {
+    const unsigned b = order_bits(x);
+    if (!st.has(b, i)) return;
+    const uint64_t k = key_of(b, i);
+    const int bin = st.bin(x, k);
+    if ((bin < pl.low_u || bin > pl.high_u) && bin != pl.bin_p) return;
+    const unsigned at = atomicAdd(&sh.listed, 1u);
+    if (at < (unsigned)kList) sh.list[at] = Entry{k, 0};
+  });
+  __syncthreads();
+  if (sh.listed <= (unsigned)kList) {
+    weigh_list<THREADS>(w, (int)sh.listed, sh);
+    finish_from_list<THREADS>(set, st, pl, (int)sh.listed, p.out + r, sh);
+    return;
+  }
+  __syncthreads();
+  bool ready = false;
+  uint64_t kept = pl.strong;
+  if (set.top_p < 1.0) kept = min(kept, find<false, THREADS>(row, w, st, members, border_of(set.top_p, pl.all), ready, sh).upto);
   const Found f = find<false, THREADS>(row, w, st, members, position_of(set.u, kept), ready, sh);
   if (threadIdx.x == 0) p.out[r] = (int64_t)(0xffffffffu - (unsigned)f.key);
 }
@@ -655,12 +793,12 @@ __global__ void __launch_bounds__(THREADS, 4) sample_row_kernel(SampleP p) {
 // sum of the strong ones.  3: from the histogram, which bins the answers lie in; their labels into a list.  4: one workgroup per row
 // looks up the answers in the list.  Where the list overflows (equal logits in masses, a temperature of extremes) it draws the row
 // by itself.
-constexpr int kSplitThreads = 512, kSplitList = 4096;
+constexpr int kSplitThreads = 512, kSplitList = 4096, kSplitBins = Shared<kSplitThreads>::kBins;
 struct SplitRow {
-  uint64_t mass[kBins];
+  uint64_t mass[kSplitBins];
   uint64_t strong;
   uint64_t list[kSplitList];
-  unsigned count[kBins];
+  unsigned count[kSplitBins];
   unsigned listed, first;                 // first: the lowest index of the largest logit, where one label alone is kept
 };
 struct SplitP {
@@ -719,7 +857,7 @@ __global__ void __launch_bounds__(kSplitThreads, 4) split_best_kernel(SampleP p,
     sp.least[r * sp.parts + blockIdx.x] = least;
   }
   SplitRow& sr = sp.rows[r];                                     // cleared for the kernels behind this one
-  for (int i = blockIdx.x * kSplitThreads + threadIdx.x; i < kBins; i += sp.parts * kSplitThreads) {
+  for (int i = blockIdx.x * kSplitThreads + threadIdx.x; i < kSplitBins; i += sp.parts * kSplitThreads) {
     sr.mass[i] = 0;
     sr.count[i] = 0;
     if (i == 0) { sr.strong = 0; sr.listed = 0; sr.first = 0xffffffffu; }
@@ -743,80 +881,14 @@ __global__ void __launch_bounds__(kSplitThreads, 4) split_histogram_kernel(Sampl
   }
   fill_table(sh.table);
   const Weight w = weight_of(p, set, top, sh.table);
-  uint64_t strong = histogram<false, kSplitThreads>(row, w, all_steps(w, top, least_label(sp, r)), reach_of(set.min_p), sh);
-  for (int i = threadIdx.x; i < kBins; i += kSplitThreads)
+  uint64_t strong = histogram<false, kSplitThreads>(row, w, all_steps<kSplitThreads>(w, top, least_label(sp, r)), reach_of(set.min_p), sh);
+  for (int i = threadIdx.x; i < kSplitBins; i += kSplitThreads)
     if (sh.count[i]) {
       atomicAdd(&sr.count[i], sh.count[i]);
       atomicAdd((unsigned long long*)&sr.mass[i], (unsigned long long)sh.mass[i]);
     }
   strong = block_all<kSplitThreads, OpSum>(strong, sh);
   if (threadIdx.x == 0 && strong) atomicAdd((unsigned long long*)&sr.strong, (unsigned long long)strong);
-}
-
-// What the histogram says of a row: with a top_k that cuts, the labels of bins 0 .. last_k are the candidates; else the border of
-// top_p lies in bin_p and u's position in one of bins low_u .. high_u.  sh.mass: the weight in front of each bin.
-struct Places {
-  uint64_t all, strong;
-  int last_k, bin_p, low_u, high_u;
-};
-template <int THREADS>
-__device__ Places places_of(const SplitRow& sr, const Settings& set, Shared<THREADS>& sh) {
-  constexpr int PER = kBins / THREADS;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  uint64_t m[PER], sum = 0;
-  unsigned c[PER], count = 0;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    m[i] = sr.mass[tid * PER + i];
-    c[i] = sr.count[tid * PER + i];
-    sum += m[i];
-    count += c[i];
-  }
-  const uint64_t mi = lanes_scan<64>(sum);
-  const unsigned ci = (unsigned)lanes_scan<64>((uint64_t)count);
-  if (lane == 63) { sh.part_m[wave] = mi; sh.part_c[wave] = ci; }
-  int* const found = reinterpret_cast<int*>(&sh.count[0]);       // last_k, bin_p, low_u, high_u
-  uint64_t* const border_bin = &sh.list_mass[0];                 // weight in front of bin_p, and with it
-  if (tid == 0) found[0] = -1;
-  __syncthreads();
-  uint64_t before = mi - sum, all = 0;
-  unsigned before_c = ci - count;
-  for (int x = 0; x < THREADS / 64; ++x) {
-    if (x < wave) { before += sh.part_m[x]; before_c += sh.part_c[x]; }
-    all += sh.part_m[x];
-  }
-  Places pl;
-  pl.all = all;
-  pl.strong = sr.strong;
-  const bool cut = set.top_p < 1.0;
-  const uint64_t border = cut ? border_of(set.top_p, all) : all - 1;
-  uint64_t mb = before;
-  unsigned cb = before_c;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    if (set.top_k > 0 && cb < (unsigned)set.top_k && (unsigned)set.top_k <= cb + c[i]) found[0] = tid * PER + i;
-    if (mb <= border && border < mb + m[i]) { found[1] = tid * PER + i; border_bin[0] = mb; border_bin[1] = mb + m[i]; }
-    sh.mass[tid * PER + i] = mb;
-    mb += m[i];
-    cb += c[i];
-  }
-  __syncthreads();
-  pl.last_k = found[0];
-  pl.bin_p = cut ? found[1] : -1;
-  const uint64_t least = cut ? border_bin[0] + 1 : all, most = cut ? border_bin[1] : all;
-  const uint64_t low = position_of(set.u, min(least, pl.strong)), high = position_of(set.u, min(most, pl.strong));
-  mb = before;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    if (mb <= low && low < mb + m[i]) found[2] = tid * PER + i;
-    if (mb <= high && high < mb + m[i]) found[3] = tid * PER + i;
-    mb += m[i];
-  }
-  __syncthreads();
-  pl.low_u = found[2];
-  pl.high_u = found[3];
-  __syncthreads();
-  return pl;
 }
 
 template <class E>
@@ -827,9 +899,9 @@ __global__ void __launch_bounds__(kSplitThreads, 4) split_collect_kernel(SampleP
   const unsigned top = top_of(sp, r);
   if (top == kNothing || is_single(set)) return;
   const Weight w = weight_of(p, set, top, sh.table);             // (no weight is formed: the table stays empty)
-  const Steps st = all_steps(w, top, least_label(sp, r));
+  const Steps st = all_steps<kSplitThreads>(w, top, least_label(sp, r));
   SplitRow& sr = sp.rows[r];
-  const Places pl = places_of<kSplitThreads>(sr, set, sh);
+  const Places pl = places_of<kSplitThreads>(sr.mass, sr.count, sr.strong, set, sh);
   const int from = pl.last_k >= 0 ? 0 : pl.low_u, to = pl.last_k >= 0 ? pl.last_k : pl.high_u, also = pl.last_k >= 0 ? -1 : pl.bin_p;
   part_of<E>(p, sp, r).each([&](float x, int i) {
     if (!(x > -__builtin_inff())) return;
@@ -857,21 +929,21 @@ __global__ void __launch_bounds__(kSplitThreads, 4) split_draw_kernel(SampleP p,
   const int n = (int)min(sr.listed, (unsigned)kSplitList);
   fill_table(sh.table);
   const Weight w = weight_of(p, set, top, sh.table);
-  const Steps st = all_steps(w, top, least_label(sp, r));
-  const Places pl = places_of<kSplitThreads>(sr, set, sh);
+  const Steps st = all_steps<kSplitThreads>(w, top, least_label(sp, r));
+  const Places pl = places_of<kSplitThreads>(sr.mass, sr.count, sr.strong, set, sh);
   if (sr.listed > (unsigned)(pl.last_k >= 0 ? kList : kSplitList)) {
     __syncthreads();
     draw_row<E, kSplitThreads>(p, r, sh);
     return;
   }
-  if (pl.last_k >= 0) {
+  if (n <= kList) {
     for (int e = tid; e < n; e += kSplitThreads) {
       const uint64_t k = sr.list[e];
-      sh.list_key[e] = k;
-      sh.list_mass[e] = w.of(value_of((unsigned)(k >> 32)));
+      sh.list[e] = Entry{k, w.of(value_of((unsigned)(k >> 32)))};
     }
     __syncthreads();
-    draw_from_list<kSplitThreads>(w, set, n, p.out + r, sh);
+    if (pl.last_k >= 0) draw_from_list<kSplitThreads>(w, set, n, p.out + r, sh);
+    else finish_from_list<kSplitThreads>(set, st, pl, n, p.out + r, sh);
     return;
   }
   // the label of one bin on which a position falls
@@ -898,7 +970,7 @@ __global__ void __launch_bounds__(kSplitThreads, 4) split_draw_kernel(SampleP p,
   const int bins_u = pl.high_u - pl.low_u;
   uint64_t front_u[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) front_u[i] = sh.mass[min(pl.low_u + i, kBins - 1)];
+  for (int i = 0; i < 4; ++i) front_u[i] = sh.mass[min(pl.low_u + i, kSplitBins - 1)];
   const bool near = bins_u < 4;                                  // u's position moves over a few bins at most; else search again
   __syncthreads();
   if (pl.bin_p >= 0) kept = min(kept, look_up(pl.bin_p, front_p, border_of(set.top_p, pl.all)).upto);
@@ -927,7 +999,7 @@ inline SplitPlan split_plan(long n, int v, int vec) {
   const int pieces = v / vec;
   long parts = n > 0 ? 1024 / n : 0;
   if (parts > v / 4096) parts = v / 4096;
-  if (n > 512 || parts < 2) return SplitPlan{1, pieces};
+  if (n > 128 || parts < 2) return SplitPlan{1, pieces};
   const int per = (int)((pieces + parts - 1) / parts);
   return SplitPlan{(pieces + per - 1) / per, per};
 }
@@ -966,8 +1038,10 @@ int launch_sample(const SampleP& p, void* workspace, hipStream_t s) {
       hipLaunchKernelGGL((split_draw_kernel<E>), dim3((unsigned)p.n), block, 0, s, p, sp);
     } else if (p.v <= 4096) {
       hipLaunchKernelGGL((sample_row_kernel<E, 256>), dim3((unsigned)p.n), dim3(256), 0, s, p);
-    } else {
+    } else if (p.n > 256) {                                      // two of these on a CU, one of the larger
       hipLaunchKernelGGL((sample_row_kernel<E, 512>), dim3((unsigned)p.n), dim3(512), 0, s, p);
+    } else {
+      hipLaunchKernelGGL((sample_row_kernel<E, 1024>), dim3((unsigned)p.n), dim3(1024), 0, s, p);
     }
   }
 #undef OBJ_SORTED
