@@ -25,6 +25,7 @@ namespace objnerf {
 namespace {
 
 constexpr int kList = 512, kPrune = 128;
+constexpr int64_t kOpen = -2;             // between two kernels of a call: this row is still to be drawn
 
 struct SampleP {
   long n;
@@ -295,15 +296,15 @@ struct Shared {
   uint64_t red[THREADS / 64];
   uint64_t part_m[THREADS / 64];
   unsigned part_c[THREADS / 64];
-  unsigned listed;
+  unsigned listed, bound;
   int bin;
   unsigned base_c, in_bin;
   uint64_t base_m;
   Found found;
 };
 
-template <int THREADS, class OP, class T>
-__device__ __forceinline__ T block_all(T v, Shared<THREADS>& sh) {
+template <int THREADS, class OP, class T, class SH>
+__device__ __forceinline__ T block_all(T v, SH& sh) {
   v = lanes_reduce<64, OP>(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6] = (uint64_t)v;
@@ -482,14 +483,14 @@ __device__ Found find(const ROW& row, const Weight& w, Steps st, unsigned member
 }
 
 // weights of the list's labels (here and not where they are found: every lane has one to work on)
-template <int THREADS> __device__ __forceinline__ void weigh_list(const Weight& w, int n, Shared<THREADS>& sh) {
+template <int THREADS, class SH> __device__ __forceinline__ void weigh_list(const Weight& w, int n, SH& sh) {
   for (int e = threadIdx.x; e < n; e += THREADS) sh.list[e].mass = w.of(value_of((unsigned)(sh.list[e].key >> 32)));
   __syncthreads();
 }
 
 // The whole draw among the n labels of the list, of which the top_k count.
-template <int THREADS>
-__device__ __forceinline__ void draw_from_list(const Weight& w, const Settings& set, int n, int64_t* out, Shared<THREADS>& sh) {
+template <int THREADS, class SH>
+__device__ __forceinline__ void draw_from_list(const Weight& w, const Settings& set, int n, int64_t* out, SH& sh) {
   const int tid = threadIdx.x;
   constexpr int H = kList / THREADS > 0 ? kList / THREADS : 1;     // labels per thread
   uint64_t key[H], own[H], before[H];
@@ -660,8 +661,51 @@ __device__ __forceinline__ void finish_from_list(const Settings& set, const Step
     if (bin[h] >= 0 && ahead[h] <= want && want < ahead[h] + me[h].mass) *out = (int64_t)(0xffffffffu - (unsigned)me[h].key);
 }
 
+// Rows of which a few labels at most are kept (top_k <= kPrune).  A label under the top_k-th largest of 256 groups' maxima has top_k better
+// ones: it is out, and about top_k labels are left.  False where more are left than the list takes (equal logits in masses).
+template <int THREADS, class ROW, class SH>
+__device__ __forceinline__ bool draw_top(const ROW& row, const Weight& w, const Settings& set, unsigned mine, unsigned* maxima, int64_t* out, SH& sh) {
+  constexpr int kGroups = 256, kGroup = THREADS / kGroups;
+  static_assert(kGroup == 1 || kGroup == 2 || kGroup == 4, "a thread, a pair or a quad");
+  const int tid = threadIdx.x;
+  unsigned group = mine;
+  if constexpr (kGroup >= 2) group = max(group, lane_step<0xB1>(group));
+  if constexpr (kGroup == 4) group = max(group, lane_step<0x4E>(group));
+  if (tid % kGroup == 0) maxima[tid / kGroup] = group;
+  if (tid == 0) { sh.listed = 0; sh.bound = kNothing; }
+  __syncthreads();
+  if (tid < kGroups) {
+    const unsigned me = maxima[tid];
+    int better = 0, equal = 0;
+#pragma unroll 4
+    for (int l = 0; l < kGroups / 4; ++l) {
+      const u32x4 o = reinterpret_cast<const u32x4*>(maxima)[l];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        better += o[i] > me;
+        equal += o[i] == me;
+      }
+    }
+    if (better < set.top_k && set.top_k <= better + equal) sh.bound = me;        // (equal ones write the same)
+  }
+  __syncthreads();
+  const float bound = value_of(sh.bound);                        // -inf: fewer groups with a label than top_k
+  row.each([&](float x, int i) {
+    if (!(x >= bound) || x == -__builtin_inff()) return;
+    const unsigned at = atomicAdd(&sh.listed, 1u);
+    if (at < (unsigned)kList) sh.list[at] = Entry{key_of(order_bits(x), i), 0};
+  });
+  __syncthreads();
+  const unsigned n = sh.listed;
+  __syncthreads();                                               // everybody has read it
+  if (n > (unsigned)kList) return false;
+  weigh_list<THREADS>(w, (int)n, sh);
+  draw_from_list<THREADS>(w, set, (int)n, out, sh);
+  return true;
+}
+
 template <class E, int THREADS>
-__device__ void draw_row(const SampleP& p, long r, Shared<THREADS>& sh) {
+__device__ void draw_row(const SampleP& p, long r, bool rest, Shared<THREADS>& sh) {
   const RowInMemory<E, THREADS> row{static_cast<const char*>(p.z) + r * p.ldz * E::kBytes, p.v};
   const Settings set = settings_of(p, r);
   fill_table(sh.table);
@@ -687,46 +731,7 @@ __device__ void draw_row(const SampleP& p, long r, Shared<THREADS>& sh) {
   unsigned members = (unsigned)p.v;
 
   if (set.top_k > 0 && set.top_k < p.v) {
-    if (set.top_k <= kPrune) {
-      // a label under the top_k-th largest of 256 groups' maxima has top_k better ones: it is out
-      constexpr int kGroups = 256, kGroup = THREADS / kGroups;
-      static_assert(kGroup == 1 || kGroup == 2 || kGroup == 4, "a thread, a pair or a quad");
-      unsigned* const maxima = sh.count;
-      unsigned group = mine;
-      if constexpr (kGroup >= 2) group = max(group, lane_step<0xB1>(group));
-      if constexpr (kGroup == 4) group = max(group, lane_step<0x4E>(group));
-      if (threadIdx.x % kGroup == 0) maxima[threadIdx.x / kGroup] = group;
-      if (threadIdx.x == 0) { sh.listed = 0; sh.bin = (int)kNothing; }
-      __syncthreads();
-      if (threadIdx.x < kGroups) {
-        const unsigned me = maxima[threadIdx.x];
-        int better = 0, equal = 0;
-#pragma unroll 8
-        for (int l = 0; l < kGroups / 4; ++l) {
-          const u32x4 o = reinterpret_cast<const u32x4*>(maxima)[l];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            better += o[i] > me;
-            equal += o[i] == me;
-          }
-        }
-        if (better < set.top_k && set.top_k <= better + equal) sh.bin = (int)me;        // (equal ones write the same)
-      }
-      __syncthreads();
-      const float bound = value_of((unsigned)sh.bin);            // -inf: fewer groups with a label than top_k
-      row.each([&](float x, int i) {
-        if (!(x >= bound) || x == -__builtin_inff()) return;
-        const unsigned at = atomicAdd(&sh.listed, 1u);
-        if (at < (unsigned)kList) sh.list[at] = Entry{key_of(order_bits(x), i), 0};
-      });
-      __syncthreads();
-      if (sh.listed <= (unsigned)kList) {
-        weigh_list<THREADS>(w, (int)sh.listed, sh);
-        draw_from_list<THREADS>(w, set, (int)sh.listed, p.out + r, sh);
-        return;
-      }
-      __syncthreads();                                           // sh.listed has been read
-    }
+    if (set.top_k <= kPrune && !rest && draw_top<THREADS>(row, w, set, mine, sh.count, p.out + r, sh)) return;
     unsigned some = 0;
     float least = (float)w.zmax;
     row.each([&](float x, int) {
@@ -783,9 +788,41 @@ __device__ void draw_row(const SampleP& p, long r, Shared<THREADS>& sh) {
 }
 
 template <class E, int THREADS>
-__global__ void __launch_bounds__(THREADS, 4) sample_row_kernel(SampleP p) {
+__global__ void __launch_bounds__(THREADS, 4) sample_row_kernel(SampleP p, bool rest) {
   __shared__ Shared<THREADS> sh;
-  draw_row<E, THREADS>(p, blockIdx.x, sh);
+  if (rest && p.out[blockIdx.x] != kOpen) return;                // sample_top_kernel has drawn it
+  draw_row<E, THREADS>(p, blockIdx.x, rest, sh);
+}
+
+// Such rows in a kernel of their own: two light passes and a list, many rows at a time on a CU.  Rows of other settings, and rows with
+// more left than the list takes, are marked for sample_row_kernel.
+template <class E>
+__global__ void __launch_bounds__(256, 6) sample_top_kernel(SampleP p) {
+  __shared__ struct {
+    __align__(16) unsigned maxima[256];
+    Entry list[kList];
+    double table[32];
+    uint64_t red[4];
+    unsigned listed, bound;
+  } sh;
+  const long r = blockIdx.x;
+  Settings set = settings_of(p, r);
+  if (is_single(set)) set.top_k = 1;
+  if (set.top_k < 1 || set.top_k > kPrune) {
+    if (threadIdx.x == 0) p.out[r] = kOpen;
+    return;
+  }
+  const RowInMemory<E, 256> row{static_cast<const char*>(p.z) + r * p.ldz * E::kBytes, p.v};
+  fill_table(sh.table);
+  float most = -__builtin_inff();
+  row.each([&](float x, int) { most = fmaxf(most, x); });
+  const unsigned mine = order_bits(most), top = block_all<256, OpMax>(mine, sh);
+  if (top == kNothing) {
+    if (threadIdx.x == 0) p.out[r] = -1;
+    return;
+  }
+  const Weight w = weight_of(p, set, top, sh.table);
+  if (!draw_top<256>(row, w, set, mine, sh.maxima, p.out + r, sh) && threadIdx.x == 0) p.out[r] = kOpen;
 }
 
 // ---- few long rows: a row's passes spread over several workgroups, one kernel per pass ----
@@ -933,7 +970,7 @@ __global__ void __launch_bounds__(kSplitThreads, 4) split_draw_kernel(SampleP p,
   const Places pl = places_of<kSplitThreads>(sr.mass, sr.count, sr.strong, set, sh);
   if (sr.listed > (unsigned)(pl.last_k >= 0 ? kList : kSplitList)) {
     __syncthreads();
-    draw_row<E, kSplitThreads>(p, r, sh);
+    draw_row<E, kSplitThreads>(p, r, false, sh);
     return;
   }
   if (n <= kList) {
@@ -1036,12 +1073,16 @@ int launch_sample(const SampleP& p, void* workspace, hipStream_t s) {
       hipLaunchKernelGGL((split_histogram_kernel<E>), grid, block, 0, s, p, sp);
       hipLaunchKernelGGL((split_collect_kernel<E>), grid, block, 0, s, p, sp);
       hipLaunchKernelGGL((split_draw_kernel<E>), dim3((unsigned)p.n), block, 0, s, p, sp);
-    } else if (p.v <= 4096) {
-      hipLaunchKernelGGL((sample_row_kernel<E, 256>), dim3((unsigned)p.n), dim3(256), 0, s, p);
-    } else if (p.n > 256) {                                      // two of these on a CU, one of the larger
-      hipLaunchKernelGGL((sample_row_kernel<E, 512>), dim3((unsigned)p.n), dim3(512), 0, s, p);
     } else {
-      hipLaunchKernelGGL((sample_row_kernel<E, 1024>), dim3((unsigned)p.n), dim3(1024), 0, s, p);
+      // a kernel for small top_k pays where rows wait for a place on the card (2048 rows of 32768 bf16, top_k 50: 80 -> 57 us); where
+      // all are on it at once, a second kernel only follows the first (257 rows of 30011, some with a top_k: 46 -> 62 us)
+      const bool small = p.t || p.top_k || !(p.t0 > 0.0) || (p.top_k0 >= 1 && p.top_k0 <= kPrune), light = small && p.n > 512;
+      const dim3 grid((unsigned)p.n);
+      if (light) hipLaunchKernelGGL((sample_top_kernel<E>), grid, dim3(256), 0, s, p);
+      // one workgroup of 1,024 threads to a CU, two of 512: the larger where that is a row's CU to itself
+      if (p.v <= 4096) hipLaunchKernelGGL((sample_row_kernel<E, 256>), grid, dim3(256), 0, s, p, light);
+      else if (p.n > 256) hipLaunchKernelGGL((sample_row_kernel<E, 512>), grid, dim3(512), 0, s, p, light);
+      else hipLaunchKernelGGL((sample_row_kernel<E, 1024>), grid, dim3(1024), 0, s, p, light);
     }
   }
 #undef OBJ_SORTED
