@@ -629,6 +629,7 @@ int objnerf_repeat_rows(const float* src, int64_t lds, int64_t n_rows, int C, in
 #define OBJNERF_TYPE_F32 0
 #define OBJNERF_TYPE_BF16 1
 #define OBJNERF_TYPE_F16 2
+#define OBJNERF_TYPE_FP8 3        /* e4m3 with block scales, as objnerf_fp8_quantize writes it */
 
 /* Distillation from a teacher's top logits.  Per row: p = softmax(teacher / T) over the slots whose index lies in [0, v) (any other
  * index: an empty slot; so is a teacher value of -inf), q = softmax(student / T) over the v logits,
@@ -697,14 +698,16 @@ int objnerf_fp8_quantize(const objnerf_fp8_quantize_args* args, void* stream);
  * C in fp32: fp32 sums throughout. */
 typedef struct {
   int64_t M, N, K;           /* M, N < 2^31; K <= 2^26 */
-  const uint8_t* a; int64_t a_stride; const uint8_t* a_scale; int64_t a_scale_stride;
+  int32_t a_type, _pad;      /* OBJNERF_TYPE_FP8, or the type of an `a` that the product rounds on its way (blocks of one row) */
+  const void* a; int64_t a_stride; const uint8_t* a_scale; int64_t a_scale_stride;
+  int64_t a_cols;            /* a to be rounded: its columns (a_stride in elements, no a_scale); K = a_cols filled up to whole blocks */
   const uint8_t* b; int64_t b_stride; const uint8_t* b_scale; int64_t b_scale_stride;
   const float* bias;         /* (N) or NULL */
   int32_t leaky, c_type;     /* OBJNERF_TYPE_* */
   void* c; int64_t c_stride;
   float* workspace;          /* objnerf_gemm_fp8_workspace_floats() (0: may be NULL): sums over a long K are split and joined in order */
 } objnerf_gemm_fp8_args;
-int64_t objnerf_gemm_fp8_workspace_floats(int64_t M, int64_t N, int64_t K, int c_type);
+int64_t objnerf_gemm_fp8_workspace_floats(int64_t M, int64_t N, int64_t K, int a_type, int c_type);
 int objnerf_gemm_fp8(const objnerf_gemm_fp8_args* args, void* stream);
 
 /* ---- measurement hooks (bench.py): HIP-event timing of the MLP kernel on `stream` ---- */

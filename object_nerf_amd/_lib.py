@@ -209,7 +209,8 @@ class Fp8QuantizeArgs(C.Structure):
 class GemmFp8Args(C.Structure):
     _fields_ = [
         ("M", C.c_int64), ("N", C.c_int64), ("K", C.c_int64),
-        ("a", C.c_void_p), ("a_stride", C.c_int64), ("a_scale", C.c_void_p), ("a_scale_stride", C.c_int64),
+        ("a_type", C.c_int32), ("_pad", C.c_int32),
+        ("a", C.c_void_p), ("a_stride", C.c_int64), ("a_scale", C.c_void_p), ("a_scale_stride", C.c_int64), ("a_cols", C.c_int64),
         ("b", C.c_void_p), ("b_stride", C.c_int64), ("b_scale", C.c_void_p), ("b_scale_stride", C.c_int64),
         ("bias", C.c_void_p), ("leaky", C.c_int32), ("c_type", C.c_int32), ("c", C.c_void_p), ("c_stride", C.c_int64),
         ("workspace", C.c_void_p),
@@ -287,7 +288,7 @@ SIGNATURES = {
     "objnerf_distill_top": (C.c_int, [C.POINTER(DistillArgs), _VP]),
     "objnerf_fp8_quantize_workspace_floats": (C.c_int64, [C.c_int64, C.c_int64]),
     "objnerf_fp8_quantize": (C.c_int, [C.POINTER(Fp8QuantizeArgs), _VP]),
-    "objnerf_gemm_fp8_workspace_floats": (C.c_int64, [C.c_int64, C.c_int64, C.c_int64, C.c_int]),
+    "objnerf_gemm_fp8_workspace_floats": (C.c_int64, [C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int]),
     "objnerf_gemm_fp8": (C.c_int, [C.POINTER(GemmFp8Args), _VP]),
     "objnerf_sample_logits_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int32, C.c_int]),
     "objnerf_sample_logits": (C.c_int, [C.POINTER(SampleArgs), _VP]),

@@ -22,6 +22,7 @@
 #include "host_api.h"
 #include "device_math.h"
 #include "label_ops.h"
+#include <type_traits>
 
 namespace objnerf {
 namespace {
@@ -243,7 +244,8 @@ int launch_quantize(const QuantP& p, bool square, float* sum, hipStream_t s) {
 
 struct GemmP {
   long M, N, K;                            // K: whole blocks
-  const uint8_t* a; long lda; const uint8_t* sa; long ldsa;
+  const uint8_t* a; long lda; const uint8_t* sa; long ldsa;      // a not yet rounded: elements (M, cols), lda in elements, no sa
+  long cols;
   const uint8_t* b; long ldb; const uint8_t* sb; long ldsb;
   const float* bias;
   int leaky;
@@ -309,19 +311,20 @@ template <int BM, int BN> __device__ __forceinline__ void tile_of(const GemmP& p
 // The copies of a workgroup's rows from memory straight into LDS.  A step is one block of 128: BM + BN rows of 128 bytes into one of two
 // slots.  The 16-byte pieces of a row are permuted (piece_key) on the addresses the lanes read from, since LDS is filled in order.  Scales:
 // a dword of each row, four steps' worth, into two slots of their own; a wave copies those of 64 rows.
-template <int BM, int BN, int WAVES> struct Copies {
-  static constexpr int kSlot = (BM + BN) * kBlock, kBytes = 2 * kSlot + 2 * (BM + BN) * 4;
-  static constexpr int RA = BM / WAVES / 8, RB = BN / WAVES / 8, kScaleCopies = (BM + BN) / 64 / WAVES;
-  static_assert((BM + BN) / 64 % WAVES == 0, "whole copies of 64 rows' scales per wave");
+template <int BM, int BN, int WAVES, bool RAW> struct Copies {
+  static constexpr int kScaleRows = (BM + BN + 63) / 64 * 64, kScaleCopies = (kScaleRows / 64 + WAVES - 1) / WAVES;
+  static constexpr int kSlot = (BM + BN) * kBlock, kBytes = 2 * kSlot + 2 * kScaleRows * 4;
+  static constexpr int RA = RAW ? 0 : BM / WAVES / 8, RB = BN / WAVES / 8;
+  static_assert((RAW || BM % (8 * WAVES) == 0) && BN % (8 * WAVES) == 0, "whole groups of 8 rows per wave");
   const uint8_t *abase, *bbase, *sbase[kScaleCopies];
-  unsigned aoff[RA], boff[RB];
+  unsigned aoff[RA + 1], boff[RB];
   long first;
   lds_byte* lds;
   __device__ __forceinline__ Copies(const GemmP& p, long m0, long n0, long first_block, lds_byte* ring) : first(first_block), lds(ring) {
     const int lane = threadIdx.x & 63, wave = uni((int)(threadIdx.x >> 6));
     // this lane's part: row lane / 8 of every 8, piece lane % 8 of LDS
     const long arow = min(m0 + wave * RA * 8, p.M - 1), brow = min(n0 + wave * RB * 8, p.N - 1);
-    abase = p.a + arow * p.lda + first * kBlock;
+    abase = RAW ? nullptr : p.a + arow * p.lda + first * kBlock;
     bbase = p.b + brow * p.ldb + first * kBlock;
 #pragma unroll
     for (int c = 0; c < RA; ++c) {
@@ -335,8 +338,8 @@ template <int BM, int BN, int WAVES> struct Copies {
     }
 #pragma unroll
     for (int c = 0; c < kScaleCopies; ++c) {
-      const int r = (wave * kScaleCopies + c) * 64 + lane;
-      sbase[c] = r < BM ? p.sa + min(m0 + r, p.M - 1) * p.ldsa : p.sb + min(n0 + r - BM, p.N - 1) * p.ldsb;
+      const int r = (c * WAVES + wave) * 64 + lane;
+      sbase[c] = r < BM && !RAW ? p.sa + min(m0 + r, p.M - 1) * p.ldsa : p.sb + max(min(n0 + r - BM, p.N - 1), 0l) * p.ldsb;
     }
   }
   __device__ __forceinline__ void rows(long step) const {
@@ -352,19 +355,74 @@ template <int BM, int BN, int WAVES> struct Copies {
     for (int c = 0; c < RB; ++c)
       __builtin_amdgcn_global_load_lds((global_byte*)(from + boff[c]), (__attribute__((address_space(3))) void*)(slot + c * 1024), 16, 0, 0);
   }
+  // (a's rows where it is rounded here: their dwords are another wave's stores, the copy starts behind them)
   __device__ __forceinline__ void scales(long step) const {
-    const int wave = uni((int)(threadIdx.x >> 6));
+    const int wave = uni((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     const long group = (first + step) >> 2;
 #pragma unroll
-    for (int c = 0; c < kScaleCopies; ++c)
-      __builtin_amdgcn_global_load_lds((global_byte*)(sbase[c] + group * 4), (__attribute__((address_space(3))) void*)(lds + 2 * kSlot + ((int)(group & 1) * (BM + BN) + (wave * kScaleCopies + c) * 64) * 4), 4, 0, 0);
+    for (int c = 0; c < kScaleCopies; ++c) {
+      const int from = (c * WAVES + wave) * 64;
+      if (from >= kScaleRows || (RAW && from + 64 <= BM)) continue;
+      if (RAW && from < BM && from + lane < BM) continue;        // lanes of a's rows copy nothing: their places stay as they are
+      __builtin_amdgcn_global_load_lds((global_byte*)(sbase[c] + group * 4), (__attribute__((address_space(3))) void*)(lds + 2 * kSlot + ((int)(group & 1) * kScaleRows + from) * 4), 4, 0, 0);
+    }
   }
   // scale byte of row 0 of the tile in this step; rows are 4 bytes apart, b's rows behind a's
   __device__ __forceinline__ const lds_byte* scale_at(long step) const {
     const long at = first + step;
-    return lds + 2 * kSlot + ((int)(at >> 2 & 1) * (BM + BN)) * 4 + (int)(at & 3);
+    return lds + 2 * kSlot + (int)(at >> 2 & 1) * kScaleRows * 4 + (int)(at & 3);
   }
 };
+// a's rows of a step where they are rounded on their way into LDS: 16 lanes per row and block, held in registers from the load to the
+// store, so that the step in between hides the load.
+template <class A, int BM, int THREADS, class COPY> struct RawRows {
+  static constexpr int kPasses = BM * 16 / THREADS, kPieces = 8 / A::kVec;
+  u32x4 held[kPasses][kPieces];
+  __device__ __forceinline__ void load(const GemmP& p, long m0, long block) {
+    const int l = threadIdx.x & 15, g = threadIdx.x >> 4;
+    const long c = block * kBlock + l * 8;
+#pragma unroll
+    for (int s = 0; s < kPasses; ++s) {
+      const char* row = reinterpret_cast<const char*>(p.a) + min(m0 + s * (THREADS / 16) + g, p.M - 1) * p.lda * A::kBytes;
+      if (c + 8 <= p.cols) {
+#pragma unroll
+        for (int h = 0; h < kPieces; ++h) held[s][h] = load16(row, (c + h * A::kVec) * A::kBytes);
+      } else {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = c + i < p.cols ? A::load(row, c + i) : 0.f;
+#pragma unroll
+        for (int h = 0; h < kPieces; ++h) held[s][h] = A::pack(x + h * A::kVec);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(const COPY& copy, long step) const {
+    const int l = threadIdx.x & 15, g = threadIdx.x >> 4;
+    lds_byte* const rows = copy.lds + (int)(step & 1) * COPY::kSlot;
+    lds_byte* const scale = const_cast<lds_byte*>(copy.scale_at(step));
+#pragma unroll
+    for (int s = 0; s < kPasses; ++s) {
+      float x[8];
+#pragma unroll
+      for (int h = 0; h < kPieces; ++h) A::unpack(held[s][h], x + h * A::kVec);
+      float largest = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) largest = fmaxf(largest, finite_abs(x[i]));
+      const unsigned byte = scale_byte(lanes_reduce<16, OpMax>(largest));
+      const float inv = inverse_scale(byte);
+      typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+      const u32x2 o = {fp8x4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv), fp8x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv)};
+      const int r = s * (THREADS / 16) + g;
+      *(__attribute__((address_space(3))) u32x2*)(rows + r * kBlock + (((l >> 1) ^ piece_key(r)) << 4) + (l & 1) * 8) = o;
+      if (l == 0) scale[r * 4] = (uint8_t)byte;
+    }
+  }
+};
+struct NoRaw {
+  template <class... T> __device__ __forceinline__ void load(T...) {}
+  template <class... T> __device__ __forceinline__ void store(T...) const {}
+};
+
 // a lane's 32 bytes of a fragment: row i of the 16 rows at `rows`, the h-th run of 32 of the block
 __device__ __forceinline__ i32x8 fragment(const lds_byte* rows, int i, int h) {
   const int key = piece_key(i);
@@ -376,61 +434,66 @@ __device__ __forceinline__ f32x4 mfma8(i32x8 b, i32x8 a, f32x4 c, int sb, int sa
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, 0, 0, 0, sb, 0, sa);
 }
 
-// A wave's TM x TN tiles of 16 x 16 to memory: lane (i, h) holds columns 4 h .. 4 h + 3 of row i of each.
+// A wave's TM x TN tiles of 16 x 16 to memory, 16 rows at a time through 16 x (16 TN + 4) floats of LDS that are the wave's own (it serves
+// a wave's accesses in order: no barrier), so that neighbouring lanes store neighbouring 16 bytes of a row.
 template <class E, int TM, int TN>
-__device__ __forceinline__ void write_tile(const GemmP& p, long m0, long n0, bool whole, const f32x4 (&acc)[TM][TN]) {
-  const int i = threadIdx.x & 15, h = threadIdx.x >> 4 & 3;
-  if (!p.partial && whole) {                                     // no questions
-    char* c = static_cast<char*>(p.c) + ((m0 + i) * p.ldc + n0 + h * 4) * E::kBytes;
-    const long down = 16 * p.ldc * E::kBytes;
+__device__ __forceinline__ void write_tile(const GemmP& p, long m0, long n0, lds_byte* area, const f32x4 (&acc)[TM][TN]) {
+  typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+  constexpr int kPitch = TN * 16 + 4, kLanes = TN * 16 / E::kVec, kRows = 64 / kLanes;       // lanes per row, rows at once
+  const int lane = threadIdx.x & 63, i = lane & 15, h = lane >> 4, c = lane % kLanes * E::kVec;
+  const long n = n0 + c;
+  const int have = (int)min(max(p.N - n, 0l), (long)E::kVec);    // columns of this lane that exist
+  float bias[E::kVec];
 #pragma unroll
-    for (int u = 0; u < TM; ++u, c += down)
+  for (int e = 0; e < E::kVec; ++e) bias[e] = p.bias && e < have ? p.bias[n + e] : 0.f;
 #pragma unroll
-      for (int t = 0; t < TN; ++t) {
-        float bias[4] = {0.f, 0.f, 0.f, 0.f};
-        if (p.bias)
+  for (int u = 0; u < TM; ++u) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) bias[r] = p.bias[n0 + t * 16 + h * 4 + r];
-        f32x4 v;
+    for (int t = 0; t < TN; ++t) *(lds_f32x4*)(area + (i * kPitch + t * 16 + h * 4) * 4) = acc[u][t];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+    for (int r = lane / kLanes; r < 16; r += kRows) {
+      const long m = m0 + u * 16 + r;
+      if (m >= p.M || have == 0) continue;
+      float x[E::kVec];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = finished(acc[u][t][r], p, bias[r]);
-        write4<E>(c + t * 16 * E::kBytes, v);
+      for (int q = 0; q < E::kVec / 4; ++q) {
+        const f32x4 v = *(const lds_f32x4*)(area + (r * kPitch + c + q * 4) * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[q * 4 + e] = v[e];
       }
-    return;
-  }
-#pragma unroll
-  for (int t = 0; t < TN; ++t) {
-    const long n = n0 + t * 16 + h * 4;
-    if (n >= p.N) continue;
-    float bias[4] = {0.f, 0.f, 0.f, 0.f};
-    if (p.bias && !p.partial)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) bias[r] = n + r < p.N ? p.bias[n + r] : 0.f;
-#pragma unroll
-    for (int u = 0; u < TM; ++u) {
-      const long m = m0 + u * 16 + i;
-      if (m >= p.M) continue;
       if (p.partial) {
         float* o = p.partial + ((long)blockIdx.y * p.M + m) * p.N + n;
+        if (have == E::kVec) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (n + r < p.N) o[r] = acc[u][t][r];
+          for (int q = 0; q < E::kVec / 4; ++q) store16(o, q * 16, u32x4{__float_as_uint(x[q * 4]), __float_as_uint(x[q * 4 + 1]), __float_as_uint(x[q * 4 + 2]), __float_as_uint(x[q * 4 + 3])});
+        } else {
+#pragma unroll 1
+          for (int e = 0; e < have; ++e) o[e] = *(const __attribute__((address_space(3))) float*)(area + (r * kPitch + c + e) * 4);
+        }
         continue;
       }
-      f32x4 v;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = finished(acc[u][t][r], p, bias[r]);
-      store4<E>(p, m, n, v);
+      for (int e = 0; e < E::kVec; ++e) x[e] = finished(x[e], p, bias[e]);
+      char* o = static_cast<char*>(p.c) + (m * p.ldc + n) * E::kBytes;
+      if (have == E::kVec) store16(o, 0, E::pack(x));
+      else
+#pragma unroll
+        for (int e = 0; e < E::kVec; ++e)
+          if (e < have) E::store(o, e, x[e]);
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
 
 // BM x BN of C per workgroup of WM x WN waves, rows copied one step ahead, one barrier a step.  The instruction's "A" is b's rows and its
 // "B" a's: a lane's four results are four neighbouring columns of one row of C.  In the widened form the four instructions of a
 // block take 8 bytes of every lane's 32 each: another order of the same sum.
-template <class E, bool WIDE, int BM, int BN, int WM, int WN>
+template <class E, class A, bool WIDE, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(WM * WN * 64, 2) gemm_fp8_kernel(GemmP p) {
-  using Copy = Copies<BM, BN, WM * WN>;
+  constexpr bool kRaw = !std::is_same<A, void>::value;
+  using Copy = Copies<BM, BN, WM * WN, kRaw>;
+  using Raw = typename std::conditional<kRaw, RawRows<typename std::conditional<kRaw, A, ElemF32>::type, BM, WM * WN * 64, Copy>, NoRaw>::type;
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
   __shared__ __align__(16) uint8_t ring[Copy::kBytes];           // one object: the copies' waits stay with the barrier
   long m0, n0;
@@ -441,13 +504,17 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) gemm_fp8_kernel(GemmP p) {
   const Copy copy(p, m0, n0, first, (lds_byte*)ring);
 
   f32x4 acc[TM][TN] = {};
+  Raw raw;
   if (steps > 0) {
+    raw.load(p, m0, first);
     copy.rows(0);
     copy.scales(0);
+    raw.store(copy, 0l);
   }
   for (long step = 0; step < steps; ++step) {
     __syncthreads();                                             // the step's rows have landed; the other slot has been read
     if (step + 1 < steps) {
+      raw.load(p, m0, first + step + 1);
       copy.rows(step + 1);
       if (((first + step) & 3) == 3) copy.scales(step + 1);
     }
@@ -486,8 +553,11 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) gemm_fp8_kernel(GemmP p) {
         for (int u = 0; u < TM; ++u) acc[u][t] = mfma8(fb, fa[u], acc[u][t], sb, sa[u]);
       }
     }
+    if (step + 1 < steps) raw.store(copy, step + 1);
   }
-  write_tile<E, TM, TN>(p, m0 + wm, n0 + wn, m0 + BM <= p.M && n0 + BN <= p.N, acc);
+  static_assert(WM * WN * 16 * (TN * 16 + 4) * 4 <= Copy::kBytes, "the waves' areas fit where the rows lay");
+  __syncthreads();
+  write_tile<E, TM, TN>(p, m0 + wm, n0 + wn, copy.lds + wave * 16 * (TN * 16 + 4) * 4, acc);
 }
 
 // C from the partial sums of the splits, in their order
@@ -508,35 +578,43 @@ __global__ void __launch_bounds__(256) join_splits_kernel(GemmP p, int splits) {
   store4<E>(p, m, n, v);
 }
 
-// Tile and split of a product.  256 x 256 per workgroup (one per CU, 128 KB of LDS) where such tiles fill the card and the sum is long
-// enough to run behind its copies; else 128 x 128 (two per CU), with the sum split where there are fewer tiles than places.
-struct Plan { bool big; int splits; long blocks; };
-inline Plan plan_of(long M, long N, long K, bool wide) {
+// Tile and split of a product.  Up to 32 rows: 32 x 128 per workgroup.  256 x 256 (one workgroup per CU, 128 KB of LDS) where such tiles
+// fill the card and the sum is long enough to run behind its copies.  Else 128 x 128, two workgroups per CU.  The sum is split
+// where there are fewer tiles than places.
+struct Plan { int bm, bn, splits; long blocks; };
+inline Plan plan_of(long M, long N, long K, bool wide, bool raw) {
   const long blocks = K / kBlock;
-  if (!wide && blocks >= 8 && ((M + 255) / 256) * ((N + 255) / 256) >= 224) return Plan{true, 1, blocks};
-  const long tiles = ((M + 127) / 128) * ((N + 127) / 128);
+  if (!wide && !raw && blocks >= 8 && ((M + 255) / 256) * ((N + 255) / 256) >= 224) return Plan{256, 256, 1, blocks};
+  const int bm = M <= 32 ? 32 : 128;
+  const long tiles = ((M + bm - 1) / bm) * ((N + 127) / 128);
   long splits = tiles >= 256 ? 1 : 512 / tiles;                  // two workgroups per CU
   splits = splits < blocks / 4 ? splits : blocks / 4;            // of at least four blocks each
-  if (splits < 2) return Plan{false, 1, blocks};
+  if (splits < 2) return Plan{bm, 128, 1, blocks};
   const long per = (blocks + splits - 1) / splits;
-  return Plan{false, (int)((blocks + per - 1) / per), per};
+  return Plan{bm, 128, (int)((blocks + per - 1) / per), per};
 }
 
-template <class E>
+template <class E, class A>
 int launch_gemm_fp8(GemmP p, float* workspace, hipStream_t s) {
-  constexpr bool wide = E::kBytes == 4;
-  const Plan plan = plan_of(p.M, p.N, p.K, wide);
+  constexpr bool wide = E::kBytes == 4, raw = !std::is_same<A, void>::value;
+  const Plan plan = plan_of(p.M, p.N, p.K, wide, raw);
   p.blocks_per_split = plan.blocks;
   p.partial = plan.splits > 1 ? workspace : nullptr;
-  if (plan.big) {
-    if constexpr (!wide)
-      hipLaunchKernelGGL((gemm_fp8_kernel<E, false, 256, 256, 2, 4>), dim3((unsigned)(((p.M + 255) / 256) * ((p.N + 255) / 256))), dim3(512), 0, s, p);
+  const dim3 grid((unsigned)(((p.M + plan.bm - 1) / plan.bm) * ((p.N + plan.bn - 1) / plan.bn)), (unsigned)plan.splits);
+  if (plan.bm == 256) {
+    if constexpr (!wide && !raw) hipLaunchKernelGGL((gemm_fp8_kernel<E, A, false, 256, 256, 2, 4>), grid, dim3(512), 0, s, p);
+  } else if (plan.bm == 32) {
+    hipLaunchKernelGGL((gemm_fp8_kernel<E, A, wide, 32, 128, 1, 4>), grid, dim3(256), 0, s, p);
   } else {
-    hipLaunchKernelGGL((gemm_fp8_kernel<E, wide, 128, 128, 2, 2>), dim3((unsigned)(((p.M + 127) / 128) * ((p.N + 127) / 128)), (unsigned)plan.splits), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((gemm_fp8_kernel<E, A, wide, 128, 128, 2, 2>), grid, dim3(256), 0, s, p);
   }
   if (plan.splits > 1)
     hipLaunchKernelGGL((join_splits_kernel<E>), dim3((unsigned)((p.M * ((p.N + 3) / 4) + 255) / 256)), dim3(256), 0, s, p, plan.splits);
   return check_launch("gemm_fp8");
+}
+template <class E> int launch_gemm_of(int a_type, const GemmP& p, float* workspace, hipStream_t s) {
+  return a_type == OBJNERF_TYPE_FP8 ? launch_gemm_fp8<E, void>(p, workspace, s) : a_type == OBJNERF_TYPE_F32 ? launch_gemm_fp8<E, ElemF32>(p, workspace, s)
+         : a_type == OBJNERF_TYPE_BF16 ? launch_gemm_fp8<E, ElemBf16>(p, workspace, s) : launch_gemm_fp8<E, ElemF16>(p, workspace, s);
 }
 
 constexpr int64_t kMaxSize = 1ll << 31, kMaxK = 1ll << 26;     // 32 rows of kMaxK bytes: 32-bit offsets in a wave's copies
@@ -575,9 +653,9 @@ int objnerf_fp8_quantize(const objnerf_fp8_quantize_args* a, void* stream) {
                                         : launch_quantize<ElemF16>(p, square, a->column_sums, s);
 }
 
-int64_t objnerf_gemm_fp8_workspace_floats(int64_t M, int64_t N, int64_t K, int c_type) {
+int64_t objnerf_gemm_fp8_workspace_floats(int64_t M, int64_t N, int64_t K, int a_type, int c_type) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  const Plan plan = plan_of(M, N, K, c_type == OBJNERF_TYPE_F32);
+  const Plan plan = plan_of(M, N, K, c_type == OBJNERF_TYPE_F32, a_type != OBJNERF_TYPE_FP8);
   return plan.splits > 1 ? plan.splits * M * N : 0;
 }
 
@@ -585,28 +663,31 @@ int objnerf_gemm_fp8(const objnerf_gemm_fp8_args* a, void* stream) {
   if (!a) return set_error(-1, "gemm_fp8: no arguments");
   if (a->M < 0 || a->N < 0 || a->K < 0 || a->M >= kMaxSize || a->N >= kMaxSize || a->K > kMaxK || a->K % kBlock)
     return set_error(-1, "gemm_fp8: bad sizes (M, N < 2^31, K <= 2^26, K a multiple of 128)");
-  if (!label_type_ok(a->c_type)) return set_error(-1, "gemm_fp8: unknown element type");
-  if ((a->K && (a->a_stride < a->K || a->b_stride < a->K || a->a_stride % 16 || a->b_stride % 16 || a->a_stride > kMaxK || a->b_stride > kMaxK)) || a->c_stride < a->N)
-    return set_error(-1, "gemm_fp8: bad strides (operands: multiples of 16, at least K, at most 2^26)");
+  const bool raw = a->a_type != OBJNERF_TYPE_FP8;
+  if (!label_type_ok(a->c_type) || (raw && !label_type_ok(a->a_type))) return set_error(-1, "gemm_fp8: unknown element type");
+  if (raw && (a->a_cols <= a->K - kBlock || a->a_cols > a->K)) return set_error(-1, "gemm_fp8: K is a_cols filled up to whole blocks");
+  if (a->K && ((raw ? a->a_stride < 0 : a->a_stride < a->K || a->a_stride % 16 || a->a_stride > kMaxK) || a->b_stride < a->K || a->b_stride % 16 || a->b_stride > kMaxK))
+    return set_error(-1, "gemm_fp8: bad strides (8-bit operands: multiples of 16, at least K, at most 2^26)");
+  if (a->c_stride < a->N) return set_error(-1, "gemm_fp8: bad strides (c: at least N)");
   const int64_t nb = a->K / kBlock;
-  if (a->K && (a->a_scale_stride < nb || a->b_scale_stride < nb || a->a_scale_stride % 4 || a->b_scale_stride % 4))
+  if (a->K && ((!raw && (a->a_scale_stride < nb || a->a_scale_stride % 4)) || a->b_scale_stride < nb || a->b_scale_stride % 4))
     return set_error(-1, "gemm_fp8: bad scale strides (multiples of 4, at least K / 128)");
-  if (((uintptr_t)a->a | (uintptr_t)a->b) & 15 || ((uintptr_t)a->a_scale | (uintptr_t)a->b_scale) & 3)
-    return set_error(-1, "gemm_fp8: operands must be 16-byte, scales 4-byte aligned");
+  if (((raw ? 0 : (uintptr_t)a->a) | (uintptr_t)a->b) & 15 || ((raw ? 0 : (uintptr_t)a->a_scale) | (uintptr_t)a->b_scale) & 3)
+    return set_error(-1, "gemm_fp8: 8-bit operands must be 16-byte, scales 4-byte aligned");
   if (a->M == 0 || a->N == 0) return 0;
-  if (((a->M + 127) / 128) > (1 << 30) / ((a->N + 127) / 128)) return set_error(-1, "gemm_fp8: more than 2^30 tiles");
-  if (objnerf_gemm_fp8_workspace_floats(a->M, a->N, a->K, a->c_type) && !a->workspace) return set_error(-1, "gemm_fp8: a workspace is needed");
-  if (!a->c || (a->K && (!a->a || !a->b || !a->a_scale || !a->b_scale))) return set_error(-1, "gemm_fp8: a needed buffer is missing");
+  if (((a->M + 31) / 32) > (1 << 30) / ((a->N + 127) / 128)) return set_error(-1, "gemm_fp8: more than 2^30 tiles");
+  if (!a->c || (a->K && (!a->a || !a->b || (!raw && !a->a_scale) || !a->b_scale))) return set_error(-1, "gemm_fp8: a needed buffer is missing");
+  if (objnerf_gemm_fp8_workspace_floats(a->M, a->N, a->K, a->a_type, a->c_type) && !a->workspace) return set_error(-1, "gemm_fp8: a workspace is needed");
   GemmP p;
   p.M = a->M; p.N = a->N; p.K = a->K;
-  p.a = a->a; p.lda = a->a_stride; p.sa = a->a_scale; p.ldsa = a->a_scale_stride;
+  p.a = static_cast<const uint8_t*>(a->a); p.lda = a->a_stride; p.sa = a->a_scale; p.ldsa = a->a_scale_stride; p.cols = a->a_cols;
   p.b = a->b; p.ldb = a->b_stride; p.sb = a->b_scale; p.ldsb = a->b_scale_stride;
   p.bias = a->bias; p.leaky = a->leaky;
   p.c = a->c; p.ldc = a->c_stride;
   p.partial = nullptr; p.blocks_per_split = 0;
   hipStream_t s = (hipStream_t)stream;
-  return a->c_type == OBJNERF_TYPE_F32 ? launch_gemm_fp8<ElemF32>(p, a->workspace, s)
-         : a->c_type == OBJNERF_TYPE_BF16 ? launch_gemm_fp8<ElemBf16>(p, a->workspace, s) : launch_gemm_fp8<ElemF16>(p, a->workspace, s);
+  return a->c_type == OBJNERF_TYPE_F32 ? launch_gemm_of<ElemF32>(a->a_type, p, a->workspace, s)
+         : a->c_type == OBJNERF_TYPE_BF16 ? launch_gemm_of<ElemBf16>(a->a_type, p, a->workspace, s) : launch_gemm_of<ElemF16>(a->a_type, p, a->workspace, s);
 }
 
 }  // extern "C"

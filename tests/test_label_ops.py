@@ -99,7 +99,7 @@ def test_quantize_refuses_at_the_c_abi(bad):
 
 def _gemm_args(**kw):
     a = _lib.GemmFp8Args()
-    base = dict(M=4, N=8, K=256, a=64, a_stride=256, a_scale=64, a_scale_stride=4, b=64, b_stride=256, b_scale=64, b_scale_stride=4, bias=None, leaky=0, c_type=1,
+    base = dict(M=4, N=8, K=256, a_type=3, a_cols=0, a=64, a_stride=256, a_scale=64, a_scale_stride=4, b=64, b_stride=256, b_scale=64, b_scale_stride=4, bias=None, leaky=0, c_type=1,
                 c=64, c_stride=8)
     for k, v in {**base, **kw}.items():
         setattr(a, k, v)
@@ -108,7 +108,8 @@ def _gemm_args(**kw):
 
 @pytest.mark.parametrize("bad", [dict(M=-1), dict(N=-1), dict(K=-128), dict(K=200), dict(M=1 << 31), dict(M=(1 << 31) - 1, N=(1 << 31) - 1, c_stride=1 << 31), dict(c_type=4),
                                  dict(a_stride=128), dict(b_stride=250), dict(b_stride=260), dict(c_stride=7), dict(a_scale_stride=2), dict(b_scale_stride=5), dict(K=640, a_stride=640, b_stride=640),
-                                 dict(a=72), dict(b_scale=65), dict(a=None), dict(b=None), dict(a_scale=None), dict(b_scale=None), dict(c=None)])
+                                 dict(a=72), dict(b_scale=65), dict(a=None), dict(b=None), dict(a_scale=None), dict(b_scale=None), dict(c=None), dict(a_type=4), dict(a_type=-1), dict(a_type=1, a_cols=128),
+                                 dict(a_type=1, a_cols=257), dict(a_type=1, a_cols=256, a_stride=-1)])
 def test_gemm_refuses_at_the_c_abi(bad):
     l = _lib.lib()
     assert l.objnerf_gemm_fp8(C.byref(_gemm_args(**bad)), None) < 0
