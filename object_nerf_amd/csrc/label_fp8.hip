@@ -46,17 +46,31 @@ __device__ __forceinline__ unsigned fp8x4(float a, float b, float c, float d) {
   return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
 }
 
-// eight consecutive columns of a row; what lies behind its end is 0
-template <class E>
-__device__ __forceinline__ void load8(const char* row, long c, long cols, float* x) {
-  if (c + 8 <= cols) {
+// eight consecutive columns of a row as they lie in memory; what lies behind its end is 0
+template <class E> struct Eight {
+  static constexpr int kPieces = 8 / E::kVec;
+  u32x4 r[kPieces];
+  __device__ __forceinline__ void load(const char* row, long c, long cols) {
+    if (c + 8 <= cols) {
 #pragma unroll
-    for (int h = 0; h < 8 / E::kVec; ++h) E::unpack(load16(row, (c + h * E::kVec) * E::kBytes), x + h * E::kVec);
-  } else {
+      for (int h = 0; h < kPieces; ++h) r[h] = load16(row, (c + h * E::kVec) * E::kBytes);
+    } else {
+      float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = c + i < cols ? E::load(row, c + i) : 0.f;
+      for (int i = 0; i < 8; ++i) x[i] = c + i < cols ? E::load(row, c + i) : 0.f;
+#pragma unroll
+      for (int h = 0; h < kPieces; ++h) r[h] = E::pack(x + h * E::kVec);
+    }
   }
-}
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int h = 0; h < kPieces; ++h) r[h] = u32x4{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ void values(float* x) const {
+#pragma unroll
+    for (int h = 0; h < kPieces; ++h) E::unpack(r[h], x + h * E::kVec);
+  }
+};
 
 struct QuantP {
   long rows, cols;
@@ -77,8 +91,10 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantP p) {
   const bool in = block < p.rows * kb;
   const long row = in ? block / kb : 0, b = in ? block - row * kb : 0;
   const char* xr = static_cast<const char*>(p.x) + row * p.ldx * E::kBytes;
+  Eight<E> held;
+  held.load(xr, b * kBlock + l * 8, p.cols);
   float x[8];
-  load8<E>(xr, b * kBlock + l * 8, p.cols, x);
+  held.values(x);
   float a = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) a = fmaxf(a, finite_abs(x[i]));
@@ -95,39 +111,49 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantP p) {
 }
 
 // A 128 x 128 tile: blocks of 128 x 128, the transposed form, both forms at once, and the column sums.  Thread (g, l): rows 8 g .. 8 g + 7,
-// columns 8 l .. 8 l + 7, so that a column's eight bytes of a thread are one 8-byte LDS write of the transposed tile.
+// columns 8 l .. 8 l + 7, held as they were read.  A row of the transposed tile is 144 bytes of LDS.
 constexpr int kPitch = 144;
 template <class E, bool ROWS, bool TRANS, bool SQUARE>
-__global__ void __launch_bounds__(256) quantize_tile_kernel(QuantP p) {
-  __shared__ float col_max[16][kBlock];
+__global__ void __launch_bounds__(256, 4) quantize_tile_kernel(QuantP p) {
+  __shared__ float per_thread[16][kBlock];
   __shared__ unsigned col_byte[kBlock];
   __shared__ __align__(16) uint8_t tile[TRANS ? kBlock * kPitch : 16];
   const long kb = blocks_of(p.cols), sb = scale_stride(p.cols), mb = blocks_of(p.rows), sbt = scale_stride(p.rows);
   const long bc = blockIdx.x % kb, br = blockIdx.x / kb;
   const int g = threadIdx.x >> 4, l = threadIdx.x & 15;
   const long r0 = br * kBlock + g * 8, c0 = bc * kBlock + l * 8;
-  float x[8][8];
+  Eight<E> held[8];
 #pragma unroll
   for (int s = 0; s < 8; ++s) {
-    if (r0 + s < p.rows) load8<E>(static_cast<const char*>(p.x) + (r0 + s) * p.ldx * E::kBytes, c0, p.cols, x[s]);
-    else
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[s][i] = 0.f;
+    if (r0 + s < p.rows) held[s].load(static_cast<const char*>(p.x) + (r0 + s) * p.ldx * E::kBytes, c0, p.cols);
+    else held[s].clear();
   }
-  unsigned square_byte = 0;
-  if (TRANS || SQUARE) {
+  // one pass over the rows: largest of each row (16 lanes), of each column (16 threads), column sums (8 rows in order, then 16 threads)
+  float column[8], sum[8];
+  unsigned row_byte[8], square_byte = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) { column[i] = 0.f; sum[i] = 0.f; }
+#pragma unroll
+  for (int s = 0; s < 8; ++s) {
+    float x[8], a = 0.f;
+    held[s].values(x);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float a = 0.f;
-#pragma unroll
-      for (int s = 0; s < 8; ++s) a = fmaxf(a, finite_abs(x[s][i]));
-      col_max[g][l * 8 + i] = a;
+      const float v = finite_abs(x[i]);
+      a = fmaxf(a, v);
+      column[i] = fmaxf(column[i], v);
+      sum[i] = s == 0 ? x[i] : sum[i] + x[i];
     }
+    if (ROWS && !SQUARE) row_byte[s] = scale_byte(lanes_reduce<16, OpMax>(a));
+  }
+  if (TRANS || SQUARE) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) per_thread[g][l * 8 + i] = column[i];
     __syncthreads();
     if (threadIdx.x < kBlock) {
       float a = 0.f;
 #pragma unroll
-      for (int s = 0; s < 16; ++s) a = fmaxf(a, col_max[s][threadIdx.x]);
+      for (int s = 0; s < 16; ++s) a = fmaxf(a, per_thread[s][threadIdx.x]);
       col_byte[threadIdx.x] = SQUARE ? __float_as_uint(a) : scale_byte(a);
     }
     __syncthreads();
@@ -136,22 +162,31 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(QuantP p) {
       square_byte = scale_byte(__uint_as_float(lanes_reduce<64, OpMax>(a)));
     }
   }
+  if (p.part) {
+    if (TRANS || SQUARE) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) per_thread[g][l * 8 + i] = sum[i];
+    __syncthreads();
+    const long col = bc * kBlock + threadIdx.x;
+    if (threadIdx.x < kBlock && col < p.cols) {
+      float a = per_thread[0][threadIdx.x];
+#pragma unroll
+      for (int s = 1; s < 16; ++s) a += per_thread[s][threadIdx.x];
+      p.part[br * p.cols + col] = a;
+    }
+  }
   if (ROWS) {
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
-      unsigned byte = square_byte;
-      if (!SQUARE) {
-        float a = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a = fmaxf(a, finite_abs(x[s][i]));
-        byte = scale_byte(lanes_reduce<16, OpMax>(a));
-      }
+      const unsigned byte = SQUARE ? square_byte : row_byte[s];
       const float inv = inverse_scale(byte);
       const long row = r0 + s;
       if (row < p.rows) {
+        float x[8];
+        held[s].values(x);
         uint2 o;
-        o.x = fp8x4(x[s][0] * inv, x[s][1] * inv, x[s][2] * inv, x[s][3] * inv);
-        o.y = fp8x4(x[s][4] * inv, x[s][5] * inv, x[s][6] * inv, x[s][7] * inv);
+        o.x = fp8x4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+        o.y = fp8x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
         *reinterpret_cast<uint2*>(p.q + row * kb * kBlock + c0) = o;
         if (l == 0) p.scale[row * sb + bc] = (uint8_t)byte;
         if (bc == kb - 1 && l > 0 && bc + l < sb) p.scale[row * sb + bc + l] = 127;
@@ -159,13 +194,17 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(QuantP p) {
     }
   }
   if (TRANS) {
+    // four rows at a time: four bytes of each of the eight columns
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float inv = inverse_scale(SQUARE ? square_byte : col_byte[l * 8 + i]);
-      uint2 o;
-      o.x = fp8x4(x[0][i] * inv, x[1][i] * inv, x[2][i] * inv, x[3][i] * inv);
-      o.y = fp8x4(x[4][i] * inv, x[5][i] * inv, x[6][i] * inv, x[7][i] * inv);
-      *reinterpret_cast<uint2*>(&tile[(l * 8 + i) * kPitch + g * 8]) = o;
+    for (int q = 0; q < 2; ++q) {
+      float x[4][8];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) held[q * 4 + s].values(x[s]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float inv = inverse_scale(SQUARE ? square_byte : col_byte[l * 8 + i]);
+        *reinterpret_cast<unsigned*>(&tile[(l * 8 + i) * kPitch + g * 8 + q * 4]) = fp8x4(x[0][i] * inv, x[1][i] * inv, x[2][i] * inv, x[3][i] * inv);
+      }
     }
     __syncthreads();
 #pragma unroll
@@ -179,24 +218,6 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(QuantP p) {
       p.scale_t[col * sbt + br] = (uint8_t)(SQUARE ? square_byte : col_byte[threadIdx.x]);
       if (br == mb - 1)
         for (long e = mb; e < sbt; ++e) p.scale_t[col * sbt + e] = 127;
-    }
-  }
-  if (p.part) {                                                  // sums of 8 rows in order, then of 16 threads in order
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float a = x[0][i];
-#pragma unroll
-      for (int s = 1; s < 8; ++s) a += x[s][i];
-      col_max[g][l * 8 + i] = a;
-    }
-    __syncthreads();
-    const long col = bc * kBlock + threadIdx.x;
-    if (threadIdx.x < kBlock && col < p.cols) {
-      float a = col_max[0][threadIdx.x];
-#pragma unroll
-      for (int s = 1; s < 16; ++s) a += col_max[s][threadIdx.x];
-      p.part[br * p.cols + col] = a;
     }
   }
 }
@@ -297,12 +318,13 @@ template <class E> __device__ __forceinline__ void store4(const GemmP& p, long m
   }
 }
 
-// Which BM x BN of C a workgroup has.  Workgroups go round the 8 XCDs: each XCD takes one run of tiles, in panels of 8 tile rows, so that
-// its L2 serves neighbours.
-template <int BM, int BN> __device__ __forceinline__ void tile_of(const GemmP& p, long& m0, long& n0) {
+// Which BM x BN of C is number `at` of a launch's tiles.  Workgroups go round the 8 XCDs (and a workgroup's tiles are a multiple of 8
+// apart): each XCD takes one run of tiles, in panels of 8 tile rows, so that its L2 serves neighbours.
+template <int BM, int BN> __device__ __forceinline__ long tiles_of(const GemmP& p) { return (p.M + BM - 1) / BM * ((p.N + BN - 1) / BN); }
+template <int BM, int BN> __device__ __forceinline__ void tile_of(const GemmP& p, long at, long& m0, long& n0) {
   const long mt = (p.M + BM - 1) / BM, nt = (p.N + BN - 1) / BN, tiles = mt * nt;
-  const long xcd = blockIdx.x % 8, per = tiles / 8, more = tiles % 8;
-  const long tile = xcd * per + min(xcd, more) + blockIdx.x / 8;
+  const long xcd = at % 8, per = tiles / 8, more = tiles % 8;
+  const long tile = xcd * per + min(xcd, more) + at / 8;
   const long panel = tile / (8 * nt), rows = min(mt - panel * 8, 8l), in = tile - panel * 8 * nt;
   m0 = (panel * 8 + in % rows) * BM;
   n0 = in / rows * BN;
@@ -310,7 +332,7 @@ template <int BM, int BN> __device__ __forceinline__ void tile_of(const GemmP& p
 
 // The copies of a workgroup's rows from memory straight into LDS.  A step is one block of 128: BM + BN rows of 128 bytes into one of two
 // slots.  The 16-byte pieces of a row are permuted (piece_key) on the addresses the lanes read from, since LDS is filled in order.  Scales:
-// a dword of each row, four steps' worth, into two slots of their own; a wave copies those of 64 rows.
+// a dword of each row, four steps' worth, into two slots of their own; a wave copies those of 64 rows.  Which slot is the caller's count.
 template <int BM, int BN, int WAVES, bool RAW> struct Copies {
   static constexpr int kScaleRows = (BM + BN + 63) / 64 * 64, kScaleCopies = (kScaleRows / 64 + WAVES - 1) / WAVES;
   static constexpr int kSlot = (BM + BN) * kBlock, kBytes = 2 * kSlot + 2 * kScaleRows * 4;
@@ -318,9 +340,8 @@ template <int BM, int BN, int WAVES, bool RAW> struct Copies {
   static_assert((RAW || BM % (8 * WAVES) == 0) && BN % (8 * WAVES) == 0, "whole groups of 8 rows per wave");
   const uint8_t *abase, *bbase, *sbase[kScaleCopies];
   unsigned aoff[RA + 1], boff[RB];
-  long first;
   lds_byte* lds;
-  __device__ __forceinline__ Copies(const GemmP& p, long m0, long n0, long first_block, lds_byte* ring) : first(first_block), lds(ring) {
+  __device__ __forceinline__ void aim(const GemmP& p, long m0, long n0, long first) {
     const int lane = threadIdx.x & 63, wave = uni((int)(threadIdx.x >> 6));
     // this lane's part: row lane / 8 of every 8, piece lane % 8 of LDS
     const long arow = min(m0 + wave * RA * 8, p.M - 1), brow = min(n0 + wave * RB * 8, p.N - 1);
@@ -342,69 +363,51 @@ template <int BM, int BN, int WAVES, bool RAW> struct Copies {
       sbase[c] = r < BM && !RAW ? p.sa + min(m0 + r, p.M - 1) * p.ldsa : p.sb + max(min(n0 + r - BM, p.N - 1), 0l) * p.ldsb;
     }
   }
-  __device__ __forceinline__ void rows(long step) const {
+  __device__ __forceinline__ void rows(long step, int to) const {
     const int wave = uni((int)(threadIdx.x >> 6));
-    lds_byte* slot = lds + (int)(step & 1) * kSlot + wave * RA * 1024;
+    lds_byte* slot = lds + to * kSlot + wave * RA * 1024;
     const uint8_t* from = abase + step * kBlock;
 #pragma unroll
     for (int c = 0; c < RA; ++c)
       __builtin_amdgcn_global_load_lds((global_byte*)(from + aoff[c]), (__attribute__((address_space(3))) void*)(slot + c * 1024), 16, 0, 0);
-    slot = lds + (int)(step & 1) * kSlot + BM * kBlock + wave * RB * 1024;
+    slot = lds + to * kSlot + BM * kBlock + wave * RB * 1024;
     from = bbase + step * kBlock;
 #pragma unroll
     for (int c = 0; c < RB; ++c)
       __builtin_amdgcn_global_load_lds((global_byte*)(from + boff[c]), (__attribute__((address_space(3))) void*)(slot + c * 1024), 16, 0, 0);
   }
   // (a's rows where it is rounded here: their dwords are another wave's stores, the copy starts behind them)
-  __device__ __forceinline__ void scales(long step) const {
+  __device__ __forceinline__ void scales(long group, int to) const {
     const int wave = uni((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
-    const long group = (first + step) >> 2;
 #pragma unroll
     for (int c = 0; c < kScaleCopies; ++c) {
       const int from = (c * WAVES + wave) * 64;
       if (from >= kScaleRows || (RAW && from + 64 <= BM)) continue;
       if (RAW && from < BM && from + lane < BM) continue;        // lanes of a's rows copy nothing: their places stay as they are
-      __builtin_amdgcn_global_load_lds((global_byte*)(sbase[c] + group * 4), (__attribute__((address_space(3))) void*)(lds + 2 * kSlot + ((int)(group & 1) * kScaleRows + from) * 4), 4, 0, 0);
+      __builtin_amdgcn_global_load_lds((global_byte*)(sbase[c] + group * 4), (__attribute__((address_space(3))) void*)(lds + 2 * kSlot + (to * kScaleRows + from) * 4), 4, 0, 0);
     }
   }
-  // scale byte of row 0 of the tile in this step; rows are 4 bytes apart, b's rows behind a's
-  __device__ __forceinline__ const lds_byte* scale_at(long step) const {
-    const long at = first + step;
-    return lds + 2 * kSlot + (int)(at >> 2 & 1) * kScaleRows * 4 + (int)(at & 3);
-  }
+  // scale byte of row 0 of the tile for a block; rows are 4 bytes apart, b's rows behind a's
+  __device__ __forceinline__ lds_byte* scale_at(long block, int slot) const { return lds + 2 * kSlot + slot * kScaleRows * 4 + (int)(block & 3); }
 };
 // a's rows of a step where they are rounded on their way into LDS: 16 lanes per row and block, held in registers from the load to the
 // store, so that the step in between hides the load.
 template <class A, int BM, int THREADS, class COPY> struct RawRows {
-  static constexpr int kPasses = BM * 16 / THREADS, kPieces = 8 / A::kVec;
-  u32x4 held[kPasses][kPieces];
+  static constexpr int kPasses = BM * 16 / THREADS;
+  Eight<A> held[kPasses];
   __device__ __forceinline__ void load(const GemmP& p, long m0, long block) {
     const int l = threadIdx.x & 15, g = threadIdx.x >> 4;
-    const long c = block * kBlock + l * 8;
 #pragma unroll
-    for (int s = 0; s < kPasses; ++s) {
-      const char* row = reinterpret_cast<const char*>(p.a) + min(m0 + s * (THREADS / 16) + g, p.M - 1) * p.lda * A::kBytes;
-      if (c + 8 <= p.cols) {
-#pragma unroll
-        for (int h = 0; h < kPieces; ++h) held[s][h] = load16(row, (c + h * A::kVec) * A::kBytes);
-      } else {
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = c + i < p.cols ? A::load(row, c + i) : 0.f;
-#pragma unroll
-        for (int h = 0; h < kPieces; ++h) held[s][h] = A::pack(x + h * A::kVec);
-      }
-    }
+    for (int s = 0; s < kPasses; ++s)
+      held[s].load(reinterpret_cast<const char*>(p.a) + min(m0 + s * (THREADS / 16) + g, p.M - 1) * p.lda * A::kBytes, block * kBlock + l * 8, p.cols);
   }
-  __device__ __forceinline__ void store(const COPY& copy, long step) const {
+  __device__ __forceinline__ void store(const COPY& copy, int slot, lds_byte* scale) const {
     const int l = threadIdx.x & 15, g = threadIdx.x >> 4;
-    lds_byte* const rows = copy.lds + (int)(step & 1) * COPY::kSlot;
-    lds_byte* const scale = const_cast<lds_byte*>(copy.scale_at(step));
+    lds_byte* const rows = copy.lds + slot * COPY::kSlot;
 #pragma unroll
     for (int s = 0; s < kPasses; ++s) {
       float x[8];
-#pragma unroll
-      for (int h = 0; h < kPieces; ++h) A::unpack(held[s][h], x + h * A::kVec);
+      held[s].values(x);
       float largest = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) largest = fmaxf(largest, finite_abs(x[i]));
@@ -491,73 +494,94 @@ __device__ __forceinline__ void write_tile(const GemmP& p, long m0, long n0, lds
 // block take 8 bytes of every lane's 32 each: another order of the same sum.
 template <class E, class A, bool WIDE, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(WM * WN * 64, 2) gemm_fp8_kernel(GemmP p) {
-  constexpr bool kRaw = !std::is_same<A, void>::value;
+  constexpr bool kRaw = !std::is_same<A, void>::value, kRun = BM < 256;      // (256 x 256: no registers to spare for a next tile)
   using Copy = Copies<BM, BN, WM * WN, kRaw>;
   using Raw = typename std::conditional<kRaw, RawRows<typename std::conditional<kRaw, A, ElemF32>::type, BM, WM * WN * 64, Copy>, NoRaw>::type;
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
   __shared__ __align__(16) uint8_t ring[Copy::kBytes];           // one object: the copies' waits stay with the barrier
-  long m0, n0;
-  tile_of<BM, BN>(p, m0, n0);
+  static_assert(WM * WN * 16 * (TN * 16 + 4) * 4 <= Copy::kSlot, "the waves' areas of write_tile fit into a slot");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, h = lane >> 4;
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
   const long first = blockIdx.y * p.blocks_per_split, steps = min(p.blocks_per_split, p.K / kBlock - first);
-  const Copy copy(p, m0, n0, first, (lds_byte*)ring);
-
-  f32x4 acc[TM][TN] = {};
+  long at = blockIdx.x, m0, n0;
+  tile_of<BM, BN>(p, at, m0, n0);
+  Copy copy;
+  copy.lds = (lds_byte*)ring;
+  copy.aim(p, m0, n0, first);
   Raw raw;
+  int slot = 0, scale_slot = 0;
   if (steps > 0) {
     raw.load(p, m0, first);
-    copy.rows(0);
-    copy.scales(0);
-    raw.store(copy, 0l);
+    copy.rows(0, 0);
+    copy.scales(first >> 2, 0);
+    raw.store(copy, 0, copy.scale_at(first, 0));
   }
-  for (long step = 0; step < steps; ++step) {
-    __syncthreads();                                             // the step's rows have landed; the other slot has been read
-    if (step + 1 < steps) {
-      raw.load(p, m0, first + step + 1);
-      copy.rows(step + 1);
-      if (((first + step) & 3) == 3) copy.scales(step + 1);
-    }
-    const lds_byte* const rows_a = copy.lds + (step & 1) * Copy::kSlot + wm * kBlock;
-    const lds_byte* const rows_b = copy.lds + (step & 1) * Copy::kSlot + (BM + wn) * kBlock;
-    const lds_byte* const scale_a = copy.scale_at(step) + (wm + i) * 4;
-    const lds_byte* const scale_b = copy.scale_at(step) + (BM + wn + i) * 4;
-    i32x8 fa[TM];
-    int sa[TM];
-#pragma unroll
-    for (int t = 0; t < TM; ++t) sa[t] = scale_a[t * 64];
-#pragma unroll
-    for (int t = 0; t < TM; ++t) fa[t] = fragment(rows_a + t * 16 * kBlock, i, h);
-    if constexpr (WIDE) {
-      i32x8 fb[TN];
-#pragma unroll
-      for (int t = 0; t < TN; ++t) fb[t] = fragment(rows_b + t * 16 * kBlock, i, h);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        bf16x8 xa[TM];
-#pragma unroll
-        for (int t = 0; t < TM; ++t) xa[t] = widened(fa[t][2 * q], fa[t][2 * q + 1], scale_of(sa[t]));
-#pragma unroll
-        for (int t = 0; t < TN; ++t) {
-          const bf16x8 xb = widened(fb[t][2 * q], fb[t][2 * q + 1], scale_of(scale_b[t * 64]));
-#pragma unroll
-          for (int u = 0; u < TM; ++u) acc[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb, xa[u], acc[u][t], 0, 0, 0);
+  // a workgroup's tiles one after the other: the next one's first rows are on their way while this one's results are written
+  for (bool more = true; more;) {
+    f32x4 acc[TM][TN] = {};
+    const long m = m0, n = n0;
+    at += gridDim.x;
+    more = kRun && at < tiles_of<BM, BN>(p);
+    for (long step = 0; step < steps; ++step) {
+      __syncthreads();                                             // the step's rows have landed; the other slot has been read
+      const lds_byte* const rows_a = copy.lds + slot * Copy::kSlot + wm * kBlock;
+      const lds_byte* const rows_b = copy.lds + slot * Copy::kSlot + (BM + wn) * kBlock;
+      const lds_byte* const scale_a = copy.scale_at(first + step, scale_slot) + (wm + i) * 4;
+      const lds_byte* const scale_b = copy.scale_at(first + step, scale_slot) + (BM + wn + i) * 4;
+      const bool last = step + 1 == steps;
+      const long block = last ? first : first + step + 1;          // the next one, of this tile or of the next
+      slot ^= 1;
+      if (!last || more) {
+        if (last) {
+          tile_of<BM, BN>(p, at, m0, n0);
+          copy.aim(p, m0, n0, first);
+        }
+        raw.load(p, m0, block);
+        copy.rows(block - first, slot);
+        if (last || (block & 3) == 0) {
+          scale_slot ^= 1;
+          copy.scales(block >> 2, scale_slot);
         }
       }
-    } else {
+      i32x8 fa[TM];
+      int sa[TM];
 #pragma unroll
-      for (int t = 0; t < TN; ++t) {
-        const i32x8 fb = fragment(rows_b + t * 16 * kBlock, i, h);
-        const int sb = scale_b[t * 64];
+      for (int t = 0; t < TM; ++t) sa[t] = scale_a[t * 64];
 #pragma unroll
-        for (int u = 0; u < TM; ++u) acc[u][t] = mfma8(fb, fa[u], acc[u][t], sb, sa[u]);
+      for (int t = 0; t < TM; ++t) fa[t] = fragment(rows_a + t * 16 * kBlock, i, h);
+      if constexpr (WIDE) {
+        i32x8 fb[TN];
+#pragma unroll
+        for (int t = 0; t < TN; ++t) fb[t] = fragment(rows_b + t * 16 * kBlock, i, h);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          bf16x8 xa[TM];
+#pragma unroll
+          for (int t = 0; t < TM; ++t) xa[t] = widened(fa[t][2 * q], fa[t][2 * q + 1], scale_of(sa[t]));
+#pragma unroll
+          for (int t = 0; t < TN; ++t) {
+            const bf16x8 xb = widened(fb[t][2 * q], fb[t][2 * q + 1], scale_of(scale_b[t * 64]));
+#pragma unroll
+            for (int u = 0; u < TM; ++u) acc[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb, xa[u], acc[u][t], 0, 0, 0);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < TN; ++t) {
+          const i32x8 fb = fragment(rows_b + t * 16 * kBlock, i, h);
+          const int sb = scale_b[t * 64];
+#pragma unroll
+          for (int u = 0; u < TM; ++u) acc[u][t] = mfma8(fb, fa[u], acc[u][t], sb, sa[u]);
+        }
       }
+      if (!last || more) raw.store(copy, slot, copy.scale_at(block, scale_slot));
     }
-    if (step + 1 < steps) raw.store(copy, step + 1);
+    // the slot that has just been read serves the results; the other one's copies are under way: a barrier that waits for none
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    write_tile<E, TM, TN>(p, m + wm, n + wn, copy.lds + (slot ^ 1) * Copy::kSlot + wave * 16 * (TN * 16 + 4) * 4, acc);
   }
-  static_assert(WM * WN * 16 * (TN * 16 + 4) * 4 <= Copy::kBytes, "the waves' areas fit where the rows lay");
-  __syncthreads();
-  write_tile<E, TM, TN>(p, m0 + wm, n0 + wn, copy.lds + wave * 16 * (TN * 16 + 4) * 4, acc);
 }
 
 // C from the partial sums of the splits, in their order
@@ -600,7 +624,10 @@ int launch_gemm_fp8(GemmP p, float* workspace, hipStream_t s) {
   const Plan plan = plan_of(p.M, p.N, p.K, wide, raw);
   p.blocks_per_split = plan.blocks;
   p.partial = plan.splits > 1 ? workspace : nullptr;
-  const dim3 grid((unsigned)(((p.M + plan.bm - 1) / plan.bm) * ((p.N + plan.bn - 1) / plan.bn)), (unsigned)plan.splits);
+  // as many workgroups as the card holds at once, each with every so manieth tile (a multiple of 8 apart)
+  const long tiles = ((p.M + plan.bm - 1) / plan.bm) * ((p.N + plan.bn - 1) / plan.bn);
+  const long places = plan.bm == 256 || p.K == 0 ? tiles : plan.bm == 128 ? 512 : 768;
+  const dim3 grid((unsigned)(tiles < places ? tiles : places), (unsigned)plan.splits);
   if (plan.bm == 256) {
     if constexpr (!wide && !raw) hipLaunchKernelGGL((gemm_fp8_kernel<E, A, false, 256, 256, 2, 4>), grid, dim3(512), 0, s, p);
   } else if (plan.bm == 32) {
