@@ -98,7 +98,7 @@ __device__ __forceinline__ void mask_tiles(const f32x16 (&acc)[NT], const MaskBi
 #pragma unroll
       for (int r = 15; r >= 0; r -= 2) {
         const f32x2 v = {acc[t][r - 1], acc[t][r]};
-        const f32x2 sl = v * 0.01f;                  // v_pk_mul_f32
+        const f32x2 sl = v * 0.01f;
         float o1, o0;
         asm volatile("v_add_co_u32 %0, vcc, %0, %0\n\tv_cndmask_b32 %1, %2, %3, vcc"
                      : "+v"(m), "=v"(o1) : "v"(sl[1]), "v"(v[1]) : "vcc");

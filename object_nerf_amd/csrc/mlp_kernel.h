@@ -263,8 +263,8 @@ __device__ __forceinline__ void finish(const f32x16 (&acc)[NT], f32x16 (&h)[NT])
 #pragma unroll
     for (int r = 0; r < 16; r += 2) {
       if constexpr (ACT && OBJ_PK_LEAKY) {
-        // 0.01 v for two values in one v_pk_mul_f32 (gfx950 has packed fp32 mul / fma, no packed max): the same two IEEE
-        // operations per value as leaky() -- bit-equal -- in 1.5 instead of 2 VALU instructions
+        // 0.01 v for two values at a time: the same two IEEE operations per value as leaky(), bit-equal (the build has packed fp32
+        // instructions switched off: Makefile)
         const f32x2 v = {acc[m][r], acc[m][r + 1]};
         const f32x2 sl = v * 0.01f;
         h[m][r] = fmaxf(v[0], sl[0]);
@@ -333,7 +333,7 @@ __device__ __forceinline__ void finish_add(const f32x16 (&acc)[NT], const f32x16
   for (int m = 0; m < NT; ++m)
 #pragma unroll
     for (int r = 0; r < 16; r += 2) {
-      if constexpr (OBJ_PK_LEAKY) {      // packed add (+ packed 0.01 v): the same IEEE operations, half the instructions
+      if constexpr (OBJ_PK_LEAKY) {      // two values at a time: the same IEEE operations
         const f32x2 a2 = {acc[m][r], acc[m][r + 1]}, b2 = {add[m][r], add[m][r + 1]};
         const f32x2 v = a2 + b2;
         if constexpr (ACT) {
