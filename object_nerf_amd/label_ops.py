@@ -14,6 +14,7 @@ a call can be captured in a graph.  Arguments of a wrong type raise TypeError, o
 failing launches RuntimeError.
 """
 import ctypes as C
+import operator
 from typing import NamedTuple
 
 import torch
@@ -70,7 +71,7 @@ class Fp8Matrix(NamedTuple):
     """A matrix (R, cols) in e4m3 with a power-of-two scale for each block of 128 columns of a row.
 
     data (R, C') float8_e4m3fn, C' = cols filled up to a multiple of 128 with zeros; scale (R, B') uint8, B' = C' / 128 filled up to a
-    multiple of 4: element [r, c] stands for data[r, c] * 2 ** (scale[r, c // 128] - 127)."""
+    multiple of 4: element [r, c] stands for data[r, c] * 2 ** (scale[r, c // 128] - 127), scale in [1, 254]."""
     data: torch.Tensor
     scale: torch.Tensor
     cols: int
@@ -315,7 +316,8 @@ def distill_top_logits(student, teacher, index, temperature=1.0):
 
     student (N, V); teacher (N, k) logits or log-probabilities, k <= 1024; index (N, k) int32 or int64, the labels that the
     teacher's values belong to.  A slot whose index lies outside [0, V) or whose value is -inf is empty; a row without a filled slot
-    has loss 0 and gradient 0.  An index may occur more than once (its shares add).  Differentiable with respect to `student`
+    has loss 0 and gradient 0; otherwise NaN in the row gives a loss of NaN, a label ruled out by the student (-inf) under a filled slot a loss
+    of +inf.  An index may occur more than once (its shares add).  Differentiable with respect to `student`
     alone; the usual factor T^2 is the caller's.  The backward pass reads the student's row again instead of keeping a copy."""
     if torch.is_grad_enabled() and isinstance(student, torch.Tensor) and student.requires_grad:
         return _DistillFn.apply(student, teacher, index, temperature)
@@ -360,30 +362,30 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         keep.append(_column(temperature, "temperature", n, dev))
         a.temperature_rows = keep[-1].data_ptr()
     else:
+        a.temperature = temperature = float(temperature)
         if not 0.0 <= temperature < 1e300:
-            raise ValueError("temperature must be >= 0 and finite, got %r" % (temperature,))
-        a.temperature = temperature
+            raise ValueError("temperature must be >= 0 and finite, got %r" % temperature)
     if isinstance(top_k, torch.Tensor):
         keep.append(_column(top_k, "top_k", n, dev, torch.int32))
         a.top_k_rows = keep[-1].data_ptr()
     else:
+        a.top_k = top_k = operator.index(top_k)
         if not 0 <= top_k < 1 << 31:
-            raise ValueError("top_k must be >= 0, got %r" % (top_k,))
-        a.top_k = top_k
+            raise ValueError("top_k must be >= 0, got %r" % top_k)
     if isinstance(top_p, torch.Tensor):
         keep.append(_column(top_p, "top_p", n, dev))
         a.top_p_rows = keep[-1].data_ptr()
     else:
+        a.top_p = top_p = float(top_p)
         if not top_p >= 0.0:
-            raise ValueError("top_p must be >= 0, got %r" % (top_p,))
-        a.top_p = top_p
+            raise ValueError("top_p must be >= 0, got %r" % top_p)
     if isinstance(min_p, torch.Tensor):
         keep.append(_column(min_p, "min_p", n, dev))
         a.min_p_rows = keep[-1].data_ptr()
     else:
+        a.min_p = min_p = float(min_p)
         if not 0.0 <= min_p <= 1.0:
-            raise ValueError("min_p must lie in [0, 1], got %r" % (min_p,))
-        a.min_p = min_p
+            raise ValueError("min_p must lie in [0, 1], got %r" % min_p)
     labels = torch.empty(n, dtype=torch.int64, device=dev)
     a.labels = labels.data_ptr()
     lib = _lib.lib()

@@ -221,6 +221,26 @@ def test_sample_sizes_types_and_filters(n, v, dtype, kw):
     _draw_check((torch.randn(n, v, generator=g) * 2.5).to(dtype), torch.rand(n, generator=g), **kw)
 
 
+@pytest.mark.parametrize("kw", [dict(top_k=1), dict(top_k=5), dict(temperature=0.8, top_k=40, top_p=0.95, min_p=0.01), dict(top_k=128), dict(top_k=300), dict(temperature=0.0),
+                                dict(top_p=0.9), dict(temperature=30.0, top_p=0.6)], ids=str)
+@pytest.mark.parametrize("n,v,dtype", [(600, 700, BF16), (520, 5003, F32), (200, 9001, F16), (300, 8200, F32), (129, 8192, BF16)])
+def test_sample_many_rows(n, v, dtype, kw):
+    """more rows than places: the kernel for small top_k and the one for the rest; workgroups of 256, 512 and 1,024 threads"""
+    g = _gen(v)
+    z = (torch.randn(n, v, generator=g) * 2.5).to(dtype)
+    z[:4] = 0.5                                           # equal logits: the list of candidates overflows
+    z[5] = -math.inf
+    z[6, 10:] = -math.inf                                 # fewer labels than top_k
+    _draw_check(z, torch.rand(n, generator=g), **kw)
+
+
+def test_sample_many_rows_with_settings_of_their_own():
+    n, v = 700, 900
+    g = _gen(4)
+    z, u = torch.randn(n, v, generator=g) * 2, torch.rand(n, generator=g)
+    _draw_check(z, u, temperature=torch.rand(n, generator=g) * 2 - 0.1, top_k=torch.randint(-1, 300, (n,), generator=g), top_p=torch.rand(n, generator=g) * 1.2)
+
+
 @pytest.mark.parametrize("v", [3, 64, 100, 900, 3001, 66000])
 def test_sample_ties(v):
     g = _gen(1)
@@ -476,6 +496,52 @@ def test_fp8_refusals():
         A.linear_fp8(x, q, torch.zeros(8, device=DEV, requires_grad=True))
 
 
+def _check_large(y, x, w8, bias=None):
+    """rows of a large product against 64-bit sums on the GPU, with _check_product's bound"""
+    a, b = R_values(A.quantize_fp8(x)), R_values(w8)
+    want, size = torch.mm(a, b.t().contiguous()), torch.mm(a.abs(), b.abs().t().contiguous())
+    if bias is not None:
+        want, size = want + bias.double(), size + bias.double().abs()
+    part = (a.shape[1] + 2) * 2 * R.STEP[F32] + (0 if y.dtype == F32 else 7 * 2.0 ** -13)
+    bound = R.STEP[y.dtype] * want.abs() + part * size * (1 + R.STEP[y.dtype]) + 2.0 ** -24
+    err = (y.double() - want).abs()
+    assert (err <= bound).all(), (err / bound).max().item()
+
+
+def R_values(q):
+    """what an Fp8Matrix stands for, in 64 bits on its device"""
+    return (q.data.double() * torch.exp2(q.scale.double() - 127).repeat_interleave(128, 1)[:, :q.data.shape[1]])[:, :q.cols]
+
+
+@pytest.mark.parametrize("m,n,k,out", [(4000, 3700, 1100, BF16), (4000, 3700, 1100, F32), (20000, 520, 300, F16), (9000, 1100, 130, F32), (8, 100100, 130, BF16), (100, 300, 20000, BF16),
+                                       (20, 300, 20000, F32), (3500, 70, 700, BF16), (70000, 128, 64, BF16), (129, 33000, 200, F32)])
+def test_linear_fp8_tiles_and_splits(m, n, k, out):
+    """large tiles, more tiles than places, tiles of 32 rows, split sums, x rounded inside the product: each with a ragged edge"""
+    g = torch.Generator(device=DEV).manual_seed(m)
+    x = (torch.randn(m, k, device=DEV, generator=g) * torch.exp(torch.randn(m, 1, device=DEV, generator=g))).to(BF16)
+    w8 = A.quantize_fp8(torch.randn(n, k, device=DEV, generator=g) * k ** -0.5, 128)
+    bias = torch.randn(n, device=DEV, generator=g)
+    y = A.linear_fp8(x, w8, bias, out_dtype=out)
+    _check_large(y, x, w8, bias)
+    apart = A.matmul_fp8(A.quantize_fp8(x), w8, bias, out_dtype=out)
+    _check_large(apart, x, w8, bias)
+    assert torch.equal(y, A.linear_fp8(x, w8, bias, out_dtype=out)) and torch.equal(apart, A.matmul_fp8(A.quantize_fp8(x), w8, bias, out_dtype=out))
+
+
+def test_fp8_offsets_past_32_bits():
+    k, stride = 200, (1 << 30) + 8
+    near = torch.randn(3, k, generator=_gen(1)).to(BF16).to(DEV)
+    store = torch.empty(2 * stride + k, dtype=BF16, device=DEV)
+    far = store.as_strided((3, k), (stride, 1))
+    far.copy_(near)
+    w = torch.randn(150, k, generator=_gen(2)).to(DEV)
+    assert torch.equal(A.linear_fp8(far, w), A.linear_fp8(near, w))
+    for block_rows in (1, 128):
+        for transpose in (False, True):
+            a, b = A.quantize_fp8(far, block_rows, transpose), A.quantize_fp8(near, block_rows, transpose)
+            assert torch.equal(a.data.view(torch.uint8), b.data.view(torch.uint8)) and torch.equal(a.scale, b.scale)
+
+
 # ---- the operators together: a label head over rays, its training step and its answers ----
 
 def test_label_head_learns_and_answers():
@@ -533,6 +599,29 @@ def test_replayed_graph_and_second_stream():
         assert torch.equal(loss, want[0]) and torch.equal(grad, want[1]) and torch.equal(label, A.sample_logits(z, u, top_p=0.9))
         assert torch.equal(y, A.linear_fp8(z, z[:100]))
         torch.cuda.synchronize()
+
+
+def test_two_calls_at_once():
+    """the same calls on two streams at a time: nothing is shared between them"""
+    z, t, i, u = (x.to(DEV) for x in _case(40, 20000, 9, BF16, F32, 6))
+    u = u - 0.25
+    w8 = A.quantize_fp8(z[:, :4000], 128)
+    x = z[:, 4000:8000]
+
+    def calls():
+        return (A.sample_logits(z, u, top_p=0.9), *A.distill_top_logits_grad(z, t, i, u), A.linear_fp8(x, w8), A.sample_logits(z, u, temperature=2.0))
+
+    want = calls()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(calls())
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, want))
 
 
 def test_replayed_training_step():
