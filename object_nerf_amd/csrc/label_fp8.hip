@@ -602,13 +602,16 @@ __global__ void __launch_bounds__(256) join_splits_kernel(GemmP p, int splits) {
   store4<E>(p, m, n, v);
 }
 
-// Tile and split of a product.  Up to 32 rows: 32 x 128 per workgroup.  256 x 256 (one workgroup per CU, 128 KB of LDS) where such tiles
-// fill the card and the sum is long enough to run behind its copies.  Else 128 x 128, two workgroups per CU.  The sum is split
-// where there are fewer tiles than places.
+// Tile and split of a product.  Up to 32 rows: 32 x 128 per workgroup.  Else 256 x 256, one workgroup per CU, or 128 x 128, two per CU.  A
+// round of the larger takes as long as 1.8 of the smaller (four times the work at 1.1 times the rate, against twice); the larger is
+// taken where its whole rounds take less and the sum has four blocks at least: 8192 x 8192 x 8192 480 us against 525, 8192 x 8192 x 512
+// 58 against 64, but 16383 x 2056 x 640 (2.25 rounds) 49 against 42, 307200 x 256 x 256 60 against 57.  The sum is split where there
+// are fewer tiles than places.
 struct Plan { int bm, bn, splits; long blocks; };
 inline Plan plan_of(long M, long N, long K, bool wide, bool raw) {
   const long blocks = K / kBlock;
-  if (!wide && !raw && blocks >= 8 && ((M + 255) / 256) * ((N + 255) / 256) >= 224) return Plan{256, 256, 1, blocks};
+  const long big = (((M + 255) / 256) * ((N + 255) / 256) + 255) / 256, small = (((M + 127) / 128) * ((N + 127) / 128) + 511) / 512;     // rounds
+  if (!wide && !raw && blocks >= 4 && small > 1 && big * 18 < small * 10) return Plan{256, 256, 1, blocks};
   const int bm = M <= 32 ? 32 : 128;
   const long tiles = ((M + bm - 1) / bm) * ((N + 127) / 128);
   long splits = tiles >= 256 ? 1 : 512 / tiles;                  // two workgroups per CU

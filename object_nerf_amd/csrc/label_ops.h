@@ -83,7 +83,7 @@ struct OpMax {
 struct OpMin { template <class T> static __device__ __forceinline__ T f(T a, T b) { return a < b ? a : b; } };
 
 template <int CTRL> __device__ __forceinline__ unsigned dpp_u32(unsigned v) {
-  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, false);
+  return (unsigned)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
 }
 // CTRL of the steps inside a row of 16: lanes xor 1, xor 2 (quad_perm), then quads (half mirror), then halves (mirror)
 template <int CTRL> __device__ __forceinline__ float lane_step(float v) { return __uint_as_float(dpp_u32<CTRL>(__float_as_uint(v))); }

@@ -32,24 +32,28 @@ struct SampleP {
   int v;
   const void* z; long ldz;
   const float* u; long ldu;
-  const float* t; double t0;              // per row, or one number where the pointer is null
+  const float* t; double c0;              // per row, or one number where the pointer is null: log2(e) / T, 0 for the first of the order
   const int32_t* top_k; int top_k0;
   const float* top_p; double top_p0;
-  const float* min_p; double min_p0;
+  const float* min_p; double reach0;      // -log2(min_p)
   int shift;
   int64_t* out;
 };
 struct Settings {
-  double t, top_p, min_p;
+  double c;                               // log2(e) / T; 0: the first of the order
+  double reach;                           // how far a label may lie below the largest, in (logit c): -log2(min_p); the strongest always stays
+  double top_p;
   int top_k;                              // <= 0: off
   float u;
 };
+__host__ __device__ __forceinline__ double scale_of(double t) { return t > 0.0 ? fmin(1.4426950408889634 / t, 1e300) : 0.0; }
+__host__ __device__ __forceinline__ double reach_of(double min_p) { return min_p > 0.0 ? fmax(-log2(min_p), 0.0) : __builtin_inf(); }
 __device__ __forceinline__ Settings settings_of(const SampleP& p, long r) {
   Settings s;
-  s.t = p.t ? (double)p.t[r] : p.t0;
+  s.c = p.t ? scale_of((double)p.t[r]) : p.c0;
   s.top_k = p.top_k ? p.top_k[r] : p.top_k0;
   s.top_p = p.top_p ? (double)p.top_p[r] : p.top_p0;
-  s.min_p = p.min_p ? (double)p.min_p[r] : p.min_p0;
+  s.reach = p.min_p ? reach_of((double)p.min_p[r]) : p.reach0;
   s.u = p.u[r * p.ldu];
   return s;
 }
@@ -86,8 +90,18 @@ struct Weight {
     return z == zmax ? 1ull << shift : whole;                    // also where both are +inf
   }
 };
+__constant__ const double kTable[32] = {
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002,
+};
 __device__ __forceinline__ void fill_table(double* table) {
-  if (threadIdx.x < 32) table[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / 32.0));
+  if (threadIdx.x < 32) table[threadIdx.x] = kTable[threadIdx.x];
 }
 
 // positions in the running sum: the one on which the top_p border falls (its label is the last one kept), and u's
@@ -101,21 +115,11 @@ __device__ __forceinline__ uint64_t position_of(float u, uint64_t kept) {
   const uint64_t at = want >= 1.0 ? (want < (double)kept ? (uint64_t)want : kept - 1) : 0;
   return at < kept ? at : kept - 1;
 }
-// -log2(min_p): what a label may lie below the largest in units of log2(e) / T; the strongest label always stays
-__device__ __forceinline__ double reach_of(double min_p) { return min_p > 0.0 ? fmax(-log2(min_p), 0.0) : __builtin_inf(); }
 __device__ __forceinline__ bool is_strong(const Weight& w, float logit, double reach) { return !((w.zmax - (double)logit) * w.c > reach); }
 
 // ---- rows of up to LANES x PER labels: a sorting network in registers ----
-// The key as a double, so that a comparison is one instruction: sign 0, exponent field in [0x400, 0x5ff] (never NaN), order bits, then
-// the complement of the index; nothing to draw: 0.0.
-constexpr uint64_t kKeyBase = 0x4000000000000000ull;
-constexpr unsigned kIndexMask = 0x1fffffffu;
-__device__ __forceinline__ double sort_key(float z, int index) {
-  const unsigned b = order_bits(z);
-  return b == kNothing ? 0.0 : __longlong_as_double((long long)(kKeyBase | ((uint64_t)b << 29) | (kIndexMask - (unsigned)index)));
-}
-__device__ __forceinline__ unsigned sorted_bits(double k) { return (unsigned)((uint64_t)__double_as_longlong(k) >> 29); }
-__device__ __forceinline__ int sorted_index(double k) { return (int)(kIndexMask - ((unsigned)(uint64_t)__double_as_longlong(k) & kIndexMask)); }
+// On the order bits alone: weights of equal logits are equal, so the running sums do not ask which of them comes first.  Position
+// t PER + i of the order is register i of lane t.
 
 template <int MASK> __device__ __forceinline__ unsigned lane_xor(unsigned v) {
   if constexpr (MASK == 1) return dpp_u32<0xB1>(v);
@@ -135,30 +139,27 @@ template <int MASK> __device__ __forceinline__ unsigned lane_xor(unsigned v) {
     return upper ? a : b;
   }
 }
-template <int MASK> __device__ __forceinline__ double lane_xor(double v) {
-  const uint64_t x = (uint64_t)__double_as_longlong(v);
-  return __longlong_as_double((long long)(((uint64_t)lane_xor<MASK>((unsigned)(x >> 32)) << 32) | lane_xor<MASK>((unsigned)x)));
-}
-__device__ __forceinline__ void order_pair(double& a, double& b) {
-  const double hi = fmax(a, b), lo = fmin(a, b);
+__device__ __forceinline__ void order_pair(unsigned& a, unsigned& b) {
+  const unsigned hi = max(a, b), lo = min(a, b);
   a = hi;
   b = lo;
 }
-// one step across lanes: the lower lane keeps the larger.  MIRROR: the partner's registers in reverse order
-template <int MASK, int PER, bool MIRROR> __device__ __forceinline__ void lane_exchange(double (&x)[PER]) {
+// one step across lanes: the lower lane keeps the larger -- the median of both and all ones, or 0.  MIRROR: the partner's registers in
+// reverse order
+template <int MASK, int PER, bool MIRROR> __device__ __forceinline__ void lane_exchange(unsigned (&x)[PER]) {
   constexpr int top = MASK >= 32 ? 32 : MASK >= 16 ? 16 : MASK >= 8 ? 8 : MASK >= 4 ? 4 : MASK >= 2 ? 2 : 1;
-  const bool upper = threadIdx.x & top;
-  double y[PER];
+  const unsigned third = threadIdx.x & top ? 0u : ~0u;
+  unsigned y[PER];
 #pragma unroll
   for (int r = 0; r < PER; ++r) y[r] = lane_xor<MASK>(x[r]);
 #pragma unroll
   for (int r = 0; r < PER; ++r) {
-    const double o = y[MIRROR ? PER - 1 - r : r];
-    x[r] = (x[r] > o) != upper ? x[r] : o;
+    const unsigned o = y[MIRROR ? PER - 1 - r : r];
+    x[r] = max(min(x[r], o), min(max(x[r], o), third));
   }
 }
 // merges of register pairs at distances D, D / 2, .. 1
-template <int PER, int D> __device__ __forceinline__ void register_steps(double (&x)[PER]) {
+template <int PER, int D> __device__ __forceinline__ void register_steps(unsigned (&x)[PER]) {
   if constexpr (D >= 1) {
 #pragma unroll
     for (int r = 0; r < PER; ++r)
@@ -166,7 +167,7 @@ template <int PER, int D> __device__ __forceinline__ void register_steps(double 
     register_steps<PER, D / 2>(x);
   }
 }
-template <int PER, int K> __device__ __forceinline__ void register_sort(double (&x)[PER]) {
+template <int PER, int K> __device__ __forceinline__ void register_sort(unsigned (&x)[PER]) {
   if constexpr (K <= PER) {
 #pragma unroll
     for (int r = 0; r < PER; ++r)
@@ -175,13 +176,13 @@ template <int PER, int K> __device__ __forceinline__ void register_sort(double (
     register_sort<PER, K * 2>(x);
   }
 }
-template <int PER, int D> __device__ __forceinline__ void lane_steps(double (&x)[PER]) {
+template <int PER, int D> __device__ __forceinline__ void lane_steps(unsigned (&x)[PER]) {
   if constexpr (D >= 1) {
     lane_exchange<D, PER, false>(x);
     lane_steps<PER, D / 2>(x);
   }
 }
-template <int LANES, int PER, int K> __device__ __forceinline__ void lane_sort(double (&x)[PER]) {     // K lanes hold a sorted run afterwards
+template <int LANES, int PER, int K> __device__ __forceinline__ void lane_sort(unsigned (&x)[PER]) {     // K lanes hold a sorted run afterwards
   if constexpr (K <= LANES) {
     lane_exchange<K - 1, PER, true>(x);
     lane_steps<PER, K / 4>(x);
@@ -190,9 +191,13 @@ template <int LANES, int PER, int K> __device__ __forceinline__ void lane_sort(d
   }
 }
 template <int CTRL, int ROWS> __device__ __forceinline__ uint64_t shifted_in(uint64_t v) {
-  const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)v, CTRL, ROWS, 0xf, true);
-  const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), CTRL, ROWS, 0xf, true);
-  return ((uint64_t)hi << 32) | lo;
+  if constexpr (ROWS == 0xf) {                                   // lanes without a source get 0
+    return ((uint64_t)dpp_u32<CTRL>((unsigned)(v >> 32)) << 32) | dpp_u32<CTRL>((unsigned)v);
+  } else {
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)v, CTRL, ROWS, 0xf, true);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), CTRL, ROWS, 0xf, true);
+    return ((uint64_t)hi << 32) | lo;
+  }
 }
 // inclusive prefix sum over the lanes of a row
 template <int LANES> __device__ __forceinline__ uint64_t lanes_scan(uint64_t v) {
@@ -217,46 +222,35 @@ __global__ void __launch_bounds__(256) sample_sorted_kernel(SampleP p) {
   const long r = at < p.n ? at : p.n - 1;
   const char* z = static_cast<const char*>(p.z) + r * p.ldz * E::kBytes;
   const Settings set = settings_of(p, r);
-  double x[PER];
-  if constexpr (PER * E::kBytes >= 16) {
-    if (t * PER + PER <= p.v) {
+  unsigned own[PER], x[PER];                                     // as they lie in the row; in order
+  if (PER * E::kBytes >= 16 && t * PER + PER <= p.v) {
 #pragma unroll
-      for (int h = 0; h < PER / E::kVec; ++h) {
-        float f[E::kVec];
-        E::unpack(load16(z, ((long)t * PER + h * E::kVec) * E::kBytes), f);
+    for (int h = 0; h < PER / E::kVec; ++h) {
+      float f[E::kVec];
+      E::unpack(load16(z, ((long)t * PER + h * E::kVec) * E::kBytes), f);
 #pragma unroll
-        for (int i = 0; i < E::kVec; ++i) x[h * E::kVec + i] = sort_key(f[i], t * PER + h * E::kVec + i);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < PER; ++i) x[i] = t * PER + i < p.v ? sort_key(E::load(z, t * PER + i), t * PER + i) : 0.0;
+      for (int i = 0; i < E::kVec; ++i) own[h * E::kVec + i] = order_bits(f[i]);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) x[i] = t * PER + i < p.v ? sort_key(E::load(z, t * PER + i), t * PER + i) : 0.0;
+    for (int i = 0; i < PER; ++i) own[i] = t * PER + i < p.v ? order_bits(E::load(z, t * PER + i)) : kNothing;
   }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) x[i] = own[i];
   register_sort<PER, 2>(x);
   lane_sort<LANES, PER, 2>(x);
 
-  // the largest, in every lane of the row
-  const uint64_t own = (uint64_t)__double_as_longlong(x[0]);
-  const uint64_t first = ((uint64_t)(unsigned)__shfl((int)(own >> 32), 0, LANES) << 32) | (unsigned)__shfl((int)(unsigned)own, 0, LANES);
-  const bool some = first != 0;
-  Weight w;
-  w.zmax = (double)value_of((unsigned)(first >> 29));
-  w.c = 1.4426950408889634 / set.t;
-  w.shift = p.shift;
-  w.table = table;
-  const double reach = reach_of(set.min_p);
+  const unsigned top = lanes_reduce<LANES, OpMax>(x[0]);
+  const Weight w{(double)value_of(top), set.c, p.shift, table};
   uint64_t run[PER], sum = 0;
   unsigned strong = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const bool in = x[i] != 0.0 && (set.top_k <= 0 || t * PER + i < set.top_k);
-    const float logit = value_of(sorted_bits(x[i]));
+    const bool in = x[i] != kNothing && (set.top_k <= 0 || t * PER + i < set.top_k);
+    const float logit = value_of(x[i]);
     sum += in ? w.of(logit) : 0;
     run[i] = sum;
-    if (in && is_strong(w, logit, reach)) strong |= 1u << i;
+    if (in && is_strong(w, logit, set.reach)) strong |= 1u << i;
   }
   const uint64_t before = lanes_scan<LANES>(sum) - sum;
   const uint64_t all = lanes_reduce<LANES, OpSum>(sum);
@@ -269,16 +263,35 @@ __global__ void __launch_bounds__(256) sample_sorted_kernel(SampleP p) {
   }
   kept = lanes_reduce<LANES, OpMax>(kept);
   const uint64_t want = position_of(set.u, kept);
-  if (at >= p.n) return;
-  if (!some || !(set.t > 0.0)) {                                 // nothing to draw; or the first alone
-    if (t == 0) p.out[r] = some ? sorted_index(x[0]) : -1;
-    return;
-  }
+  unsigned hit = 0, place = 0;                                   // the logit on which `want` falls, and its place in the order
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const uint64_t ahead = before + (i ? run[i - 1] : 0);
-    if (ahead <= want && want < before + run[i]) p.out[r] = sorted_index(x[i]);
+    if (ahead <= want && want < before + run[i]) { hit = x[i]; place = (unsigned)(t * PER + i); }
   }
+  hit = lanes_reduce<LANES, OpMax>(hit);
+  place = lanes_reduce<LANES, OpMax>(place);
+  if (set.c == 0.0) { hit = top; place = 0; }                    // the first alone
+  // of the labels with this logit, the one with as many in front of it, by index, as `place` has in the order
+  unsigned better = 0, equal = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    better += x[i] > hit;
+    equal += own[i] == hit;
+  }
+  const unsigned nth = place - lanes_reduce<LANES, OpSum>(better);
+  unsigned seen = (unsigned)lanes_scan<LANES>((uint64_t)equal) - equal;
+  if (at >= p.n) return;
+  if (top == kNothing) {
+    if (t == 0) p.out[r] = -1;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (own[i] == hit) {
+      if (seen == nth) p.out[r] = t * PER + i;
+      ++seen;
+    }
 }
 
 // ---- longer rows: a workgroup each ----
@@ -515,11 +528,10 @@ __device__ __forceinline__ void draw_from_list(const Weight& w, const Settings& 
   }
   const uint64_t all = block_all<THREADS, OpSum>(sum, sh);
   const uint64_t border = set.top_p < 1.0 ? border_of(set.top_p, all) : ~0ull;
-  const double reach = reach_of(set.min_p);
   uint64_t kept = 0;
 #pragma unroll
   for (int h = 0; h < H; ++h)
-    if (key[h] && before[h] <= border && is_strong(w, value_of((unsigned)(key[h] >> 32)), reach)) kept = max(kept, before[h] + own[h]);
+    if (key[h] && before[h] <= border && is_strong(w, value_of((unsigned)(key[h] >> 32)), set.reach)) kept = max(kept, before[h] + own[h]);
   kept = block_all<THREADS, OpMax>(kept, sh);
   const uint64_t want = position_of(set.u, kept);
 #pragma unroll
@@ -528,12 +540,7 @@ __device__ __forceinline__ void draw_from_list(const Weight& w, const Settings& 
 }
 
 __device__ __forceinline__ Weight weight_of(const SampleP& p, const Settings& set, unsigned top, const double* table) {
-  Weight w;
-  w.zmax = (double)value_of(top);
-  w.c = 1.4426950408889634 / set.t;
-  w.shift = p.shift;
-  w.table = table;
-  return w;
+  return Weight{(double)value_of(top), set.c, p.shift, table};
 }
 // All labels of a row whose largest has order bits `top`, in steps down to where a weight is 0 as an integer, or to the least label that
 // counts as one (-1e30: what lies lower masks) where that is known.
@@ -549,7 +556,7 @@ template <int THREADS> __device__ __forceinline__ Steps all_steps(const Weight& 
   st.fit_bits();
   return st;
 }
-__device__ __forceinline__ bool is_single(const Settings& set) { return !(set.t > 0.0) || set.top_k == 1; }
+__device__ __forceinline__ bool is_single(const Settings& set) { return set.c == 0.0 || set.top_k == 1; }
 
 // What the histogram says of a row: with a top_k that cuts, the labels of bins 0 .. last_k are the candidates; else the border of
 // top_p lies in bin_p and u's position in one of bins low_u .. high_u.  Afterwards sh.mass holds the weight in front of each bin, and
@@ -759,8 +766,7 @@ __device__ void draw_row(const SampleP& p, long r, bool rest, Shared<THREADS>& s
     st.low = low;
     st.fit_bits();
   }
-  const double weak = reach_of(set.min_p);
-  const uint64_t strong = block_all<THREADS, OpSum>(histogram<false, THREADS>(row, w, st, weak, sh), sh);
+  const uint64_t strong = block_all<THREADS, OpSum>(histogram<false, THREADS>(row, w, st, set.reach, sh), sh);
   Places pl = places_of<THREADS>(sh.mass, sh.count, strong, set, sh);
   if (threadIdx.x == 0) sh.listed = 0;
   __syncthreads();
@@ -918,7 +924,7 @@ __global__ void __launch_bounds__(kSplitThreads, 4) split_histogram_kernel(Sampl
   }
   fill_table(sh.table);
   const Weight w = weight_of(p, set, top, sh.table);
-  uint64_t strong = histogram<false, kSplitThreads>(row, w, all_steps<kSplitThreads>(w, top, least_label(sp, r)), reach_of(set.min_p), sh);
+  uint64_t strong = histogram<false, kSplitThreads>(row, w, all_steps<kSplitThreads>(w, top, least_label(sp, r)), set.reach, sh);
   for (int i = threadIdx.x; i < kSplitBins; i += kSplitThreads)
     if (sh.count[i]) {
       atomicAdd(&sr.count[i], sh.count[i]);
@@ -1076,7 +1082,7 @@ int launch_sample(const SampleP& p, void* workspace, hipStream_t s) {
     } else {
       // a kernel for small top_k pays where rows wait for a place on the card (2048 rows of 32768 bf16, top_k 50: 80 -> 57 us); where
       // all are on it at once, a second kernel only follows the first (257 rows of 30011, some with a top_k: 46 -> 62 us)
-      const bool small = p.t || p.top_k || !(p.t0 > 0.0) || (p.top_k0 >= 1 && p.top_k0 <= kPrune), light = small && p.n > 512;
+      const bool small = p.t || p.top_k || p.c0 == 0.0 || (p.top_k0 >= 1 && p.top_k0 <= kPrune), light = small && p.n > 512;
       const dim3 grid((unsigned)p.n);
       if (light) hipLaunchKernelGGL((sample_top_kernel<E>), grid, dim3(256), 0, s, p);
       // one workgroup of 1,024 threads to a CU, two of 512: the larger where that is a row's CU to itself
@@ -1116,10 +1122,10 @@ extern "C" int objnerf_sample_logits(const objnerf_sample_args* a, void* stream)
   p.n = a->n; p.v = a->v;
   p.z = a->logits; p.ldz = a->logits_stride;
   p.u = a->u; p.ldu = a->u_stride;
-  p.t = a->temperature_rows; p.t0 = a->temperature;
+  p.t = a->temperature_rows; p.c0 = scale_of(a->temperature);
   p.top_k = a->top_k_rows; p.top_k0 = (int)(a->top_k < a->v ? a->top_k : 0);
   p.top_p = a->top_p_rows; p.top_p0 = a->top_p;
-  p.min_p = a->min_p_rows; p.min_p0 = a->min_p;
+  p.min_p = a->min_p_rows; p.reach0 = reach_of(a->min_p);
   int log_v = 0;
   while ((1ll << log_v) < (long long)a->v) ++log_v;
   p.shift = 62 - log_v < 51 ? 62 - log_v : 51;
