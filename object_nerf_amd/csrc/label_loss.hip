@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES, LANES < 1024 ? 6 : 
   constexpr bool kGroups = LANES <= 64;                          // several rows per workgroup: one slot per thread at most
   constexpr float kInf = __builtin_inff();
   __shared__ float tmp[6][kThreads / 64];
-  __shared__ int slot_i[kGroups ? kThreads : kMaxSlots];
+  __shared__ __align__(16) int slot_i[kGroups ? kThreads : kMaxSlots];
   __shared__ float slot_e[kGroups ? kThreads : kMaxSlots];
   const int t = kGroups ? threadIdx.x & (LANES - 1) : threadIdx.x;
   const long at = kGroups ? (long)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES : blockIdx.x;
@@ -130,6 +130,7 @@ __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES, LANES < 1024 ? 6 : 
   float tm = t0, some = i0 >= 0 ? 1.f : 0.f;
   if constexpr (!kGroups) {
     if (t < p.k) { my_i[t] = i0; my_e[t] = t0; }
+    if (t < (p.k + 3) / 4 * 4 - p.k) my_i[p.k + t] = -1;
     for (int j = t + LANES; j < p.k; j += LANES) {
       int i = slot_column(p, row, j);
       const float v = i >= 0 ? load_any(p.t, row * p.ldt + j, p.t_type) : -kInf;
@@ -222,11 +223,18 @@ __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES, LANES < 1024 ? 6 : 
     if (i < 0) continue;
     float share = 0.f;
     bool first = true;
-    for (int l = 0; l < p.k; ++l)
-      if (my_i[l] == i) {
-        if (l < j) first = false;
-        share += my_e[l];
-      }
+#pragma unroll 4
+    for (int l = 0; l < p.k; l += 4) {                           // (behind the last slot: -1)
+      const int4 o = *reinterpret_cast<const int4*>(my_i + l);
+      const int same[4] = {o.x == i, o.y == i, o.z == i, o.w == i};
+      if (same[0] | same[1] | same[2] | same[3])
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (same[q]) {
+            if (l + q < j) first = false;
+            share += my_e[l + q];
+          }
+    }
     const float zi = j == t ? z0 : E::load(z, i);
     if (first) E::store(dz, i, g * (fast_exp2((zi - m) * p.c) / s - share / A));
   }

@@ -93,16 +93,12 @@ def _quantize(x, block_rows, rows=True, columns=False, sums=False):
     q = _empty_fp8(r, c, x.device) if rows else None
     t = _empty_fp8(c, r, x.device) if columns else None
     total = None
-    a = _lib.Fp8QuantizeArgs()
-    a.rows, a.cols, a.x, a.x_stride, a.type, a.block_rows = r, c, x.data_ptr(), x.stride(0), _TYPES[x.dtype], block_rows
-    if rows:
-        a.values, a.scales = q.data.data_ptr(), q.scale.data_ptr()
-    if columns:
-        a.values_t, a.scales_t = t.data.data_ptr(), t.scale.data_ptr()
+    work = None
     if sums:
         work = torch.empty(_up(r, BLOCK) // BLOCK * c, dtype=torch.float32, device=x.device)
         total = torch.empty(c, dtype=torch.float32, device=x.device)
-        a.workspace, a.column_sums = work.data_ptr(), total.data_ptr()
+    a = _lib.Fp8QuantizeArgs(r, c, x.data_ptr(), x.stride(0), _TYPES[x.dtype], block_rows, *((q.data.data_ptr(), q.scale.data_ptr()) if rows else (None, None)),
+                             *((t.data.data_ptr(), t.scale.data_ptr()) if columns else (None, None)), *((total.data_ptr(), work.data_ptr()) if sums else (None, None)))
     if r and c:
         _call(_lib.lib().objnerf_fp8_quantize, a, x.device, "fp8_quantize")
     return q, t, total
