@@ -4,6 +4,13 @@
 //         max|block| / s <= 448, held as the byte 127 + log2 s; element = e4m3(x / s), to nearest even
 //   C[m][n] = sum_k a[m][k] b[n][k] (+ bias[n]) (LeakyReLU)
 //
+// Measured (copy of this card 4.96 TB/s, fp8 product of the library at 8192 x 8192 x 8192 2.77 PFLOP/s): rounding 307,200 x 256 bf16 by
+// rows 46 us = 5.1 TB/s, 16,383 x 2,056 in both forms 33 us = 4.1 TB/s; product 8192 x 8192 x 8192 480 us = 2.29 PFLOP/s, x 4096
+// 259 us = 2.12 PFLOP/s, 4096 x 4096 x 4096 64 us = 2.15 PFLOP/s, 2,056 x 520 x 16,384 with fp32 results 56 us = 0.63 PFLOP/s; four
+// rows against 32,768 x 256 (8.4 MB of weights) 4 us.  What bounds it: large products the matrix pipe at the clock that it leaves itself and the two slots' copies, which
+// have one block's products to arrive in; sums of a few blocks the launch-to-store latency of a tile; hidden layers over a frame the
+// write path.
+//
 // The scale is a power of two on purpose.  Dividing by it is exact, so an element is rounded once and the byte form has one meaning;
 // a factor up to 2 of the range it gives away costs no precision (a floating-point format's step does not depend on where in its
 // range a value lies, down to its subnormals at 2^-15 of the block's largest).  And it is the form that the matrix instruction itself
@@ -591,11 +598,22 @@ __global__ void __launch_bounds__(256) join_splits_kernel(GemmP p, int splits) {
   if (at >= p.M * groups) return;
   const long m = at / groups, n = (at - m * groups) * 4;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < splits; ++s) {
-    const float* o = p.partial + ((long)s * p.M + m) * p.N + n;
+  const bool whole = n + 4 <= p.N;
+  for (int s = 0; s < splits; s += 4) {
+    f32x4 o[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (n + r < p.N) v[r] += o[r];
+    for (int u = 0; u < 4; ++u) {
+      const float* at_s = p.partial + ((long)min(s + u, splits - 1) * p.M + m) * p.N + n;
+      if (whole) {
+        __builtin_memcpy(&o[u], at_s, 16);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[u][r] = n + r < p.N ? at_s[r] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (s + u < splits) v += o[u];
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r) v[r] = finished(v[r], p, p.bias && n + r < p.N ? p.bias[n + r] : 0.f);
@@ -603,22 +621,35 @@ __global__ void __launch_bounds__(256) join_splits_kernel(GemmP p, int splits) {
 }
 
 // Tile and split of a product.  Up to 32 rows: 32 x 128 per workgroup.  Else 256 x 256, one workgroup per CU, or 128 x 128, two per CU.  A
-// round of the larger takes as long as 1.8 of the smaller (four times the work at 1.1 times the rate, against twice); the larger is
-// taken where its whole rounds take less and the sum has four blocks at least: 8192 x 8192 x 8192 480 us against 525, 8192 x 8192 x 512
-// 58 against 64, but 16383 x 2056 x 640 (2.25 rounds) 49 against 42, 307200 x 256 x 256 60 against 57.  The sum is split where there
-// are fewer tiles than places.
+// round of the larger takes as long as 1.8 of the smaller (four times the work at 1.1 times the rate, against twice), a last round of the
+// smaller with one tile per CU 0.6; the larger is taken where its rounds take less and the sum has four blocks at least: 8192 x 8192 x
+// 4096 245-259 us against 267, 8192 x 8192 x 512 58 against 60, 4096 x 4096 x 1024 25 against 27, but 16383 x 2056 x 640 49 against 39,
+// 16383 x 520 x 2176 36 against 33, 16384 x 512 x 2048 34 against 23, 307200 x 256 x 256 59 against 55.
+// The sum is split where a workgroup's share of the blocks (0.64 us each, 1.06 for fp32, half for 32 rows) and the joining kernel (2.3 us
+// and 0.55 us per MB of partial sums) take less than the whole: 2056 x 520 x 16384 40 us against 84 in one, 512 x 512 x 4096 14 / 25, 128 x
+// 128 x 8192 11 / 44, 16 x 4096 x 4096 8.5 / 13.3, but 1000 x 1000 x 1000 in two 13.8 / 10.3, 1000 x 1000 x 2048 in four 19 / 15.5.
 struct Plan { int bm, bn, splits; long blocks; };
 inline Plan plan_of(long M, long N, long K, bool wide, bool raw) {
   const long blocks = K / kBlock;
-  const long big = (((M + 255) / 256) * ((N + 255) / 256) + 255) / 256, small = (((M + 127) / 128) * ((N + 127) / 128) + 511) / 512;     // rounds
-  if (!wide && !raw && blocks >= 4 && small > 1 && big * 18 < small * 10) return Plan{256, 256, 1, blocks};
+  const long big = (((M + 255) / 256) * ((N + 255) / 256) + 255) / 256, small = ((M + 127) / 128) * ((N + 127) / 128), over = small % 512;
+  const long rounds10 = small / 512 * 10 + (over == 0 ? 0 : over <= 256 ? 6 : 10);
+  if (!wide && !raw && blocks >= 4 && big * 18 < rounds10) return Plan{256, 256, 1, blocks};
   const int bm = M <= 32 ? 32 : 128;
   const long tiles = ((M + bm - 1) / bm) * ((N + 127) / 128);
-  long splits = tiles >= 256 ? 1 : 512 / tiles;                  // two workgroups per CU
-  splits = splits < blocks / 4 ? splits : blocks / 4;            // of at least four blocks each
-  if (splits < 2) return Plan{bm, 128, 1, blocks};
-  const long per = (blocks + splits - 1) / splits;
-  return Plan{bm, 128, (int)((blocks + per - 1) / per), per};
+  long most = tiles ? 512 / tiles : 1;                           // two workgroups per CU
+  most = most < blocks / 4 ? most : blocks / 4;                  // of at least four blocks each
+  const double block = (wide ? 1.06 : 0.64) * (bm == 32 ? 0.5 : 1.0), join = 2.2e-6 * M * N;
+  Plan best{bm, 128, 1, blocks};
+  double cost = block * blocks;
+  for (long s = 2; s <= most; s = s < most && s * 2 > most ? most : s * 2) {
+    const long per = (blocks + s - 1) / s, splits = (blocks + per - 1) / per;
+    const double c = block * per + 2.3 + join * splits;
+    if (c < cost) {
+      cost = c;
+      best = Plan{bm, 128, (int)splits, per};
+    }
+  }
+  return best;
 }
 
 template <class E, class A>
