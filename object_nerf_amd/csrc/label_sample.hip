@@ -16,6 +16,10 @@
 // picked out by a bound (the top_k-th largest of the threads' own maxima), else each question is answered by a histogram in equal
 // steps of the logit and by looking into the one bin in which the running sum crosses.
 //
+// Measured: 307,200 x 64 fp32 58 us (79 MB: 1.4 TB/s), bound by the vector units (about 550 instructions per four rows: 130 of them the
+// network, 100 the weights); 2,048 x 32,768 bf16 with top_k 50 53 us = 2.5 TB/s, bound by the chain of passes of a row; 257 x 30,011
+// fp16 39 us and one row of 131,072 32 us in four kernels, bound by latencies.
+//
 // NaN counts as -inf; a row of nothing but -inf draws -1.
 #include "host_api.h"
 #include "label_ops.h"
@@ -1037,12 +1041,14 @@ __global__ void __launch_bounds__(kSplitThreads, 4) split_draw_kernel(SampleP p,
 }
 
 struct SplitPlan { int parts, per; };
-// A row is spread where there are too few rows to fill the card: 1,024 workgroups in all, of at least 4,096 labels each.
-inline SplitPlan split_plan(long n, int v, int vec) {
+// A row is spread over several workgroups where its own passes take longer than the four kernels and the rows' turns in them: 1,024
+// workgroups in all, of at least 4,096 labels each.  bf16, one workgroup of 512 threads to a row against spread: 1 x 131072 117 against
+// 32 us, 1 x 32768 36 / 28, 64 x 131072 124 / 90, 128 x 131072 128 / 114, but 4 x 16384 24 / 28, 32 x 32768 36 / 39, 64 x 32768 37 / 48,
+// 256 x 131072 134 / 174.  With a small top_k a row costs an eighth of that by itself: 1 x 131072 26 / 29, 16 x 131072 27 / 47.
+inline SplitPlan split_plan(long n, int v, int vec, bool small_k) {
   const int pieces = v / vec;
-  long parts = n > 0 ? 1024 / n : 0;
-  if (parts > v / 4096) parts = v / 4096;
-  if (n > 128 || parts < 2) return SplitPlan{1, pieces};
+  const long most = n > 0 ? 1024 / n : 0, parts = most < v / 4096 ? most : v / 4096;
+  if (parts < 2 || v < (24576 + 768 * n) * (small_k ? 8 : 1)) return SplitPlan{1, pieces};
   const int per = (int)((pieces + parts - 1) / parts);
   return SplitPlan{(pieces + per - 1) / per, per};
 }
@@ -1050,7 +1056,9 @@ inline int64_t split_bytes(long n, const SplitPlan& plan) {
   return plan.parts < 2 ? 0 : n * (int64_t)sizeof(SplitRow) + n * plan.parts * 8;
 }
 
-// Up to 512 labels: the sorting network (16 lanes where 8 labels each are enough).  Above: a workgroup per row, or several.
+// Up to 512 labels: the sorting network, in the 16 lanes of a row of the vector unit, whose steps are all within it (65536 x 128 28 us
+// against 53 with 64 lanes), 64 lanes for 512 labels, and for 256 where that many rows do not fill the card (65536 x 256 82 us with 64
+// lanes, 52 with 16; 2048 x 256 5.4 and 7.6).  Above: a workgroup per row, or several (32768 x 512 75 us sorted, 314 in workgroups).
 template <class E>
 int launch_sample(const SampleP& p, void* workspace, hipStream_t s) {
   auto sorted = [&](auto lanes, auto per) {
@@ -1063,10 +1071,12 @@ int launch_sample(const SampleP& p, void* workspace, hipStream_t s) {
   else if (p.v <= 32) OBJ_SORTED(16, 2);
   else if (p.v <= 64) OBJ_SORTED(16, 4);
   else if (p.v <= 128) OBJ_SORTED(16, 8);
+  else if (p.v <= 256 && p.n > 4096) OBJ_SORTED(16, 16);
   else if (p.v <= 256) OBJ_SORTED(64, 4);
   else if (p.v <= 512) OBJ_SORTED(64, 8);
   else {
-    const SplitPlan plan = split_plan(p.n, p.v, E::kVec);
+    const bool small_k = p.top_k0 >= 1 && p.top_k0 <= kPrune && !p.top_k;
+    const SplitPlan plan = split_plan(p.n, p.v, E::kVec, small_k);
     if (plan.parts > 1) {
       SplitP sp;
       sp.rows = static_cast<SplitRow*>(workspace);
@@ -1080,15 +1090,15 @@ int launch_sample(const SampleP& p, void* workspace, hipStream_t s) {
       hipLaunchKernelGGL((split_collect_kernel<E>), grid, block, 0, s, p, sp);
       hipLaunchKernelGGL((split_draw_kernel<E>), dim3((unsigned)p.n), block, 0, s, p, sp);
     } else {
-      // a kernel for small top_k pays where rows wait for a place on the card (2048 rows of 32768 bf16, top_k 50: 80 -> 57 us); where
-      // all are on it at once, a second kernel only follows the first (257 rows of 30011, some with a top_k: 46 -> 62 us)
-      const bool small = p.t || p.top_k || p.c0 == 0.0 || (p.top_k0 >= 1 && p.top_k0 <= kPrune), light = small && p.n > 512;
+      // a kernel for small top_k pays where rows wait for a place on the card (2048 rows of 32768 bf16, top_k 50: 74 -> 55 us, 768: 35 ->
+      // 28); where all are on it at once, a second kernel only follows the first (512: 22 and 22, 257 of 30011: 18 -> 20)
+      const bool light = p.n > 512 && (p.t || p.top_k || p.c0 == 0.0 || small_k);
       const dim3 grid((unsigned)p.n);
       if (light) hipLaunchKernelGGL((sample_top_kernel<E>), grid, dim3(256), 0, s, p);
-      // one workgroup of 1,024 threads to a CU, two of 512: the larger where that is a row's CU to itself
-      if (p.v <= 4096) hipLaunchKernelGGL((sample_row_kernel<E, 256>), grid, dim3(256), 0, s, p, light);
-      else if (p.n > 256) hipLaunchKernelGGL((sample_row_kernel<E, 512>), grid, dim3(512), 0, s, p, light);
-      else hipLaunchKernelGGL((sample_row_kernel<E, 1024>), grid, dim3(1024), 0, s, p, light);
+      // 512 threads where all rows are on the card at once (512 x 8192 22.6 us against 24.0 with 256 threads, 200 x 32768 42 / 65, 512 x
+      // 131072 196 / 253), 256 where rows wait for places or are short (1024 x 8192 33 / 42, 2048 x 32768 178 / 193, 200 x 2048 11.7 / 13.1)
+      if (p.v <= 4096 || p.n > 512) hipLaunchKernelGGL((sample_row_kernel<E, 256>), grid, dim3(256), 0, s, p, light);
+      else hipLaunchKernelGGL((sample_row_kernel<E, 512>), grid, dim3(512), 0, s, p, light);
     }
   }
 #undef OBJ_SORTED
@@ -1102,7 +1112,7 @@ using namespace objnerf;
 
 extern "C" int64_t objnerf_sample_logits_workspace_bytes(int64_t n, int32_t v, int type) {
   if (n <= 0 || v <= 512 || !label_type_ok(type)) return 0;
-  return split_bytes(n, split_plan(n, v, 16 / label_type_bytes(type)));
+  return split_bytes(n, split_plan(n, v, 16 / label_type_bytes(type), false));
 }
 
 extern "C" int objnerf_sample_logits(const objnerf_sample_args* a, void* stream) {

@@ -241,6 +241,26 @@ def test_sample_many_rows_with_settings_of_their_own():
     _draw_check(z, u, temperature=torch.rand(n, generator=g) * 2 - 0.1, top_k=torch.randint(-1, 300, (n,), generator=g), top_p=torch.rand(n, generator=g) * 1.2)
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=5), dict(temperature=0.8, top_k=40, top_p=0.95, min_p=0.01), dict(top_k=170), dict(temperature=0.0), dict(temperature=30.0, top_p=0.6)],
+                         ids=str)
+@pytest.mark.parametrize("n,v,dtype", [(4100, 129, F16), (4500, 200, BF16), (4097, 256, F32), (2, 262144, BF16), (20, 49152, F32)])
+def test_sample_sixteen_labels_per_lane_and_rows_over_workgroups(n, v, dtype, kw):
+    g = _gen(v + 1)
+    z = (torch.randn(n, v, generator=g) * 2.5).to(dtype)
+    z[0] = 0.5
+    if n > 2:
+        z[1] = -math.inf
+        z[2, 10:] = -math.inf
+    _draw_check(z, torch.rand(n, generator=g), **kw)
+
+
+def test_sample_rows_over_workgroups_with_settings_of_their_own():
+    n, v = 20, 49152
+    g = _gen(5)
+    z, u = torch.randn(n, v, generator=g) * 2, torch.rand(n, generator=g)
+    _draw_check(z, u, temperature=torch.rand(n, generator=g) * 2 - 0.1, top_k=torch.randint(-1, 300, (n,), generator=g), top_p=torch.rand(n, generator=g) * 1.2)
+
+
 @pytest.mark.parametrize("v", [3, 64, 100, 900, 3001, 66000])
 def test_sample_ties(v):
     g = _gen(1)
