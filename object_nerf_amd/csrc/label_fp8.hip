@@ -93,7 +93,7 @@ __host__ __device__ __forceinline__ long scale_stride(long n) { return (blocks_o
 template <class E>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantP p) {
   const long kb = blocks_of(p.cols), sb = scale_stride(p.cols);
-  const long block = (long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const long block = workgroup() * 16 + (threadIdx.x >> 4);
   const int l = threadIdx.x & 15;
   const bool in = block < p.rows * kb;
   const long row = in ? block / kb : 0, b = in ? block - row * kb : 0;
@@ -126,7 +126,8 @@ __global__ void __launch_bounds__(256, 4) quantize_tile_kernel(QuantP p) {
   __shared__ unsigned col_byte[kBlock];
   __shared__ __align__(16) uint8_t tile[TRANS ? kBlock * kPitch : 16];
   const long kb = blocks_of(p.cols), sb = scale_stride(p.cols), mb = blocks_of(p.rows), sbt = scale_stride(p.rows);
-  const long bc = blockIdx.x % kb, br = blockIdx.x / kb;
+  const long bc = workgroup() % kb, br = workgroup() / kb;
+  if (br >= mb) return;
   const int g = threadIdx.x >> 4, l = threadIdx.x & 15;
   const long r0 = br * kBlock + g * 8, c0 = bc * kBlock + l * 8;
   Eight<E> held[8];
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(256, 4) quantize_tile_kernel(QuantP p) {
 __global__ void __launch_bounds__(256) join_sums_kernel(const float* __restrict__ part, long blocks, long cols, float* __restrict__ sum) {
   __shared__ float s[16][16];
   const int l = threadIdx.x & 15, g = threadIdx.x >> 4;
-  const long col = (long)blockIdx.x * 16 + l;
+  const long col = workgroup() * 16 + l;
   const long per = (blocks + 15) / 16;
   float a = 0.f;
   if (col < cols)
@@ -251,9 +252,9 @@ template <class E>
 int launch_quantize(const QuantP& p, bool square, float* sum, hipStream_t s) {
   const long tiles = blocks_of(p.rows) * blocks_of(p.cols);
   if (!square && !p.qt && !p.part) {
-    hipLaunchKernelGGL((quantize_rows_kernel<E>), dim3((unsigned)((p.rows * blocks_of(p.cols) + 15) / 16)), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((quantize_rows_kernel<E>), grid_of((p.rows * blocks_of(p.cols) + 15) / 16), dim3(256), 0, s, p);
   } else {
-    const dim3 grid((unsigned)tiles);
+    const dim3 grid = grid_of(tiles);
     if (square) {
       if (p.q && p.qt) hipLaunchKernelGGL((quantize_tile_kernel<E, true, true, true>), grid, dim3(256), 0, s, p);
       else if (p.q) hipLaunchKernelGGL((quantize_tile_kernel<E, true, false, true>), grid, dim3(256), 0, s, p);
@@ -264,7 +265,7 @@ int launch_quantize(const QuantP& p, bool square, float* sum, hipStream_t s) {
       else hipLaunchKernelGGL((quantize_tile_kernel<E, false, true, false>), grid, dim3(256), 0, s, p);
     }
   }
-  if (sum) hipLaunchKernelGGL(join_sums_kernel, dim3((unsigned)((p.cols + 15) / 16)), dim3(256), 0, s, p.part, blocks_of(p.rows), p.cols, sum);
+  if (sum) hipLaunchKernelGGL(join_sums_kernel, grid_of((p.cols + 15) / 16), dim3(256), 0, s, p.part, blocks_of(p.rows), p.cols, sum);
   return check_launch("fp8_quantize");
 }
 
@@ -737,6 +738,7 @@ int objnerf_gemm_fp8(const objnerf_gemm_fp8_args* a, void* stream) {
     return set_error(-1, "gemm_fp8: 8-bit operands must be 16-byte, scales 4-byte aligned");
   if (a->M == 0 || a->N == 0) return 0;
   if (((a->M + 31) / 32) > (1 << 30) / ((a->N + 127) / 128)) return set_error(-1, "gemm_fp8: more than 2^30 tiles");
+  if (a->K == 0 && ((a->M + 31) / 32) * ((a->N + 127) / 128) >= 1 << 22) return set_error(-1, "gemm_fp8: a sum of nothing over more than 2^22 tiles");
   if (!a->c || (a->K && (!a->a || !a->b || (!raw && !a->a_scale) || !a->b_scale))) return set_error(-1, "gemm_fp8: a needed buffer is missing");
   if (objnerf_gemm_fp8_workspace_floats(a->M, a->N, a->K, a->a_type, a->c_type) && !a->workspace) return set_error(-1, "gemm_fp8: a workspace is needed");
   GemmP p;

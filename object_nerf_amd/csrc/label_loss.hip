@@ -76,7 +76,8 @@ __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES, LANES < 1024 ? 6 : 
   __shared__ __align__(16) int slot_i[kGroups ? kThreads : kMaxSlots];
   __shared__ float slot_e[kGroups ? kThreads : kMaxSlots];
   const int t = kGroups ? threadIdx.x & (LANES - 1) : threadIdx.x;
-  const long at = kGroups ? (long)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES : blockIdx.x;
+  const long at = kGroups ? workgroup() * (kThreads / LANES) + threadIdx.x / LANES : workgroup();
+  if (!kGroups && at >= p.n) return;
   const bool live = !kGroups || at < p.n;
   const long row = live ? at : p.n - 1;
   int* const my_i = slot_i + (kGroups ? threadIdx.x - t : 0);
@@ -252,7 +253,7 @@ int launch_distill(const DistillP& p, hipStream_t s) {
   auto run = [&](auto lanes, auto held) {
     constexpr int L = decltype(lanes)::value, P = decltype(held)::value;
     constexpr int threads = L < 256 ? 256 : L;
-    hipLaunchKernelGGL((distill_kernel<E, L, P>), dim3((unsigned)((p.n + threads / L - 1) / (threads / L))), dim3(threads), 0, s, p);
+    hipLaunchKernelGGL((distill_kernel<E, L, P>), grid_of((p.n + threads / L - 1) / (threads / L)), dim3(threads), 0, s, p);
   };
   using std::integral_constant;
 #define OBJ_ROWS(L, P) run(integral_constant<int, L>{}, integral_constant<int, P>{})

@@ -7,6 +7,15 @@
 
 namespace objnerf {
 
+// A launch holds fewer than 2^32 threads in each dimension: workgroups past 2^20 go into the second one (at most 2^11 of them, for 2^31
+// rows).  The last line of workgroups is not full: a kernel returns, or writes nothing, for a number behind the end.
+constexpr int kGridLine = 20;
+inline dim3 grid_of(long workgroups) {
+  const long lines = ((workgroups - 1) >> kGridLine) + 1;
+  return dim3((unsigned)(lines > 1 ? 1l << kGridLine : workgroups), (unsigned)lines);
+}
+__device__ __forceinline__ long workgroup() { return ((long)blockIdx.y << kGridLine) + blockIdx.x; }
+
 using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
 // rows of 2-byte elements start at any even address: gfx950 takes a 16-byte global access at any element's address
 typedef u32x4 u32x4e __attribute__((aligned(2)));

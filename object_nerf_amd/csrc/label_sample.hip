@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(256) sample_sorted_kernel(SampleP p) {
   fill_table(table);
   __syncthreads();
   const int t = threadIdx.x & (LANES - 1);
-  const long at = (long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  const long at = workgroup() * (256 / LANES) + threadIdx.x / LANES;
   const long r = at < p.n ? at : p.n - 1;
   const char* z = static_cast<const char*>(p.z) + r * p.ldz * E::kBytes;
   const Settings set = settings_of(p, r);
@@ -800,8 +800,9 @@ __device__ void draw_row(const SampleP& p, long r, bool rest, Shared<THREADS>& s
 template <class E, int THREADS>
 __global__ void __launch_bounds__(THREADS, 4) sample_row_kernel(SampleP p, bool rest) {
   __shared__ Shared<THREADS> sh;
-  if (rest && p.out[blockIdx.x] != kOpen) return;                // sample_top_kernel has drawn it
-  draw_row<E, THREADS>(p, blockIdx.x, rest, sh);
+  const long r = workgroup();
+  if (r >= p.n || (rest && p.out[r] != kOpen)) return;           // sample_top_kernel has drawn it
+  draw_row<E, THREADS>(p, r, rest, sh);
 }
 
 // Such rows in a kernel of their own: two light passes and a list, many rows at a time on a CU.  Rows of other settings, and rows with
@@ -815,7 +816,8 @@ __global__ void __launch_bounds__(256, 6) sample_top_kernel(SampleP p) {
     uint64_t red[4];
     unsigned listed, bound;
   } sh;
-  const long r = blockIdx.x;
+  const long r = workgroup();
+  if (r >= p.n) return;
   Settings set = settings_of(p, r);
   if (is_single(set)) set.top_k = 1;
   if (set.top_k < 1 || set.top_k > kPrune) {
@@ -1063,7 +1065,7 @@ template <class E>
 int launch_sample(const SampleP& p, void* workspace, hipStream_t s) {
   auto sorted = [&](auto lanes, auto per) {
     constexpr int L = decltype(lanes)::value, P = decltype(per)::value;
-    hipLaunchKernelGGL((sample_sorted_kernel<E, L, P>), dim3((unsigned)((p.n + 256 / L - 1) / (256 / L))), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((sample_sorted_kernel<E, L, P>), grid_of((p.n + 256 / L - 1) / (256 / L)), dim3(256), 0, s, p);
   };
   using std::integral_constant;
 #define OBJ_SORTED(L, P) sorted(integral_constant<int, L>{}, integral_constant<int, P>{})
@@ -1093,7 +1095,7 @@ int launch_sample(const SampleP& p, void* workspace, hipStream_t s) {
       // a kernel for small top_k pays where rows wait for a place on the card (2048 rows of 32768 bf16, top_k 50: 74 -> 55 us, 768: 35 ->
       // 28); where all are on it at once, a second kernel only follows the first (512: 22 and 22, 257 of 30011: 18 -> 20)
       const bool light = p.n > 512 && (p.t || p.top_k || p.c0 == 0.0 || small_k);
-      const dim3 grid((unsigned)p.n);
+      const dim3 grid = grid_of(p.n);
       if (light) hipLaunchKernelGGL((sample_top_kernel<E>), grid, dim3(256), 0, s, p);
       // 512 threads where all rows are on the card at once (512 x 8192 22.6 us against 24.0 with 256 threads, 200 x 32768 42 / 65, 512 x
       // 131072 196 / 253), 256 where rows wait for places or are short (1024 x 8192 33 / 42, 2048 x 32768 178 / 193, 200 x 2048 11.7 / 13.1)

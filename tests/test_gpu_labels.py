@@ -225,7 +225,7 @@ def test_sample_sizes_types_and_filters(n, v, dtype, kw):
                                 dict(top_p=0.9), dict(temperature=30.0, top_p=0.6)], ids=str)
 @pytest.mark.parametrize("n,v,dtype", [(600, 700, BF16), (520, 5003, F32), (200, 9001, F16), (300, 8200, F32), (129, 8192, BF16)])
 def test_sample_many_rows(n, v, dtype, kw):
-    """more rows than places: the kernel for small top_k and the one for the rest; workgroups of 256, 512 and 1,024 threads"""
+    """more rows than places: the kernel for small top_k and the one for the rest; workgroups of 256 and 512 threads"""
     g = _gen(v)
     z = (torch.randn(n, v, generator=g) * 2.5).to(dtype)
     z[:4] = 0.5                                           # equal logits: the list of candidates overflows
@@ -560,6 +560,63 @@ def test_fp8_offsets_past_32_bits():
         for transpose in (False, True):
             a, b = A.quantize_fp8(far, block_rows, transpose), A.quantize_fp8(near, block_rows, transpose)
             assert torch.equal(a.data.view(torch.uint8), b.data.view(torch.uint8)) and torch.equal(a.scale, b.scale)
+
+
+# ---- more workgroups than a line of a launch's grid holds (2^20) ----
+
+LINE = 1 << 20
+
+
+@pytest.mark.parametrize("v,per,dtype,k", [(9, 16, F32, 3), (2100, 1, BF16, 2)])
+def test_distill_more_rows_than_a_line(v, per, dtype, k):
+    """the rows on both sides of the line's end and the last ones, against the same rows by themselves"""
+    n = LINE * per + 5 * per + 3
+    g = torch.Generator(device=DEV).manual_seed(v)
+    z = torch.empty(n, v, dtype=dtype, device=DEV).normal_(generator=g)
+    t, i = torch.randn(n, k, device=DEV, generator=g), torch.randint(-1, v, (n, k), device=DEV, generator=g, dtype=torch.int32)
+    up = torch.randn(n, device=DEV, generator=g)
+    loss, grad = A.distill_top_logits_grad(z, t, i, up)
+    for at in (slice(0, 40), slice(LINE * per - 40, LINE * per + 40), slice(n - 40, n)):
+        want = A.distill_top_logits_grad(z[at], t[at], i[at], up[at])
+        assert torch.equal(loss[at], want[0]) and torch.equal(grad[at], want[1])
+    assert torch.isfinite(loss).all()
+
+
+@pytest.mark.parametrize("v,per,dtype,kw", [(9, 16, F32, dict(top_p=0.9)), (520, 1, BF16, dict(top_k=20)), (520, 1, BF16, dict(top_p=0.9))])
+def test_sample_more_rows_than_a_line(v, per, dtype, kw):
+    n = LINE * per + 5 * per + 3
+    g = torch.Generator(device=DEV).manual_seed(v)
+    z = torch.empty(n, v, dtype=dtype, device=DEV).normal_(generator=g)
+    u = torch.rand(n, device=DEV, generator=g)
+    label = A.sample_logits(z, u, **kw)
+    for at in (slice(0, 40), slice(LINE * per - 40, LINE * per + 40), slice(n - 40, n)):
+        assert torch.equal(label[at].cpu(), R.sample(z[at].cpu(), u[at].cpu(), kw.get("temperature", 1.0), kw.get("top_k", 0), kw.get("top_p", 1.0), 0.0))
+    assert label.min() >= 0 and label.max() < v
+
+
+def test_quantize_more_blocks_than_a_line():
+    rows = 128 * LINE + 128 * 5 + 3                              # tiles of 128 x 128; 16 blocks of a row to a workgroup
+    x = torch.empty(rows, 1, dtype=BF16, device=DEV).normal_(generator=torch.Generator(device=DEV).manual_seed(1))
+    for block_rows in (1, 128):
+        q = A.quantize_fp8(x, block_rows, transpose=True)
+        for at in (slice(0, 256), slice(128 * LINE - 256, 128 * LINE + 256), slice(128 * LINE + 512, rows)):
+            want = A.quantize_fp8(x[at], block_rows, transpose=True)
+            width = want.data.shape[1]
+            assert torch.equal(q.data.view(torch.uint8)[:, at.start:at.start + width], want.data.view(torch.uint8))
+            assert torch.equal(q.scale[:, at.start // 128:at.start // 128 + width // 128], want.scale[:, :width // 128])
+    del q
+    x = x[:16 * LINE + 85]
+    q = A.quantize_fp8(x)
+    for at in (slice(0, 40), slice(16 * LINE - 40, 16 * LINE + 40), slice(len(x) - 40, len(x))):
+        want = A.quantize_fp8(x[at])
+        assert torch.equal(q.data.view(torch.uint8)[at], want.data.view(torch.uint8)) and torch.equal(q.scale[at], want.scale)
+
+
+def test_column_sums_of_more_columns_than_a_line():
+    cols = 16 * LINE + 85
+    x = torch.empty(2, cols, device=DEV).normal_(generator=torch.Generator(device=DEV).manual_seed(2))
+    total = A.label_ops._quantize(x, 1, True, False, True)[2]
+    assert torch.equal(total, x[0] + x[1])
 
 
 # ---- the operators together: a label head over rays, its training step and its answers ----

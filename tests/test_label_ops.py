@@ -116,6 +116,12 @@ def test_gemm_refuses_at_the_c_abi(bad):
     assert b"gemm_fp8" in l.objnerf_last_error()
 
 
+def test_gemm_refuses_a_sum_of_nothing_over_too_many_tiles():
+    l = _lib.lib()
+    assert l.objnerf_gemm_fp8(C.byref(_gemm_args(M=(1 << 31) - 1, N=1, K=0)), None) < 0
+    assert b"2^22 tiles" in l.objnerf_last_error()
+
+
 def test_fp8_c_abi_takes_nothing_to_do():
     l = _lib.lib()
     assert l.objnerf_fp8_quantize(C.byref(_quantize_args(rows=0)), None) == 0 and l.objnerf_fp8_quantize(None, None) < 0
