@@ -656,7 +656,7 @@ int objnerf_distill_top(const objnerf_distill_args* args, void* stream);
  * those the ones with w >= min_p (0: all); label = the first of the order whose running sum is over u * (sum of the kept).
  * T <= 0 and top_k == 1: the first of the order.  NaN counts as -inf; a row of nothing but -inf: -1.  u outside [0, 1) is taken as
  * the nearer end, NaN as 0.  Every setting is a number, or one per row where its pointer is not NULL (then not checked: a
- * temperature that is not positive draws the first of the order, top_k < 0 counts as 0, NaN in top_p or min_p switches it off). */
+ * temperature that is not positive draws the first of the order, an infinite one weighs all alike, top_k < 0 counts as 0, NaN in top_p or min_p switches it off). */
 typedef struct {
   int64_t n;                 /* rows, < 2^31 */
   int32_t v, type;           /* labels >= 1; OBJNERF_TYPE_* */

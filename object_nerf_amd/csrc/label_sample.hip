@@ -50,7 +50,9 @@ struct Settings {
   int top_k;                              // <= 0: off
   float u;
 };
-__host__ __device__ __forceinline__ double scale_of(double t) { return t > 0.0 ? fmin(1.4426950408889634 / t, 1e300) : 0.0; }
+__host__ __device__ __forceinline__ double scale_of(double t) {    // 0: the first of the order
+  return t > 0.0 ? fmin(fmax(1.4426950408889634 / t, 1e-300), 1e300) : 0.0;
+}
 __host__ __device__ __forceinline__ double reach_of(double min_p) { return min_p > 0.0 ? fmax(-log2(min_p), 0.0) : __builtin_inf(); }
 __device__ __forceinline__ Settings settings_of(const SampleP& p, long r) {
   Settings s;

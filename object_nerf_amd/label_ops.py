@@ -362,6 +362,8 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         if not 0.0 <= temperature < 1e300:
             raise ValueError("temperature must be >= 0 and finite, got %r" % temperature)
     if isinstance(top_k, torch.Tensor):
+        if top_k.dtype == torch.int64:
+            top_k = top_k.clamp(-1, 2 ** 31 - 1)             # (the conversion would drop the upper half)
         keep.append(_column(top_k, "top_k", n, dev, torch.int32))
         a.top_k_rows = keep[-1].data_ptr()
     else:

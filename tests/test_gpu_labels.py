@@ -562,6 +562,25 @@ def test_fp8_offsets_past_32_bits():
             assert torch.equal(a.data.view(torch.uint8), b.data.view(torch.uint8)) and torch.equal(a.scale, b.scale)
 
 
+@pytest.mark.parametrize("n,v", [(40, 64), (8, 900), (3, 70001)])
+def test_sample_infinite_temperatures_and_wide_top_k_per_row(n, v):
+    g = _gen(21)
+    z, u = torch.randn(n, v, generator=g), torch.rand(n, generator=g)
+    z[0, ::2] = -math.inf
+    z[1] = -math.inf
+    hot = torch.full((n,), math.inf)
+    order = z.sort(dim=1, descending=True, stable=True)[1]
+    for k in (0, 7):
+        label = A.sample_logits(z.to(DEV), u.to(DEV), temperature=hot.to(DEV), top_k=k).cpu()
+        for r in range(n):                                      # equal weights: the place is u times the number of labels
+            some = int((z[r] > -math.inf).sum())
+            some = min(some, k) if k else some
+            assert label[r] == (order[r, min(int(u[r].double() * some), some - 1)] if some else -1)
+    wide = torch.tensor([2 ** 32 + 3, -2 ** 32 + 1, 2 ** 31, 5] * n)[:n]
+    label = A.sample_logits(z.to(DEV), u.to(DEV), top_k=wide.to(DEV))
+    assert torch.equal(label.cpu(), R.sample(z, u, 1.0, torch.where((wide < 0) | (wide > v), 0, wide), 1.0, 0.0))
+
+
 # ---- more workgroups than a line of a launch's grid holds (2^20) ----
 
 LINE = 1 << 20
