@@ -25,6 +25,7 @@ __all__ = ["Fp8Matrix", "quantize_fp8", "matmul_fp8", "linear_fp8", "distill_top
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # OBJNERF_TYPE_*
 MAX_SLOTS = 1024
+MAX_SUM = 1 << 26                      # terms of a product's sums
 
 
 def _rows(t, name, types=_TYPES):
@@ -108,6 +109,8 @@ def _product(a, b, bias, leaky, out_dtype):
     """(M, N) of an Fp8Matrix, or a matrix that the product rounds on its way, and an Fp8Matrix over the same columns"""
     raw = not isinstance(a, Fp8Matrix)
     data = a if raw else a.data
+    if b.cols > MAX_SUM:
+        raise ValueError("a product over more than 2^26 columns is not supported, got %d" % b.cols)
     m, n, k, dev = data.shape[0], b.data.shape[0], b.data.shape[1], data.device
     out = torch.empty(m, n, dtype=out_dtype, device=dev)
     if not (m and n):
@@ -226,10 +229,10 @@ def linear_fp8(x, weight, bias=None, out_dtype=None):
     """x @ weight.T + bias, both factors rounded to 8-bit floating point with a scale for each block of 128 (x: 128 columns of a row,
     weight: 128 x 128), (M, N) in out_dtype (default: x's type).
 
-    x (M, K); weight (N, K), a tensor -- rounded in every call, so that what an optimizer wrote is what counts -- or the Fp8Matrix that
+    x (M, K); weight (N, K), K <= 2^26, a tensor -- rounded in every call, so that what an optimizer wrote is what counts -- or the Fp8Matrix that
     quantize_fp8(weight, block_rows=128) laid out once, for inference; bias (N,).  Sizes need not be multiples of anything.  With a tensor
     as weight it is differentiable: dX and dW are products of the same kind, of the gradient rounded along their own sums, in x's and
-    weight's types; the bias gradient is an fp32 sum."""
+    weight's types (of at most 2^26 rows of x, of weight); the bias gradient is an fp32 sum."""
     x = _rows(x, "x")
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if out_dtype not in _TYPES:
@@ -248,6 +251,8 @@ def linear_fp8(x, weight, bias=None, out_dtype=None):
     if bias is not None:
         _checked_bias(bias, weight.shape[0], x.device)
     if recording and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        if (weight.requires_grad and x.shape[0] > MAX_SUM) or (x.requires_grad and weight.shape[0] > MAX_SUM):
+            raise ValueError("a gradient that sums over more than 2^26 rows is not supported: x %s, weight %s" % (tuple(x.shape), tuple(weight.shape)))
         return _LinearFp8Fn.apply(x, weight, bias, out_dtype)
     return _rounded_product(x, _quantize(weight, BLOCK)[0], _checked_bias(bias, weight.shape[0], x.device), out_dtype)
 

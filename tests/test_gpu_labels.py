@@ -581,6 +581,18 @@ def test_sample_infinite_temperatures_and_wide_top_k_per_row(n, v):
     assert torch.equal(label.cpu(), R.sample(z, u, 1.0, torch.where((wide < 0) | (wide > v), 0, wide), 1.0, 0.0))
 
 
+def test_linear_fp8_refuses_sums_that_are_too_long():
+    top = A.label_ops.MAX_SUM
+    x, w = torch.zeros(top + 1, 1, dtype=BF16, device=DEV), torch.zeros(2, 1, dtype=BF16, device=DEV)
+    with pytest.raises(ValueError, match="2\\^26 rows"):
+        A.linear_fp8(x, w.requires_grad_())
+    with pytest.raises(ValueError, match="2\\^26 rows"):
+        A.linear_fp8(w.detach().requires_grad_(), x)
+    wide = x.view(1, -1)
+    with pytest.raises(ValueError, match="2\\^26 columns"):
+        A.linear_fp8(wide, wide)
+
+
 # ---- more workgroups than a line of a launch's grid holds (2^20) ----
 
 LINE = 1 << 20
