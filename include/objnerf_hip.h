@@ -659,7 +659,7 @@ int objnerf_distill_top(const objnerf_distill_args* args, void* stream);
  * temperature that is not positive draws the first of the order, an infinite one weighs all alike, top_k < 0 counts as 0, NaN in top_p or min_p switches it off). */
 typedef struct {
   int64_t n;                 /* rows, < 2^31 */
-  int32_t v, type;           /* labels >= 1; OBJNERF_TYPE_* */
+  int32_t v, type;           /* labels, 1 <= v <= 2^19 (sums of a longer row would lack what 24 bits of u resolve); OBJNERF_TYPE_* */
   const void* logits; int64_t logits_stride;
   const float* u; int64_t u_stride;
   const float* temperature_rows; double temperature;

@@ -8,8 +8,10 @@
 //
 // A label's place is its 64-bit key: the logit's bits, ordered as integers, over the index's complement, so that keys are all different
 // and equal logits go by the index.  Weights are held as integers, round(w 2^shift) with shift + log2 v <= 62: integer sums are exact
-// and need no order, so sums formed by atomics give the same bits in every run.  An absolute error of 2^-shift per weight (2^-45 at
-// 131,072 labels, 2^-51 below 2,049) moves a border by far less than a random number of 24 bits can resolve.
+// and need no order, so sums formed by atomics give the same bits in every run.  A weight is off by half of 2^-shift at most, and weights
+// under that become 0, so the sum over a row of a strong label and a flat weak rest can lack v 2^-(shift + 1), about v^2 2^-63 of the
+// largest weight: 2^-29 at 131,072 labels, 2^-25 at 2^19.  That is half of what a random number of 24 bits resolves, and kMaxLabels: at
+// 2^22 labels it would be 2^-19, at 2^30 an eighth of the weight.
 //
 // Rows of up to 512 labels are sorted in the registers of 16 or 64 lanes, and every question -- which are the top_k, where does the
 // running sum pass top_p, where u -- is then a prefix sum away.  Longer rows are not sorted: with a small top_k the candidates are
@@ -29,6 +31,7 @@ namespace objnerf {
 namespace {
 
 constexpr int kList = 512, kPrune = 128;
+constexpr int kMaxLabels = 1 << 19;       // of a row: see the error of the sums above
 constexpr int64_t kOpen = -2;             // between two kernels of a call: this row is still to be drawn
 
 struct SampleP {
@@ -1115,13 +1118,13 @@ int launch_sample(const SampleP& p, void* workspace, hipStream_t s) {
 using namespace objnerf;
 
 extern "C" int64_t objnerf_sample_logits_workspace_bytes(int64_t n, int32_t v, int type) {
-  if (n <= 0 || v <= 512 || !label_type_ok(type)) return 0;
+  if (n <= 0 || v <= 512 || v > kMaxLabels || !label_type_ok(type)) return 0;
   return split_bytes(n, split_plan(n, v, 16 / label_type_bytes(type), false));
 }
 
 extern "C" int objnerf_sample_logits(const objnerf_sample_args* a, void* stream) {
   if (!a) return set_error(-1, "sample_logits: no arguments");
-  if (a->n < 0 || a->n > INT32_MAX || a->v < 1) return set_error(-1, "sample_logits: bad sizes (n < 2^31, v >= 1)");
+  if (a->n < 0 || a->n > INT32_MAX || a->v < 1 || a->v > kMaxLabels) return set_error(-1, "sample_logits: bad sizes (n < 2^31, 1 <= v <= 2^19)");
   if (!label_type_ok(a->type)) return set_error(-1, "sample_logits: unknown element type");
   if (a->logits_stride < 0 || a->u_stride < 0) return set_error(-1, "sample_logits: bad strides");
   if (!a->temperature_rows && !(a->temperature >= 0.0 && a->temperature < 1e300)) return set_error(-1, "sample_logits: the temperature must be >= 0 and finite");

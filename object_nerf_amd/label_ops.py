@@ -26,6 +26,7 @@ __all__ = ["Fp8Matrix", "quantize_fp8", "matmul_fp8", "linear_fp8", "distill_top
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # OBJNERF_TYPE_*
 MAX_SLOTS = 1024
 MAX_SUM = 1 << 26                      # terms of a product's sums
+MAX_LABELS = 1 << 19                   # of a row that a label is drawn from
 
 
 def _rows(t, name, types=_TYPES):
@@ -338,7 +339,7 @@ def distill_top_logits_grad(student, teacher, index, upstream, temperature=1.0):
 # ---- drawing a label ----
 
 def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
-    """One label per row, (N,) int64, drawn at the random numbers u (N,) in [0, 1).
+    """One label per row, (N,) int64, drawn from logits (N, V), V <= 2^19, at the random numbers u (N,) in [0, 1).
 
     Weights are exp(logits / temperature) (up to a factor).  The labels in order -- falling logits, equal ones by rising index -- are
     cut to the first `top_k` (0: all), of those to the shortest prefix whose share of their weight reaches `top_p` (1: all; at
@@ -350,8 +351,8 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     logits = _rows(logits, "logits")
     n, v = logits.shape
     dev = logits.device
-    if v < 1:
-        raise ValueError("sample_logits needs at least one label")
+    if not 1 <= v <= MAX_LABELS:
+        raise ValueError("sample_logits takes rows of 1 to 2^19 labels, got %d" % v)
     if not isinstance(u, torch.Tensor):
         raise TypeError("u must be a tensor, got %s" % type(u).__name__)
     u = _column(u, "u", n, dev)

@@ -1,0 +1,42 @@
+"""GPU: the label operators at the ends of what they take."""
+import math
+
+import pytest
+import torch
+
+import label_reference as R
+import object_nerf_amd as A
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ---- drawing a label ----
+
+@pytest.mark.parametrize("weak", [-14.0, -20.0, -28.0, -30.0])
+def test_sample_one_strong_label_over_the_flattest_and_longest_tail(weak):
+    """Weights are whole numbers of 2^-43 at 2^19 labels: each is off by 2^-44 at most, a sum of them by 2^-25 of the strong one.  u times the
+    total lies between the running sums in front of and behind the label, off by that twice."""
+    v, strong = 1 << 19, 12345
+    z = torch.full((1, v), weak, device=DEV)
+    z[0, strong] = 0.0
+    u = torch.tensor([0.0, 0.5, 1 - 2.0 ** -6, 1 - 2.0 ** -12, 1 - 2.0 ** -18, 1 - 2.0 ** -22, 1 - 2.0 ** -24])
+    w = math.exp(weak)
+    total = 1 + (v - 1) * w
+    for rows in (1, len(u)):                                    # a row over several workgroups; rows at a time
+        for at in range(0, len(u), rows):
+            labels = A.sample_logits(z.expand(rows, v), u[at:at + rows].to(DEV)).tolist()
+            for label, x in zip(labels, u[at:at + rows].tolist()):
+                rank = 0 if label == strong else label + (label < strong)
+                front, behind = (0.0, 1.0) if rank == 0 else (1 + (rank - 1) * w, 1 + rank * w)
+                assert front - 2.0 ** -24 <= x * total <= behind + 2.0 ** -24, (x, label)
+
+
+def test_sample_refuses_longer_rows():
+    with pytest.raises(ValueError, match="2\\^19"):
+        A.sample_logits(torch.zeros(1, (1 << 19) + 1, device=DEV), torch.zeros(1, device=DEV))
