@@ -11,13 +11,16 @@
 Rows are (N, V) on the GPU in float32, bfloat16 or float16 with any row stride; a last dimension that is not contiguous is copied.
 Python here checks arguments, allocates results and enqueues on the current stream of the tensors' device; nothing synchronises, and
 a call can be captured in a graph.  Arguments of a wrong type raise TypeError, of a wrong value or shape ValueError, CPU tensors and
-failing launches RuntimeError.
+failing launches RuntimeError.  Differentiable is meant of backward passes, once: a tensor with a forward-mode tangent raises
+NotImplementedError.  What records torch operations to run them again without Python (torch.jit.trace, make_fx) sees none of the
+kernels and is refused with a RuntimeError.
 """
 import ctypes as C
 import operator
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -29,8 +32,23 @@ MAX_SUM = 1 << 26                      # terms of a product's sums
 MAX_LABELS = 1 << 19                   # of a row that a label is drawn from
 
 
+def _refuse_recording():
+    """a recorded program would hold the allocation of the results and no kernel"""
+    if torch._C._get_tracing_state() is not None or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise RuntimeError("the label operators cannot be recorded by torch.jit.trace or make_fx: the kernels would be missing")
+
+
+def _refuse_tangents(*tensors):
+    """forward-mode derivatives go past `requires_grad`: the result would come without one"""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("the label operators have no forward-mode derivative")
+
+
 def _rows(t, name, types=_TYPES):
     """t as a 2-D GPU tensor whose rows are contiguous"""
+    _refuse_recording()
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s must be a tensor, got %s" % (name, type(t).__name__))
     if t.dim() != 2:
@@ -139,6 +157,7 @@ def _rounded_product(x, w, bias, out_dtype):
 
 
 def _checked_fp8(x, name):
+    _refuse_recording()
     if not isinstance(x, Fp8Matrix):
         raise TypeError("%s must be an Fp8Matrix (quantize_fp8), got %s" % (name, type(x).__name__))
     d, s = x.data, x.scale
@@ -188,6 +207,7 @@ def matmul_fp8(a, b, bias=None, activation=None, out_dtype=torch.bfloat16):
         raise ValueError("activation must be None or 'leaky_relu', got %r" % (activation,))
     if out_dtype not in _TYPES:
         raise TypeError("out_dtype: %s is not supported" % (out_dtype,))
+    _refuse_tangents(bias)
     if bias is not None and isinstance(bias, torch.Tensor) and bias.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("matmul_fp8 is inference-only: use linear_fp8 where a gradient is needed")
     return _product(a, b, _checked_bias(bias, b.data.shape[0], a.data.device), activation is not None, out_dtype)
@@ -210,6 +230,7 @@ class _LinearFp8Fn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _refuse_tangents(dy)
         need_x, need_w, need_b, _ = ctx.needs_input_grad
         xt, sxt, wt, swt = ctx.saved_tensors
         m, n, k = ctx.sizes
@@ -235,6 +256,7 @@ def linear_fp8(x, weight, bias=None, out_dtype=None):
     as weight it is differentiable: dX and dW are products of the same kind, of the gradient rounded along their own sums, in x's and
     weight's types (of at most 2^26 rows of x, of weight); the bias gradient is an fp32 sum."""
     x = _rows(x, "x")
+    _refuse_tangents(x, weight, bias)
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if out_dtype not in _TYPES:
         raise TypeError("out_dtype: %s is not supported" % (out_dtype,))
@@ -308,6 +330,7 @@ class _DistillFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_loss):
+        _refuse_tangents(d_loss)
         a, keep = _distill_args(*ctx.saved_tensors, ctx.temperature)
         return _run_distill(a, keep, False, d_loss if d_loss.dtype == torch.float32 else d_loss.float())[1], None, None, None
 
@@ -321,6 +344,7 @@ def distill_top_logits(student, teacher, index, temperature=1.0):
     has loss 0 and gradient 0; otherwise NaN in the row gives a loss of NaN, a label ruled out by the student (-inf) under a filled slot a loss
     of +inf.  An index may occur more than once (its shares add).  Differentiable with respect to `student`
     alone; the usual factor T^2 is the caller's.  The backward pass reads the student's row again instead of keeping a copy."""
+    _refuse_tangents(student, teacher)
     if torch.is_grad_enabled() and isinstance(student, torch.Tensor) and student.requires_grad:
         return _DistillFn.apply(student, teacher, index, temperature)
     return _run_distill(*_distill_args(student, teacher, index, temperature), True, None)[0]
@@ -332,6 +356,7 @@ def distill_top_logits_grad(student, teacher, index, upstream, temperature=1.0):
     (`logits.backward(grad)` goes on from there)."""
     if not isinstance(upstream, torch.Tensor):
         raise TypeError("upstream must be a tensor, got %s" % type(upstream).__name__)
+    _refuse_tangents(student, teacher, upstream)
     a, keep = _distill_args(student, teacher, index, temperature)
     return _run_distill(a, keep, True, _column(upstream.detach(), "upstream", a.n, keep[0].device))
 

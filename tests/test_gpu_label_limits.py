@@ -40,3 +40,22 @@ def test_sample_one_strong_label_over_the_flattest_and_longest_tail(weak):
 def test_sample_refuses_longer_rows():
     with pytest.raises(ValueError, match="2\\^19"):
         A.sample_logits(torch.zeros(1, (1 << 19) + 1, device=DEV), torch.zeros(1, device=DEV))
+
+
+# ---- derivatives ----
+
+def test_forward_mode_over_backward_is_refused():
+    fw = torch.autograd.forward_ad
+    x, w = torch.randn(4, 6, device=DEV, requires_grad=True), torch.randn(5, 6, device=DEV)
+    z, t, i = torch.randn(4, 6, device=DEV, requires_grad=True), torch.randn(4, 2, device=DEV), torch.zeros(4, 2, dtype=torch.int64, device=DEV)
+    y, loss = A.linear_fp8(x, w), A.distill_top_logits(z, t, i)
+    with fw.dual_level():
+        for out, leaf in ((y, x), (loss, z)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(out, leaf, fw.make_dual(torch.ones_like(out), torch.ones_like(out)), retain_graph=True)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            q = A.quantize_fp8(w)
+            A.matmul_fp8(q, q, fw.make_dual(torch.ones(5, device=DEV), torch.ones(5, device=DEV)))
+        label = A.sample_logits(fw.make_dual(z.detach(), torch.ones_like(z)), torch.rand(4, device=DEV))      # whole numbers have no derivative
+        assert label.shape == (4,)
+    assert torch.autograd.grad(y.sum(), x)[0].shape == x.shape

@@ -21,3 +21,30 @@ def test_sample_refuses_rows_that_its_sums_cannot_hold():
         assert _sample(v=v, logits_stride=v) < 0 and b"2^19" in l.objnerf_last_error()
         assert l.objnerf_sample_logits_workspace_bytes(1, v, 1) == 0
     assert _sample(n=0, v=1 << 19) == 0
+
+
+CALLS = [lambda z, w: A.linear_fp8(z, w), lambda z, w: A.linear_fp8(w, z), lambda z, w: A.linear_fp8(w, w, z[:, 0]), lambda z, w: A.distill_top_logits(z, w, w.long()),
+         lambda z, w: A.distill_top_logits(w, z, w.long()), lambda z, w: A.distill_top_logits_grad(z, w, w.long(), w[:, 0]),
+         lambda z, w: A.distill_top_logits_grad(w, w, w.long(), z[:, 0])]
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_forward_mode_tangents_are_refused(call, monkeypatch):
+    monkeypatch.setattr(_lib, "require_cuda", lambda *a: None)                  # the checks alone, on the CPU
+    z, w = torch.randn(3, 5), torch.randn(3, 5)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(torch.autograd.forward_ad.make_dual(z, torch.ones_like(z)), w)
+
+
+@pytest.mark.parametrize("call", [CALLS[0], CALLS[3], CALLS[5], lambda z, w: A.sample_logits(z, w[:, 0]), lambda z, w: A.quantize_fp8(z).data])
+def test_recorders_are_refused(call):
+    """what they record is the allocation of the results: the replayed program would return memory that nothing has written"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    z, w = torch.randn(3, 5), torch.randn(3, 5)
+    with pytest.raises(RuntimeError, match="recorded"):
+        torch.jit.trace(call, (z, w), check_trace=False)
+    with pytest.raises(RuntimeError, match="recorded"):
+        make_fx(call)(z, w)
+    with pytest.raises(RuntimeError, match="GPU"):
+        call(z, w)
