@@ -29,6 +29,7 @@ __all__ = ["Fp8Matrix", "quantize_fp8", "matmul_fp8", "linear_fp8", "distill_top
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # OBJNERF_TYPE_*
 MAX_SLOTS = 1024
 MAX_SUM = 1 << 26                      # terms of a product's sums
+MAX_INT = (1 << 31) - 1                # rows, and labels of the distillation
 MAX_LABELS = 1 << 19                   # of a row that a label is drawn from
 
 
@@ -299,6 +300,8 @@ def _distill_args(student, teacher, index, temperature):
     temperature = float(temperature)
     if not 1e-30 <= temperature <= 1e30:
         raise ValueError("temperature must be positive and finite, got %r" % temperature)
+    if n > MAX_INT or v > MAX_INT:
+        raise ValueError("student must have fewer than 2^31 rows and labels, got %s" % (tuple(student.shape),))
     a = _lib.DistillArgs(n, v, k, student.data_ptr(), student.stride(0), _TYPES[student.dtype], _TYPES[teacher.dtype], teacher.data_ptr(), teacher.stride(0),
                          index.data_ptr(), index.stride(0), index.element_size(), 0, temperature)
     return a, (student, teacher, index)       # the tensors whose memory the arguments point to: kept until the call is enqueued
@@ -376,8 +379,8 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     logits = _rows(logits, "logits")
     n, v = logits.shape
     dev = logits.device
-    if not 1 <= v <= MAX_LABELS:
-        raise ValueError("sample_logits takes rows of 1 to 2^19 labels, got %d" % v)
+    if not 1 <= v <= MAX_LABELS or n > MAX_INT:
+        raise ValueError("sample_logits takes fewer than 2^31 rows of 1 to 2^19 labels, got %s" % (tuple(logits.shape),))
     if not isinstance(u, torch.Tensor):
         raise TypeError("u must be a tensor, got %s" % type(u).__name__)
     u = _column(u, "u", n, dev)

@@ -42,6 +42,18 @@ def test_sample_refuses_longer_rows():
         A.sample_logits(torch.zeros(1, (1 << 19) + 1, device=DEV), torch.zeros(1, device=DEV))
 
 
+# ---- distillation ----
+
+def test_distill_refuses_more_labels_than_its_sizes_hold():
+    """2^32 + 5 labels would be 5 in 32 bits"""
+    one = torch.zeros(1, 1, device=DEV)
+    z = torch.empty(1, (1 << 32) + 5, dtype=BF16, device=DEV)                   # refused before anything reads it
+    for call in (lambda: A.distill_top_logits(z, one, one.long()), lambda: A.distill_top_logits_grad(z, one, one.long(), one[0]),
+                 lambda: A.distill_top_logits(z.requires_grad_(), one, one.long())):
+        with pytest.raises(ValueError, match="2\\^31"):
+            call()
+
+
 # ---- derivatives ----
 
 def test_forward_mode_over_backward_is_refused():
