@@ -309,15 +309,16 @@ def _distill_args(student, teacher, index, temperature):
 
 def _run_distill(a, keep, want_loss, upstream):
     student = keep[0]
+    n, v = student.shape                      # (not a.n, a.v: torch.compile takes a structure's fields for their descriptors)
     loss = grad = None
     if want_loss:
-        loss = torch.empty(a.n, dtype=torch.float32, device=student.device)
+        loss = torch.empty(n, dtype=torch.float32, device=student.device)
         a.loss = loss.data_ptr()
     if upstream is not None:
-        grad = torch.empty(a.n, a.v, dtype=student.dtype, device=student.device)
+        grad = torch.empty(n, v, dtype=student.dtype, device=student.device)
         a.upstream, a.upstream_stride = upstream.data_ptr(), (upstream.stride(0) if upstream.dim() else 0)
-        a.grad, a.grad_stride = grad.data_ptr(), a.v
-    if a.n:
+        a.grad, a.grad_stride = grad.data_ptr(), v
+    if n:
         _call(_lib.lib().objnerf_distill_top, a, student.device, "distill_top")
     return loss, grad
 
@@ -361,7 +362,7 @@ def distill_top_logits_grad(student, teacher, index, upstream, temperature=1.0):
         raise TypeError("upstream must be a tensor, got %s" % type(upstream).__name__)
     _refuse_tangents(student, teacher, upstream)
     a, keep = _distill_args(student, teacher, index, temperature)
-    return _run_distill(a, keep, True, _column(upstream.detach(), "upstream", a.n, keep[0].device))
+    return _run_distill(a, keep, True, _column(upstream.detach(), "upstream", keep[0].shape[0], keep[0].device))
 
 
 # ---- drawing a label ----

@@ -71,3 +71,23 @@ def test_forward_mode_over_backward_is_refused():
         label = A.sample_logits(fw.make_dual(z.detach(), torch.ones_like(z)), torch.rand(4, device=DEV))      # whole numbers have no derivative
         assert label.shape == (4,)
     assert torch.autograd.grad(y.sum(), x)[0].shape == x.shape
+
+
+# ---- torch.compile: the calls stay as they are, between compiled parts ----
+
+def test_calls_inside_a_compiled_function():
+    g = _gen(3)
+    x, w, b = (torch.randn(*s, generator=g).to(DEV).requires_grad_() for s in ((7, 40), (12, 40), (12,)))
+    t, i, u = torch.randn(7, 3, generator=g).to(DEV), torch.randint(-1, 12, (7, 3), generator=g).to(DEV), torch.rand(7, generator=g).to(DEV)
+
+    def step(x, w, b):
+        y = A.linear_fp8(x * 2, w, b)
+        loss = A.distill_top_logits(y, t, i)
+        both = A.distill_top_logits_grad(y.detach(), t, i, u)
+        label = A.sample_logits(y.detach(), u, top_k=3)
+        return (loss * 2).sum(), both[0] + 1, both[1] * 2, label + 1
+
+    got, want = torch.compile(step, backend="eager")(x, w, b), step(x, w, b)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    for p, q in zip(torch.autograd.grad(got[0], (x, w, b)), torch.autograd.grad(want[0], (x, w, b))):
+        assert torch.equal(p, q)
