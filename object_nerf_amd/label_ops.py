@@ -58,6 +58,8 @@ def _rows(t, name, types=_TYPES):
         raise TypeError("%s: dtype %s is not supported" % (name, t.dtype))
     if not t.is_cuda:
         _lib.require_cuda(t, name)
+    if t.is_neg():                                    # a view that stands for minus its memory (the imaginary part of a conjugate)
+        t = t.resolve_neg()
     return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 
@@ -69,7 +71,7 @@ def _column(t, name, n, device, dtype=torch.float32):
         raise ValueError("%s must be on %s, got %s" % (name, device, t.device))
     if t.is_floating_point() != dtype.is_floating_point or t.dtype == torch.bool or t.is_complex():
         raise TypeError("%s: dtype %s is not supported" % (name, t.dtype))
-    return (t if t.dtype == dtype else t.to(dtype)).contiguous()
+    return (t if t.dtype == dtype else t.to(dtype)).resolve_neg().contiguous()
 
 
 def _call(fn, args, device, what):
@@ -336,7 +338,7 @@ class _DistillFn(torch.autograd.Function):
     def backward(ctx, d_loss):
         _refuse_tangents(d_loss)
         a, keep = _distill_args(*ctx.saved_tensors, ctx.temperature)
-        return _run_distill(a, keep, False, d_loss if d_loss.dtype == torch.float32 else d_loss.float())[1], None, None, None
+        return _run_distill(a, keep, False, d_loss.float().resolve_neg())[1], None, None, None
 
 
 def distill_top_logits(student, teacher, index, temperature=1.0):

@@ -42,6 +42,28 @@ def test_sample_refuses_longer_rows():
         A.sample_logits(torch.zeros(1, (1 << 19) + 1, device=DEV), torch.zeros(1, device=DEV))
 
 
+# ---- views that stand for minus their memory ----
+
+@pytest.mark.parametrize("v", [1, 40])
+def test_negated_views(v):
+    g = _gen(v)
+    c = torch.complex(torch.randn(6, v, generator=g), torch.randn(6, v, generator=g)).to(DEV)
+    u, t, i = torch.rand(6, generator=g).to(DEV), torch.randn(6, 2, generator=g).to(DEV), torch.randint(0, v, (6, 2), generator=g).to(DEV)
+    for view in (c.conj().imag, torch._neg_view(c.real.contiguous())):
+        assert view.is_neg()
+        plain = view.resolve_neg().contiguous()
+        assert torch.equal(A.sample_logits(view, u), A.sample_logits(plain, u))
+        assert torch.equal(A.linear_fp8(view, view, view[:, 0]), A.linear_fp8(plain, plain, plain[:, 0]))
+        assert torch.equal(A.quantize_fp8(view).data.view(torch.uint8), A.quantize_fp8(plain).data.view(torch.uint8))
+        for got, want in zip(A.distill_top_logits_grad(view, t, i, view[:, 0]), A.distill_top_logits_grad(plain, t, i, plain[:, 0])):
+            assert torch.equal(got, want)
+        assert torch.equal(A.distill_top_logits(plain, torch._neg_view(t), i), A.distill_top_logits(plain, -t, i))
+        leaf = plain.requires_grad_()
+        for out in (A.distill_top_logits(leaf, t, i), A.linear_fp8(leaf, leaf.detach())):
+            d = torch.randn(out.shape, generator=g).to(DEV)
+            assert torch.equal(*(torch.autograd.grad(out, leaf, x, retain_graph=True)[0] for x in (torch._neg_view(d), -d)))
+
+
 # ---- distillation ----
 
 def test_distill_refuses_more_labels_than_its_sizes_hold():
