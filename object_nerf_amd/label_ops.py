@@ -378,7 +378,7 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     first, in that order, whose running sum of weight exceeds u times their total.  temperature 0 and top_k 1 give the first
     of the order.  NaN counts as -inf; a row of nothing but -inf gives -1.
 
-    Each setting is a number or an (N,) tensor on the logits' device, one value per row.  Runs give equal labels for equal inputs."""
+    Each setting is a number or an (N,) tensor on the logits' device, one value per row, held as float32 (top_k: int32), as u is.  Runs give equal labels for equal inputs."""
     logits = _rows(logits, "logits")
     n, v = logits.shape
     dev = logits.device
@@ -399,8 +399,8 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         if not 0.0 <= temperature < 1e300:
             raise ValueError("temperature must be >= 0 and finite, got %r" % temperature)
     if isinstance(top_k, torch.Tensor):
-        if top_k.dtype == torch.int64:
-            top_k = top_k.clamp(-1, 2 ** 31 - 1)             # (the conversion would drop the upper half)
+        if top_k.dtype in (torch.int64, torch.uint64):       # (the conversion would drop the upper half; 2^63 and more count as -1: all)
+            top_k = top_k.to(torch.int64).clamp(-1, 2 ** 31 - 1)
         keep.append(_column(top_k, "top_k", n, dev, torch.int32))
         a.top_k_rows = keep[-1].data_ptr()
     else:

@@ -42,6 +42,17 @@ def test_sample_refuses_longer_rows():
         A.sample_logits(torch.zeros(1, (1 << 19) + 1, device=DEV), torch.zeros(1, device=DEV))
 
 
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int16, torch.uint16, torch.uint32, torch.int64, torch.uint64])
+def test_sample_top_k_per_row_of_any_whole_type(dtype):
+    n, v = 12, 700
+    g = _gen(8)
+    z, u = torch.randn(n, v, generator=g), torch.rand(n, generator=g)
+    most = torch.iinfo(dtype).max
+    k = [0, 1, 5, 100, min(most, 650), most, most // 2 + 1, min(most, 1 << 31), min(most, (1 << 32) - 1), min(most, (1 << 32) + 3), min(most, 1 << 62), 7]
+    label = A.sample_logits(z.to(DEV), u.to(DEV), top_k=torch.tensor(k, dtype=dtype).to(DEV))
+    assert torch.equal(label.cpu(), R.sample(z, u, 1.0, torch.tensor([min(x, v) for x in k]), 1.0, 0.0))
+
+
 # ---- views that stand for minus their memory ----
 
 @pytest.mark.parametrize("v", [1, 40])
