@@ -87,6 +87,39 @@ def test_distill_refuses_more_labels_than_its_sizes_hold():
             call()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("v,k", [(40, 4), (40, 30), (900, 4), (5000, 70), (70001, 4)])
+def test_distill_lowest_values_under_slots(v, k, dtype):
+    """Masked labels under filled slots: the terms, up to 2^129, are brought back by their weights, their mean or T.  Relative error of a
+    loss: exp at distances up to 80 with three roundings of the argument, the term and the sums of k of them; all terms have one sign,
+    next to which the logarithms are nothing."""
+    low = torch.finfo(dtype).min
+    z, t, i = torch.zeros(7, v), torch.full((7, k), -math.inf), torch.arange(k).expand(7, k).clone()
+    t[:, :4] = torch.tensor([0.5, 0.25, 0.0, -1.0])
+    z[0, 0] = low                                         # one of four
+    z[1, :4] = low                                        # every slot: the terms' sum is over fp32's end
+    z[2, 0], t[2, 0] = low, -70.0                         # next to no weight
+    z[3, 3], t[3, 3] = low, -30.0
+    z[4], t[4, 1:] = low, -math.inf                       # the whole row masked: alike
+    z[5, 2], z[5, 7] = low, -low                          # the whole range of the type
+    z[6, 1], t[6, 1], i[6, 2] = low, -20.0, 1             # an index twice
+    u = torch.full((7,), 0.125)
+    z = z.to(dtype)
+    for temperature in (0.25, 0.5, 1.0, 3.0):
+        loss, grad = A.distill_top_logits_grad(z.to(DEV), t.to(DEV), i.to(DEV), u.to(DEV), temperature=temperature)
+        # (rows less their largest: 64 bits would lose log v next to 1e39, and a softmax does not see the shift)
+        rl, rg, _ = R.distill(z.double() - z.double().amax(1, keepdim=True), t, i, u, temperature)
+        held = rl.abs() < torch.finfo(F32).max * (1 - 2.0 ** -12)               # else: an infinity, or next to one
+        assert held[2:5].all() and torch.equal(torch.isinf(loss.cpu())[held], torch.zeros(int(held.sum()), dtype=torch.bool))
+        assert (loss.cpu()[~held] >= torch.finfo(F32).max * (1 - 2.0 ** -11)).all()
+        d = 80 / min(temperature, 1.0)
+        bound = (3 * d + k + 20) * R.STEP[F32] * rl.abs() + (80 + v / 256 + k) * R.STEP[F32] * (1 + math.log(v))
+        assert ((loss.cpu().double() - rl).abs()[held] <= bound[held]).all(), ((loss.cpu().double() - rl) / bound)
+        assert torch.equal(A.distill_top_logits(z.to(DEV), t.to(DEV), i.to(DEV), temperature=temperature), loss)
+        size = (3 * d + v / 256 + k + 20) * R.STEP[F32] * 0.25 / temperature
+        assert ((grad.cpu().double() - rg).abs() <= R.STEP[dtype] * rg.abs() + size + (2.0 ** -24 if dtype == F16 else 0)).all()
+
+
 # ---- derivatives ----
 
 def test_forward_mode_over_backward_is_refused():
