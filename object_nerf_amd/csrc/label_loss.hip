@@ -50,10 +50,10 @@ __device__ __forceinline__ int slot_column(const DistillP& p, long row, int j) {
   return i >= 0 && i < p.v ? (int)i : -1;
 }
 
-// exp(a_j) (a_j - b_j) / 2^12 of a slot with weight e
+// exp(a_j) (a_j - b_j) / 2^12 of a slot with weight e.  What the student rules out costs +inf whatever weight is left in fp32.
 constexpr float kTermScale = 0x1p-12f;
 __device__ __forceinline__ float slot_term(const DistillP& p, float e, float t, float tm, float z, float m) {
-  if (e == 0.f) return 0.f;
+  if (z == -__builtin_inff()) return __builtin_inff();
   const float d = (t * kTermScale - tm * kTermScale) - (z * kTermScale - m * kTermScale);
   return p.inv_t <= 1.f ? e * (d * p.inv_t) : e * p.inv_t * d;
 }

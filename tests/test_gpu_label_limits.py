@@ -120,6 +120,17 @@ def test_distill_lowest_values_under_slots(v, k, dtype):
         assert ((grad.cpu().double() - rg).abs() <= R.STEP[dtype] * rg.abs() + size + (2.0 ** -24 if dtype == F16 else 0)).all()
 
 
+@pytest.mark.parametrize("v,k", [(40, 2), (3000, 70), (70001, 2)])
+def test_distill_ruled_out_labels_cost_infinity_at_any_weight(v, k):
+    z, t, i = torch.zeros(3, v), torch.full((3, k), -math.inf), torch.arange(k).expand(3, k)
+    z[:, 0] = -math.inf
+    t[:, 0], t[:, 1] = torch.tensor([0.0, -90.0, -1e30]), 0.0                   # weights of 1/2 and less than fp32 holds
+    loss, grad = A.distill_top_logits_grad(z.to(DEV), t.to(DEV), i.to(DEV), torch.ones(3, device=DEV))
+    assert (loss == math.inf).all() and torch.isfinite(grad).all()
+    t[:, 0] = -math.inf                                                         # an empty slot costs nothing
+    assert torch.isfinite(A.distill_top_logits(z.to(DEV), t.to(DEV), i.to(DEV))).all()
+
+
 # ---- derivatives ----
 
 def test_forward_mode_over_backward_is_refused():
