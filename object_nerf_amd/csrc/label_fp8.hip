@@ -20,8 +20,8 @@
 // That instruction adds eight products at a time on a common exponent and drops what lies more than 13 bits under the largest of
 // them, before the sum reaches the fp32 accumulator (measured; the older v_mfma_f32_16x16x32_fp8_fp8 does the same): a product of
 // 128 normal numbers comes out 1.5e-5 off, relative to its norm.  Behind it a 16-bit result rounds by 1.7e-3 (bf16) or 2.1e-4 (fp16), so
-// C in 16 bits takes it.  C in fp32 does not: its operands are widened to bf16 in registers (exact: 4 bits and a power of two) and
-// multiplied by the bf16 instruction at half the rate, which keeps fp32 sums (1.2e-8).
+// C in 16 bits takes it.  C in fp32 does not: its operands are widened to bf16 in registers (exact: 4 bits and a power of two, down to
+// kLeastWide) and multiplied by the bf16 instruction at half the rate, which keeps fp32 sums (1.2e-8).
 //
 // Layout: values (R, C') with C' = C filled up to whole blocks with zeros; scales (R, B') bytes, one per row and block, B' = the
 // number of blocks filled up to a multiple of 4 (with 127): one aligned dword holds four blocks' scales, the instruction's op_sel
@@ -287,7 +287,9 @@ using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 typedef __attribute__((address_space(3))) uint8_t lds_byte;
 typedef const __attribute__((address_space(1))) uint8_t global_byte;
 
-// 8 elements (two dwords) times their block's scale: exact (4 bits, and bf16 has fp32's exponents)
+// 8 elements (two dwords) times their block's scale: exact where the last bit of e4m3's smallest, 2^-9 of the scale, is not under bf16's
+// smallest number, 2^-133: for scale bytes from kLeastWide on
+constexpr int kLeastWide = 3;
 __device__ __forceinline__ bf16x8 widened(int lo, int hi, float scale) {
   const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
   const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
@@ -497,6 +499,69 @@ __device__ __forceinline__ void write_tile(const GemmP& p, long m0, long n0, lds
   }
 }
 
+// A wave's tiles once more where some block's scale was under kLeastWide: the products without scales, and both exponents added to every
+// block's sums.  Straight from memory, a tile after the other: it is rare (an operand's block with nothing over 2^-116), and as code behind
+// the loop it costs the loop one minimum per scale: nothing measurable at 4096 x 4096 x 4096 (120 us), 3 % where a is fp32 rounded inside
+// (307200 x 128 x 256: 110 to 114 us, registers).
+template <class A> struct AgainRow {                               // a lane's 32 elements of a block of a's row, and its scale
+  u32x4 f[2];
+  int scale;
+  __device__ __forceinline__ void load(const GemmP& p, long row, long block, int h) {
+    if constexpr (std::is_same<A, void>::value) {
+      const u32x4* const from = reinterpret_cast<const u32x4*>(p.a + row * p.lda + block * kBlock + h * 32);
+      f[0] = from[0];
+      f[1] = from[1];
+      scale = p.sa[row * p.ldsa + block];
+    } else {
+      const char* const from = reinterpret_cast<const char*>(p.a) + row * p.lda * A::kBytes;
+      const long c = block * kBlock + h * 32;
+      Eight<A> held;
+      float largest = 0.f, x[8];
+#pragma unroll 1
+      for (int e = 0; e < 32; ++e) largest = fmaxf(largest, finite_abs(c + e < p.cols ? A::load(from, c + e) : 0.f));
+      largest = join_rows<OpMax, true>(join_rows<OpMax, false>(largest));      // the four lanes of a row
+      scale = (int)scale_byte(largest);
+      const float inv = inverse_scale(scale);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        held.load(from, c + e * 8, p.cols);
+        held.values(x);
+        f[e >> 1][(e & 1) * 2] = fp8x4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+        f[e >> 1][(e & 1) * 2 + 1] = fp8x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+};
+template <class A, int TM, int TN>
+__device__ __forceinline__ void sum_again(const GemmP& p, long m0, long n0, long first, long steps, f32x4 (&acc)[TM][TN]) {
+#pragma unroll
+  for (int u = 0; u < TM; ++u)
+#pragma unroll
+    for (int t = 0; t < TN; ++t) {
+      f32x4 total = {};
+#pragma unroll 1
+      for (long block = first; block < first + steps; ++block) {
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));                             // no address is held from block to block or through the loops around
+        const int i = lane & 15, h = lane >> 4;
+        AgainRow<A> a;
+        a.load(p, min(m0 + u * 16 + i, p.M - 1), block, h);
+        const u32x4* const at = reinterpret_cast<const u32x4*>(p.b + min(n0 + t * 16 + i, p.N - 1) * p.ldb + block * kBlock + h * 32);
+        const u32x4 fb[2] = {at[0], at[1]};
+        f32x4 sum = {};
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widened(fb[q >> 1][(q & 1) * 2], fb[q >> 1][(q & 1) * 2 + 1], 1.f),
+                                                        widened(a.f[q >> 1][(q & 1) * 2], a.f[q >> 1][(q & 1) * 2 + 1], 1.f), sum, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) total[r] += __builtin_amdgcn_ldexpf(sum[r], a.scale + p.sb[min(n0 + t * 16 + h * 4 + r, p.N - 1) * p.ldsb + block] - 254);
+      }
+      acc[u][t] = total;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
 // BM x BN of C per workgroup of WM x WN waves, rows copied one step ahead, one barrier a step.  The instruction's "A" is b's rows and its
 // "B" a's: a lane's four results are four neighbouring columns of one row of C.  In the widened form the four instructions of a
 // block take 8 bytes of every lane's 32 each: another order of the same sum.
@@ -527,6 +592,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) gemm_fp8_kernel(GemmP p) {
   // a workgroup's tiles one after the other: the next one's first rows are on their way while this one's results are written
   for (bool more = true; more;) {
     f32x4 acc[TM][TN] = {};
+    int least = kLeastWide;                                        // scale byte of this lane's rows, where C is fp32
     const long m = m0, n = n0;
     at += gridDim.x;
     more = kRun && at < tiles_of<BM, BN>(p);
@@ -562,13 +628,17 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) gemm_fp8_kernel(GemmP p) {
 #pragma unroll
         for (int t = 0; t < TN; ++t) fb[t] = fragment(rows_b + t * 16 * kBlock, i, h);
 #pragma unroll
+        for (int t = 0; t < TM; ++t) least = min(least, sa[t]);
+#pragma unroll
         for (int q = 0; q < 4; ++q) {
           bf16x8 xa[TM];
 #pragma unroll
           for (int t = 0; t < TM; ++t) xa[t] = widened(fa[t][2 * q], fa[t][2 * q + 1], scale_of(sa[t]));
 #pragma unroll
           for (int t = 0; t < TN; ++t) {
-            const bf16x8 xb = widened(fb[t][2 * q], fb[t][2 * q + 1], scale_of(scale_b[t * 64]));
+            const int sb = scale_b[t * 64];
+            if (q == 3) least = min(least, sb);
+            const bf16x8 xb = widened(fb[t][2 * q], fb[t][2 * q + 1], scale_of(sb));
 #pragma unroll
             for (int u = 0; u < TM; ++u) acc[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb, xa[u], acc[u][t], 0, 0, 0);
           }
@@ -584,6 +654,8 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) gemm_fp8_kernel(GemmP p) {
       }
       if (!last || more) raw.store(copy, slot, copy.scale_at(block, scale_slot));
     }
+    if constexpr (WIDE)
+      if (__any(least < kLeastWide)) sum_again<A, TM, TN>(p, m + wm, n + wn, first, steps, acc);
     // the slot that has just been read serves the results; the other one's copies are under way: a barrier that waits for none
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();

@@ -131,6 +131,39 @@ def test_distill_ruled_out_labels_cost_infinity_at_any_weight(v, k):
     assert torch.isfinite(A.distill_top_logits(z.to(DEV), t.to(DEV), i.to(DEV))).all()
 
 
+# ---- products in 8-bit floating point ----
+
+def _values(q):
+    return (q.data.double() * torch.exp2(q.scale.double() - 127).repeat_interleave(128, 1)[:, :q.data.shape[1]])[:, :q.cols]
+
+
+@pytest.mark.parametrize("m,n,k,dtype", [(5, 300, 130, F32), (30, 70, 4000, BF16), (200, 100, 300, F32), (200, 100, 300, BF16), (130, 520, 9000, F32), (70000, 70, 200, BF16), (300, 1000, 128, F32)])
+def test_linear_fp8_smallest_scales(m, n, k, dtype):
+    """Blocks whose values reach down to where bf16, through which fp32 results go, has no more bits.  Scales of 2^-126 and 2^-125 in some rows
+    of either factor and in some blocks of a row, next to scales that bring the results back; 64-bit sums with the bound of fp32 ones:
+    two roundings a term, of the sum of magnitudes, where fp32 holds that sum."""
+    g = _gen(m + n)
+    x, w = torch.randn(m, k, generator=g), torch.randn(n, k, generator=g)
+    x[::3] *= 2.0 ** torch.randint(-131, -110, (len(x[::3]), 1), generator=g)
+    x[1::3, :100] *= 2.0 ** -120
+    w[:128] *= 2.0 ** 90
+    w[128:256] *= 2.0 ** -124
+    x[2::3] *= 2.0 ** 30
+    x = x.to(dtype)
+    q, w8 = A.quantize_fp8(x.to(DEV)), A.quantize_fp8(w.to(DEV), 128)
+    assert (q.scale < 3).any() and (n <= 128 or (w8.scale < 3).any())
+    a, b = _values(q), _values(w8)
+    want, size = a @ b.t().contiguous(), a.abs() @ b.abs().t().contiguous()
+    bound = torch.where(size < 2.0 ** 127, (k + 2) * 2 * R.STEP[F32] * size + 2.0 ** -126, math.inf)
+    assert (bound < math.inf).double().mean() > 0.5
+    for y in (A.linear_fp8(x.to(DEV), w8, out_dtype=F32), A.matmul_fp8(q, w8, out_dtype=F32)):
+        far = ((y.double() - want).abs() > bound) & (bound < math.inf)
+        assert not far.any(), ((y.double() - want).abs() / bound)[far].max().item()
+    rows = A.matmul_fp8(q, w8, out_dtype=F32)[1]
+    other = A.quantize_fp8(torch.cat([x[1:2], torch.randn(40, k, generator=g).to(dtype)]).to(DEV))          # rows do not see their neighbours' scales
+    assert not (((A.matmul_fp8(other, w8, out_dtype=F32)[0].double() - rows.double()).abs() > bound[1]) & (bound[1] < math.inf)).any()
+
+
 # ---- derivatives ----
 
 def test_forward_mode_over_backward_is_refused():
