@@ -562,6 +562,10 @@ __device__ __forceinline__ void sum_again(const GemmP& p, long m0, long n0, long
     }
 }
 
+// Before a barrier behind which other waves read what this one's copies bring: the copies count as loads from memory, and nothing in the
+// barrier itself waits for them.
+__device__ __forceinline__ void copies_landed() { __builtin_amdgcn_s_waitcnt(0x0f70); }      // vmcnt 0; the other counters stay
+
 // BM x BN of C per workgroup of WM x WN waves, rows copied one step ahead, one barrier a step.  The instruction's "A" is b's rows and its
 // "B" a's: a lane's four results are four neighbouring columns of one row of C.  In the widened form the four instructions of a
 // block take 8 bytes of every lane's 32 each: another order of the same sum.
@@ -571,7 +575,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) gemm_fp8_kernel(GemmP p) {
   using Copy = Copies<BM, BN, WM * WN, kRaw>;
   using Raw = typename std::conditional<kRaw, RawRows<typename std::conditional<kRaw, A, ElemF32>::type, BM, WM * WN * 64, Copy>, NoRaw>::type;
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
-  __shared__ __align__(16) uint8_t ring[Copy::kBytes];           // one object: the copies' waits stay with the barrier
+  __shared__ __align__(16) uint8_t ring[Copy::kBytes];
   static_assert(WM * WN * 16 * (TN * 16 + 4) * 4 <= Copy::kSlot, "the waves' areas of write_tile fit into a slot");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, h = lane >> 4;
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
@@ -597,6 +601,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) gemm_fp8_kernel(GemmP p) {
     at += gridDim.x;
     more = kRun && at < tiles_of<BM, BN>(p);
     for (long step = 0; step < steps; ++step) {
+      copies_landed();
       __syncthreads();                                             // the step's rows have landed; the other slot has been read
       const lds_byte* const rows_a = copy.lds + slot * Copy::kSlot + wm * kBlock;
       const lds_byte* const rows_b = copy.lds + slot * Copy::kSlot + (BM + wn) * kBlock;

@@ -1,5 +1,9 @@
 """CPU: limits of the label operators, refused before anything is launched."""
 import ctypes as C
+import os
+import re
+import shutil
+import subprocess
 
 import pytest
 import torch
@@ -48,3 +52,32 @@ def test_recorders_are_refused(call):
         make_fx(call)(z, w)
     with pytest.raises(RuntimeError, match="GPU"):
         call(z, w)
+
+
+CSRC = os.path.join(os.path.dirname(os.path.abspath(A.__file__)), "csrc")
+
+
+@pytest.mark.skipif(shutil.which("hipcc") is None, reason="needs the compiler")
+def test_product_waits_for_its_copies_before_every_barrier(tmp_path):
+    """A wave's copies from memory into LDS are read by the others behind the next barrier, so each wave has to wait for its own in front of
+    it, in every instance and not where the compiler happens to.  (The one barrier in an asm block of its own, which orders reads of
+    LDS alone, waits for nothing on purpose.)"""
+    flags = re.search(r"^CXXFLAGS := (.*)$", open(os.path.join(CSRC, "Makefile")).read(), re.M).group(1)
+    flags = [f for f in flags.replace("$(ARCH)", "gfx950").replace("$(NO_PACKED)", "-Xclang -target-feature -Xclang -packed-fp32-ops").split() if "$" not in f]
+    out = str(tmp_path / "label_fp8.s")
+    subprocess.run(["hipcc", *flags, "--offload-device-only", "-S", os.path.join(CSRC, "label_fp8.hip"), "-o", out], check=True, stderr=subprocess.DEVNULL)
+    kernels = 0
+    for name, body in re.findall(r"^(_Z\S*gemm_fp8_kernel\S*):[^\n]*\n(.*?)^\.Lfunc_end", open(out).read(), re.M | re.S):
+        lines = [x.strip() for x in body.split("\n")]
+        barriers = [i for i, x in enumerate(lines) if x.startswith("s_barrier")]
+        assert any("global_load_lds" in x for x in lines) and len(barriers) >= 2, name
+        bare = 0
+        for i in barriers:
+            back = i - 1
+            while not re.match(r"s_waitcnt.*vmcnt\(0\)|\S+:|s_c?branch|;;#ASMEND", lines[back]):
+                back -= 1
+            bare += lines[back].startswith(";;#ASMEND")
+            assert "vmcnt(0)" in lines[back] or lines[back].startswith(";;#ASMEND"), (name, lines[back:i + 1])
+        assert bare <= 1, name
+        kernels += 1
+    assert kernels == 26                                        # 2 or 3 tiles x 3 result types x 4 operand types, the widened and raw forms without the largest
