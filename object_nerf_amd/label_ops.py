@@ -198,8 +198,12 @@ def quantize_fp8(x, block_rows=1, transpose=False):
 
 
 def matmul_fp8(a, b, bias=None, activation=None, out_dtype=torch.bfloat16):
-    """a @ b.T (+ bias) of two Fp8Matrix (M, K) and (N, K): fp32 sums, rounded once to out_dtype (float32, bfloat16 or float16).
-    activation: None or "leaky_relu" (slope 0.01, the reference's layers).  Not differentiable (linear_fp8 is)."""
+    """a @ b.T (+ bias) of two Fp8Matrix (M, K) and (N, K) in out_dtype (float32, bfloat16 or float16).
+
+    float32: fp32 sums.  bfloat16, float16: the 8-bit matrix instruction, at twice the rate.  It drops what lies more than 13 bits under the
+    largest of eight products on the way into the fp32 sum, 1.5e-5 of the result's norm for normal numbers: less than a rounding for
+    results of the usual size, but an element whose terms cancel can be off by more than its own rounding.  Take float32 where that
+    counts.  The result is rounded once.  activation: None or "leaky_relu" (slope 0.01, the reference's layers).  Not differentiable (linear_fp8 is)."""
     _checked_fp8(a, "a")
     _checked_fp8(b, "b")
     if a.cols != b.cols:
@@ -257,7 +261,9 @@ def linear_fp8(x, weight, bias=None, out_dtype=None):
     x (M, K); weight (N, K), K <= 2^26, a tensor -- rounded in every call, so that what an optimizer wrote is what counts -- or the Fp8Matrix that
     quantize_fp8(weight, block_rows=128) laid out once, for inference; bias (N,).  Sizes need not be multiples of anything.  With a tensor
     as weight it is differentiable: dX and dW are products of the same kind, of the gradient rounded along their own sums, in x's and
-    weight's types (of at most 2^26 rows of x, of weight); the bias gradient is an fp32 sum."""
+    weight's types (of at most 2^26 rows of x, of weight); the bias gradient is an fp32 sum.
+
+    Results and gradients in float32 are fp32 sums; in bfloat16 and float16 they are those of the 8-bit matrix instruction (matmul_fp8)."""
     x = _rows(x, "x")
     _refuse_tangents(x, weight, bias)
     out_dtype = x.dtype if out_dtype is None else out_dtype

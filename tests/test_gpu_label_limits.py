@@ -164,6 +164,44 @@ def test_linear_fp8_smallest_scales(m, n, k, dtype):
     assert not (((A.matmul_fp8(other, w8, out_dtype=F32)[0].double() - rows.double()).abs() > bound[1]) & (bound[1] < math.inf)).any()
 
 
+PRODUCTS = [(5, 300, 130), (16, 4096, 1000), (30, 70, 4000), (64, 64, 8000), (200, 100, 300), (389, 520, 9000), (1000, 96, 256), (4000, 3700, 1100), (70000, 70, 200), (9000, 1100, 130)]
+
+
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+@pytest.mark.parametrize("out", [F32, BF16, F16])
+def test_linear_fp8_counts_every_product_once(m, n, k, out):
+    """Whole numbers whose sums every type holds, under scales that differ from row to row and block to block: nothing is rounded or dropped,
+    so a lost, doubled or wrongly scaled product shows.  Rows of x: +-1 at twelve places; weights: whole numbers up to 7."""
+    g = torch.Generator(device=DEV).manual_seed(m + k)
+    kb, nb = -(-k // 128), -(-n // 128)
+    x = torch.zeros(m, k, device=DEV)
+    at = torch.randint(0, k, (m, 12), device=DEV, generator=g)
+    x.scatter_(1, at, torch.where(torch.rand(m, 12, device=DEV, generator=g) < 0.5, -1.0, 1.0))
+    w = torch.randint(-7, 8, (n, k), device=DEV, generator=g).float()
+    want = torch.mm(x, w.t().contiguous())                                      # whole numbers up to 84: exact in fp32 in any order
+    p = torch.exp2(torch.randint(-20, 21, (kb,), device=DEV, generator=g).float()).repeat_interleave(128)[:k]
+    r = torch.exp2(torch.randint(-3, 4, (m, 1), device=DEV, generator=g).float())
+    c = torch.exp2(torch.randint(-2, 3, (nb,), device=DEV, generator=g).float()).repeat_interleave(128)[:n]
+    want = want * r * c
+    w8 = A.quantize_fp8(w / p * c[:, None], 128)
+    for y in (A.linear_fp8(x * p * r, w8, out_dtype=out), A.matmul_fp8(A.quantize_fp8(x * p * r), w8, out_dtype=out)):
+        assert torch.equal(y.float(), want)
+
+
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+@pytest.mark.parametrize("out", [BF16, F16])
+def test_matmul_fp8_precision_of_16_bit_results(m, n, k, out):
+    """The instruction's error d before the rounding is 1.5e-5 of the result's norm (measured); 3e-5 is let through.  round(x + d) and
+    round(x) differ by whole steps of at most 2 h |x| (h: half a step), by |d| on average, so their squared distance is 2 h |x| |d| on
+    average and in norm at most sqrt(2 h 3e-5) of x; a tenth more for the average being one of a sample."""
+    g = torch.Generator(device=DEV).manual_seed(n)
+    a, b = A.quantize_fp8(torch.randn(m, k, device=DEV, generator=g)), A.quantize_fp8(torch.randn(n, k, device=DEV, generator=g), 128)
+    want = torch.mm(_values(a), _values(b).t().contiguous())
+    for y in (A.matmul_fp8(a, b, out_dtype=out), A.linear_fp8(_values(a).to(BF16), b, out_dtype=out)):        # 4 bits: x again what it was
+        off = (y.double() - want.to(out).double()).norm() / want.norm()
+        assert off.item() <= 1.1 * (2 * R.STEP[out] * 3e-5) ** 0.5
+
+
 # ---- derivatives ----
 
 def test_forward_mode_over_backward_is_refused():
