@@ -6,7 +6,8 @@
   distill_top_logits        loss of rows of student logits against a teacher's top logits (a 2-D segmenter of which only the largest
                             values per pixel are stored), differentiable; distill_top_logits_grad: loss and gradient in one pass
   sample_logits             one label per row at a given random number, behind temperature / top-k / top-p / min-p -- to logits what
-                            `sample_pdf` is to a ray's weights; its int64 labels are the `instance_ids` that `CodeLibrary` takes
+                            `sample_pdf` is to a ray's weights; its int64 labels are the `instance_ids` that `CodeLibrary` takes, except
+                            the -1 of a row with nothing to draw, which a table lookup on the GPU takes as out of range
 
 Rows are (N, V) on the GPU in float32, bfloat16 or float16 with any row stride; a last dimension that is not contiguous is copied.
 Python here checks arguments, allocates results and enqueues on the current stream of the tensors' device; nothing synchronises, and
@@ -382,7 +383,8 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     cut to the first `top_k` (0: all), of those to the shortest prefix whose share of their weight reaches `top_p` (1: all; at
     least one label stays), of those to the ones with at least `min_p` times the largest weight (0: all).  The label is the
     first, in that order, whose running sum of weight exceeds u times their total.  temperature 0 and top_k 1 give the first
-    of the order.  NaN counts as -inf; a row of nothing but -inf gives -1.
+    of the order.  NaN counts as -inf; a row of nothing but -inf gives -1, which is no index: clamp it, and keep `labels >= 0`, before
+    a table lookup.
 
     Each setting is a number or an (N,) tensor on the logits' device, one value per row, held as float32 (top_k: int32), as u is.  Runs give equal labels for equal inputs."""
     logits = _rows(logits, "logits")

@@ -53,6 +53,19 @@ def test_sample_top_k_per_row_of_any_whole_type(dtype):
     assert torch.equal(label.cpu(), R.sample(z, u, 1.0, torch.tensor([min(x, v) for x in k]), 1.0, 0.0))
 
 
+def test_labels_of_rays_with_an_infinite_feature_go_into_the_table():
+    """as the documentation has it: -1 clamped for the lookup, and known"""
+    g = _gen(2)
+    features, weight = torch.randn(30, 40, generator=g), torch.randn(64, 40, generator=g)
+    features[7, 3], features[11, 0] = math.inf, math.nan
+    ids = A.sample_logits(A.linear_fp8(features.to(DEV), A.quantize_fp8(weight.to(DEV), block_rows=128)), torch.rand(30, generator=g).to(DEV), temperature=0.8, top_k=8)
+    known = ids >= 0
+    assert (~known).nonzero().flatten().tolist() == [7, 11]
+    codes = A.CodeLibrary(A.default_model_config()).to(DEV)
+    code = codes({"instance_ids": ids.clamp(min=0)})["embedding_instance"]
+    assert torch.equal(code.detach()[known], codes.embedding_instance.weight.detach()[ids[known]])
+
+
 # ---- views that stand for minus their memory ----
 
 @pytest.mark.parametrize("v", [1, 40])
