@@ -252,9 +252,6 @@ __device__ __forceinline__ void load_bias(f32x16 (&acc)[NT], const float* aux, i
   for (int m = 0; m < NT; ++m) acc[m] = *(const f32x16*)(b + m * 32);
 }
 
-#ifndef OBJ_PK_LEAKY
-#define OBJ_PK_LEAKY 1
-#endif
 using f32x2 = __attribute__((ext_vector_type(2))) float;
 template <int NT, bool ACT>
 __device__ __forceinline__ void finish(const f32x16 (&acc)[NT], f32x16 (&h)[NT]) {
@@ -262,16 +259,14 @@ __device__ __forceinline__ void finish(const f32x16 (&acc)[NT], f32x16 (&h)[NT])
   for (int m = 0; m < NT; ++m)
 #pragma unroll
     for (int r = 0; r < 16; r += 2) {
-      if constexpr (ACT && OBJ_PK_LEAKY) {
-        // 0.01 v for two values at a time: the same two IEEE operations per value as leaky(), bit-equal (the build has packed fp32
-        // instructions switched off: Makefile)
+      if constexpr (ACT) {               // two values at a time: the same two IEEE operations per value as leaky(), bit-equal
         const f32x2 v = {acc[m][r], acc[m][r + 1]};
         const f32x2 sl = v * 0.01f;
         h[m][r] = fmaxf(v[0], sl[0]);
         h[m][r + 1] = fmaxf(v[1], sl[1]);
       } else {
-        h[m][r] = ACT ? leaky(acc[m][r]) : acc[m][r];
-        h[m][r + 1] = ACT ? leaky(acc[m][r + 1]) : acc[m][r + 1];
+        h[m][r] = acc[m][r];
+        h[m][r + 1] = acc[m][r + 1];
       }
     }
 }
@@ -333,21 +328,15 @@ __device__ __forceinline__ void finish_add(const f32x16 (&acc)[NT], const f32x16
   for (int m = 0; m < NT; ++m)
 #pragma unroll
     for (int r = 0; r < 16; r += 2) {
-      if constexpr (OBJ_PK_LEAKY) {      // two values at a time: the same IEEE operations
-        const f32x2 a2 = {acc[m][r], acc[m][r + 1]}, b2 = {add[m][r], add[m][r + 1]};
-        const f32x2 v = a2 + b2;
-        if constexpr (ACT) {
-          const f32x2 sl = v * 0.01f;
-          h[m][r] = fmaxf(v[0], sl[0]);
-          h[m][r + 1] = fmaxf(v[1], sl[1]);
-        } else {
-          h[m][r] = v[0];
-          h[m][r + 1] = v[1];
-        }
+      const f32x2 a2 = {acc[m][r], acc[m][r + 1]}, b2 = {add[m][r], add[m][r + 1]};
+      const f32x2 v = a2 + b2;
+      if constexpr (ACT) {
+        const f32x2 sl = v * 0.01f;
+        h[m][r] = fmaxf(v[0], sl[0]);
+        h[m][r + 1] = fmaxf(v[1], sl[1]);
       } else {
-        const float v0 = acc[m][r] + add[m][r], v1 = acc[m][r + 1] + add[m][r + 1];
-        h[m][r] = ACT ? leaky(v0) : v0;
-        h[m][r + 1] = ACT ? leaky(v1) : v1;
+        h[m][r] = v[0];
+        h[m][r + 1] = v[1];
       }
     }
 }
