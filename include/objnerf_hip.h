@@ -634,7 +634,7 @@ int objnerf_repeat_rows(const float* src, int64_t lds, int64_t n_rows, int C, in
 /* Distillation from a teacher's top logits.  Per row: p = softmax(teacher / T) over the slots whose index lies in [0, v) (any other
  * index: an empty slot; so is a teacher value of -inf), q = softmax(student / T) over the v logits,
  *   loss = sum_j p_j (log p_j - log q_{i_j}),    grad_v = (upstream / T) (q_v - sum_{j: i_j = v} p_j).
- * A row without a filled slot has loss 0 and gradient 0 whatever its logits hold; otherwise NaN in the row, or no finite student
+ * A row without a filled slot has loss 0 and gradient 0 whatever its logits hold; otherwise NaN or +inf in the row, or no finite student
  * logit, gives a loss of NaN; a student logit of -inf under a filled slot a loss of +inf.  An index may occur more than once.  loss or grad may
  * be NULL; grad must not overlap student.  Sums in a fixed order: bit-reproducible.  fp32 statistics, grad rounded once. */
 typedef struct {

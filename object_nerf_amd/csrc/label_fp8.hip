@@ -401,7 +401,7 @@ template <int BM, int BN, int WAVES, bool RAW> struct Copies {
   __device__ __forceinline__ lds_byte* scale_at(long block, int slot) const { return lds + 2 * kSlot + slot * kScaleRows * 4 + (int)(block & 3); }
 };
 // a's rows of a step where they are rounded on their way into LDS: 16 lanes per row and block, held in registers from the load to the
-// store, so that the step in between hides the load.
+// store.  The load is not hidden by the step in between: as built, the step's products stand behind the wait for it.
 template <class A, int BM, int THREADS, class COPY> struct RawRows {
   static constexpr int kPasses = BM * 16 / THREADS;
   Eight<A> held[kPasses];
@@ -593,7 +593,8 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) gemm_fp8_kernel(GemmP p) {
     copy.scales(first >> 2, 0);
     raw.store(copy, 0, copy.scale_at(first, 0));
   }
-  // a workgroup's tiles one after the other: the next one's first rows are on their way while this one's results are written
+  // a workgroup's tiles one after the other: the next one's first rows are asked for before this one's results are written, and have
+  // arrived before the first of them is stored (write_tile's loads of the bias are counted behind them)
   for (bool more = true; more;) {
     f32x4 acc[TM][TN] = {};
     int least = kLeastWide;                                        // scale byte of this lane's rows, where C is fp32
@@ -661,7 +662,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) gemm_fp8_kernel(GemmP p) {
     }
     if constexpr (WIDE)
       if (__any(least < kLeastWide)) sum_again<A, TM, TN>(p, m + wm, n + wn, first, steps, acc);
-    // the slot that has just been read serves the results; the other one's copies are under way: a barrier that waits for none
+    // the slot that has just been read serves the results; the other one's copies are under way: a barrier that waits for none of them
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");

@@ -95,7 +95,8 @@ __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES, LANES < 1024 ? 6 : 
   const char* z = static_cast<const char*>(p.z) + row * p.ldz * E::kBytes;
   const int pieces = p.v / E::kVec, tail = p.v - pieces * E::kVec;
 
-  // everything that does not wait for anything is asked for first: the row, the slots, the students' values under them
+  // asked for first: the row, then this thread's slot -- its index, the teacher's value of a filled slot, the student's value under it,
+  // each behind the one before (and, as loads are counted in order, behind the row)
   u32x4 r[PIECES > 0 ? PIECES : 1];
   if constexpr (PIECES > 0)
 #pragma unroll

@@ -354,7 +354,7 @@ def distill_top_logits(student, teacher, index, temperature=1.0):
 
     student (N, V); teacher (N, k) logits or log-probabilities, k <= 1024; index (N, k) int32 or int64, the labels that the
     teacher's values belong to.  A slot whose index lies outside [0, V) or whose value is -inf is empty; a row without a filled slot
-    has loss 0 and gradient 0; otherwise NaN in the row gives a loss of NaN, a label ruled out by the student (-inf) under a filled slot a loss
+    has loss 0 and gradient 0; otherwise NaN or +inf in the row, or nothing but -inf among the student's values, gives a loss of NaN, a label ruled out by the student (-inf) under a filled slot a loss
     of +inf.  An index may occur more than once (its shares add).  Differentiable with respect to `student`
     alone; the usual factor T^2 is the caller's.  The backward pass reads the student's row again instead of keeping a copy."""
     _refuse_tangents(student, teacher)

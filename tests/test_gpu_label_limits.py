@@ -215,6 +215,35 @@ def test_matmul_fp8_precision_of_16_bit_results(m, n, k, out):
         assert off.item() <= 1.1 * (2 * R.STEP[out] * 3e-5) ** 0.5
 
 
+def test_results_and_rows_past_32_bits():
+    """more than 2^31 results, 2^32 bytes of 8-bit values and of logits: the rows around those ends against the same rows by themselves"""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    m, n, k = 600000, 8000, 130
+    x, w8 = torch.randn(m, k, device=DEV, generator=g).to(BF16), A.quantize_fp8(torch.randn(n, k, device=DEV, generator=g), 128)
+    ends = [0, (1 << 31) // n, (1 << 32) // n, m - 1]
+    for y in (A.linear_fp8(x, w8), A.matmul_fp8(A.quantize_fp8(x), w8)):
+        for at in ends:
+            rows = slice(max(0, at - 20), at + 20)
+            assert torch.equal(y[rows], A.linear_fp8(x[rows], w8)) or (y[rows].double() - A.linear_fp8(x[rows], w8).double()).norm() <= 1e-3 * y[rows].double().norm()
+        u, t, i = torch.rand(m, device=DEV, generator=g), torch.randn(m, 3, device=DEV, generator=g), torch.randint(0, n, (m, 3), device=DEV, generator=g)
+        label, (loss, grad) = A.sample_logits(y, u, top_p=0.9), A.distill_top_logits_grad(y, t, i, u)
+        for at in ends:
+            rows = slice(max(0, at - 20), at + 20)
+            assert torch.equal(label[rows], A.sample_logits(y[rows], u[rows], top_p=0.9))
+            for got, want in zip((loss, grad), A.distill_top_logits_grad(y[rows], t[rows], i[rows], u[rows])):
+                assert torch.equal(got[rows], want)
+        del label, loss, grad
+    for block_rows in (1, 128):
+        for transpose in (False, True):
+            q = A.quantize_fp8(y, block_rows, transpose)
+            for at in ((1 << 31) // n, (1 << 32) // n, m - 130):
+                at -= at % 128
+                want = A.quantize_fp8(y[at:at + 128], block_rows, transpose)
+                data, scale = (q.data[:, at:at + 128], q.scale[:, at // 128:at // 128 + 1]) if transpose else (q.data[at:at + 128], q.scale[at:at + 128])
+                assert torch.equal(data.view(torch.uint8), want.data.view(torch.uint8)) and torch.equal(scale, want.scale[:, :scale.shape[1]])
+            del q
+
+
 # ---- derivatives ----
 
 def test_forward_mode_over_backward_is_refused():
