@@ -34,9 +34,12 @@ MAX_INT = (1 << 31) - 1                # rows, and labels of the distillation
 MAX_LABELS = 1 << 19                   # of a row that a label is drawn from
 
 
+_tracing, _modes, _mode, _PROXY = torch._C._is_tracing, torch._C._len_torch_dispatch_stack, torch._C._get_dispatch_mode, torch._C._TorchDispatchModeKey.PROXY
+
+
 def _refuse_recording():
-    """a recorded program would hold the allocation of the results and no kernel"""
-    if torch._C._get_tracing_state() is not None or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+    """a recorded program would hold the allocation of the results and no kernel.  Once a call (0.2 us)"""
+    if _tracing() or (_modes() and _mode(_PROXY) is not None):
         raise RuntimeError("the label operators cannot be recorded by torch.jit.trace or make_fx: the kernels would be missing")
 
 
@@ -50,7 +53,6 @@ def _refuse_tangents(*tensors):
 
 def _rows(t, name, types=_TYPES):
     """t as a 2-D GPU tensor whose rows are contiguous"""
-    _refuse_recording()
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s must be a tensor, got %s" % (name, type(t).__name__))
     if t.dim() != 2:
@@ -59,7 +61,7 @@ def _rows(t, name, types=_TYPES):
         raise TypeError("%s: dtype %s is not supported" % (name, t.dtype))
     if not t.is_cuda:
         _lib.require_cuda(t, name)
-    if t.is_neg():                                    # a view that stands for minus its memory (the imaginary part of a conjugate)
+    if types is _TYPES and t.is_neg():                # a view that stands for minus its memory (the imaginary part of a conjugate)
         t = t.resolve_neg()
     return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
@@ -72,13 +74,15 @@ def _column(t, name, n, device, dtype=torch.float32):
         raise ValueError("%s must be on %s, got %s" % (name, device, t.device))
     if t.is_floating_point() != dtype.is_floating_point or t.dtype == torch.bool or t.is_complex():
         raise TypeError("%s: dtype %s is not supported" % (name, t.dtype))
-    return (t if t.dtype == dtype else t.to(dtype)).resolve_neg().contiguous()
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    return (t.resolve_neg() if t.is_neg() else t).contiguous()
 
 
 def _call(fn, args, device, what):
     """enqueues `fn` on the current stream of `device`"""
     index = device.index
-    if index != torch.cuda.current_device():
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return _call(fn, args, device, what)
     rc = fn(C.byref(args), torch._C._cuda_getCurrentRawStream(index))      # (torch.cuda.current_stream() costs 2.7 us)
@@ -161,7 +165,6 @@ def _rounded_product(x, w, bias, out_dtype):
 
 
 def _checked_fp8(x, name):
-    _refuse_recording()
     if not isinstance(x, Fp8Matrix):
         raise TypeError("%s must be an Fp8Matrix (quantize_fp8), got %s" % (name, type(x).__name__))
     d, s = x.data, x.scale
@@ -192,6 +195,7 @@ def quantize_fp8(x, block_rows=1, transpose=False):
     (block_rows 128: weights).  A block's scale is the smallest power of two with max|block| / scale <= 448, so dividing by it is exact and
     an element is rounded once, to nearest even; infinities and NaN become NaN and set no scale.  `transpose` rounds x.T -- its blocks run
     along x's rows -- without forming it."""
+    _refuse_recording()
     if block_rows not in (1, BLOCK):
         raise ValueError("block_rows must be 1 or 128, got %r" % (block_rows,))
     q, t, _ = _quantize(_rows(x, "x").detach(), block_rows, not transpose, transpose)
@@ -205,6 +209,7 @@ def matmul_fp8(a, b, bias=None, activation=None, out_dtype=torch.bfloat16):
     largest of eight products on the way into the fp32 sum, 1.5e-5 of the result's norm for normal numbers: less than a rounding for
     results of the usual size, but an element whose terms cancel can be off by more than its own rounding.  Take float32 where that
     counts.  The result is rounded once.  activation: None or "leaky_relu" (slope 0.01, the reference's layers).  Not differentiable (linear_fp8 is)."""
+    _refuse_recording()
     _checked_fp8(a, "a")
     _checked_fp8(b, "b")
     if a.cols != b.cols:
@@ -265,6 +270,7 @@ def linear_fp8(x, weight, bias=None, out_dtype=None):
     weight's types (of at most 2^26 rows of x, of weight); the bias gradient is an fp32 sum.
 
     Results and gradients in float32 are fp32 sums; in bfloat16 and float16 they are those of the 8-bit matrix instruction (matmul_fp8)."""
+    _refuse_recording()
     x = _rows(x, "x")
     _refuse_tangents(x, weight, bias)
     out_dtype = x.dtype if out_dtype is None else out_dtype
@@ -293,6 +299,7 @@ def linear_fp8(x, weight, bias=None, out_dtype=None):
 # ---- distillation ----
 
 def _distill_args(student, teacher, index, temperature):
+    _refuse_recording()
     student = _rows(student, "student")
     teacher = _rows(teacher, "teacher")
     index = _rows(index, "index", (torch.int32, torch.int64))
@@ -344,8 +351,10 @@ class _DistillFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_loss):
         _refuse_tangents(d_loss)
+        if d_loss.dtype != torch.float32 or d_loss.is_neg():
+            d_loss = d_loss.float().resolve_neg()
         a, keep = _distill_args(*ctx.saved_tensors, ctx.temperature)
-        return _run_distill(a, keep, False, d_loss.float().resolve_neg())[1], None, None, None
+        return _run_distill(a, keep, False, d_loss)[1], None, None, None
 
 
 def distill_top_logits(student, teacher, index, temperature=1.0):
@@ -387,6 +396,7 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     a table lookup.
 
     Each setting is a number or an (N,) tensor on the logits' device, one value per row, held as float32 (top_k: int32), as u is.  Runs give equal labels for equal inputs."""
+    _refuse_recording()
     logits = _rows(logits, "logits")
     n, v = logits.shape
     dev = logits.device
@@ -407,8 +417,10 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         if not 0.0 <= temperature < 1e300:
             raise ValueError("temperature must be >= 0 and finite, got %r" % temperature)
     if isinstance(top_k, torch.Tensor):
-        if top_k.dtype in (torch.int64, torch.uint64):       # (the conversion would drop the upper half; 2^63 and more count as -1: all)
-            top_k = top_k.to(torch.int64).clamp(-1, 2 ** 31 - 1)
+        if top_k.dtype == torch.uint64:                      # (2^63 and more count as -1: all)
+            top_k = top_k.to(torch.int64)
+        if top_k.dtype == torch.int64:
+            top_k = top_k.clamp(-1, 2 ** 31 - 1)             # (the conversion would drop the upper half)
         keep.append(_column(top_k, "top_k", n, dev, torch.int32))
         a.top_k_rows = keep[-1].data_ptr()
     else:
