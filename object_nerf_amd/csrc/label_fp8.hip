@@ -6,10 +6,11 @@
 //
 // Measured (copy of this card 4.96 TB/s, fp8 product of the library at 8192 x 8192 x 8192 2.77 PFLOP/s): rounding 307,200 x 256 bf16 by
 // rows 46 us = 5.1 TB/s, 16,383 x 2,056 in both forms 33 us = 4.1 TB/s; product 8192 x 8192 x 8192 480 us = 2.29 PFLOP/s, x 4096
-// 259 us = 2.12 PFLOP/s, 4096 x 4096 x 4096 64 us = 2.15 PFLOP/s, 2,056 x 520 x 16,384 with fp32 results 56 us = 0.63 PFLOP/s; four
-// rows against 32,768 x 256 (8.4 MB of weights) 4 us.  What bounds it: large products the matrix pipe at the clock that it leaves itself and the two slots' copies, which
-// have one block's products to arrive in; sums of a few blocks the launch-to-store latency of a tile; hidden layers over a frame the
-// write path.
+// 239-259 us = 2.1-2.3 PFLOP/s, 4096 x 4096 x 4096 64 us = 2.15 PFLOP/s and 120 with fp32 results = 1.14, 2,056 x 520 x 16,384 with fp32
+// results 53-56 us = 0.64 PFLOP/s; four rows against 32,768 x 256 (8.4 MB of weights) 4-6 us.  What bounds it: large products waits, for
+// fragments read just in front of their products and for a block's copies (the matrix pipe is busy 0.46 of the time); sums of a few blocks
+// the launch-to-store latency of a tile; hidden layers over a frame the write path.  Columns that are no multiple of 8 read a row's last
+// ones an element after the other.
 //
 // The scale is a power of two on purpose.  Dividing by it is exact, so an element is rounded once and the byte form has one meaning;
 // a factor up to 2 of the range it gives away costs no precision (a floating-point format's step does not depend on where in its

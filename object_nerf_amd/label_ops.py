@@ -157,7 +157,7 @@ def _rounded_product(x, w, bias, out_dtype):
     """x rounded and multiplied.  One kernel where a row of x is read by one tile of columns (307,200 x 128 x 256: 62 us against 79 us with
     x rounded first), where x is a tile itself (16 x 4096 x 4096: 15 against 20) or the product no more than a launch (2,048 x 512 x
     256: 11 against 16); x rounded first where it is read more often (307,200 x 256 x 256: 107 against 111, 64 x 4096 x 4096: 21
-    against 25)."""
+    against 25; rounding inside hides none of its loads behind the products, as built)."""
     m, k, n = x.shape[0], x.shape[1], w.data.shape[0]
     if k and (n <= 128 or m <= 32 or (k <= 1024 and _up(m, BLOCK) * _up(n, BLOCK) <= 256 * BLOCK * BLOCK)):
         return _product(x, w, bias, False, out_dtype)
