@@ -99,7 +99,8 @@ class Fp8Matrix(NamedTuple):
     """A matrix (R, cols) in e4m3 with a power-of-two scale for each block of 128 columns of a row.
 
     data (R, C') float8_e4m3fn, C' = cols filled up to a multiple of 128 with zeros; scale (R, B') uint8, B' = C' / 128 filled up to a
-    multiple of 4: element [r, c] stands for data[r, c] * 2 ** (scale[r, c // 128] - 127), scale in [1, 254]."""
+    multiple of 4: element [r, c] stands for data[r, c] * 2 ** (scale[r, c // 128] - 127), scale in [1, 247] (what numbers of fp32 need; fp32
+    results of larger scales can overflow)."""
     data: torch.Tensor
     scale: torch.Tensor
     cols: int
