@@ -209,7 +209,8 @@ def matmul_fp8(a, b, bias=None, activation=None, out_dtype=torch.bfloat16):
     float32: fp32 sums.  bfloat16, float16: the 8-bit matrix instruction, at twice the rate.  It drops what lies more than 13 bits under the
     largest of eight products on the way into the fp32 sum, 1.5e-5 of the result's norm for normal numbers: less than a rounding for
     results of the usual size, but an element whose terms cancel can be off by more than its own rounding.  Take float32 where that
-    counts.  The result is rounded once.  activation: None or "leaky_relu" (slope 0.01, the reference's layers).  Not differentiable (linear_fp8 is)."""
+    counts.  The result is rounded once.  activation: None or "leaky_relu" (slope 0.01, the reference's layers).  Not differentiable
+    (linear_fp8 is)."""
     _refuse_recording()
     _checked_fp8(a, "a")
     _checked_fp8(b, "b")
@@ -364,8 +365,8 @@ def distill_top_logits(student, teacher, index, temperature=1.0):
 
     student (N, V); teacher (N, k) logits or log-probabilities, k <= 1024; index (N, k) int32 or int64, the labels that the
     teacher's values belong to.  A slot whose index lies outside [0, V) or whose value is -inf is empty; a row without a filled slot
-    has loss 0 and gradient 0; otherwise NaN or +inf in the row, or nothing but -inf among the student's values, gives a loss of NaN, a label ruled out by the student (-inf) under a filled slot a loss
-    of +inf.  An index may occur more than once (its shares add).  Differentiable with respect to `student`
+    has loss 0 and gradient 0; otherwise NaN or +inf in the row, or nothing but -inf among the student's values, gives a loss of NaN, a
+    label ruled out by the student (-inf) under a filled slot a loss of +inf.  An index may occur more than once (its shares add).  Differentiable with respect to `student`
     alone; the usual factor T^2 is the caller's.  The backward pass reads the student's row again instead of keeping a copy."""
     _refuse_tangents(student, teacher)
     if torch.is_grad_enabled() and isinstance(student, torch.Tensor) and student.requires_grad:
@@ -396,7 +397,8 @@ def sample_logits(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     of the order.  NaN counts as -inf; a row of nothing but -inf gives -1, which is no index: clamp it, and keep `labels >= 0`, before
     a table lookup.
 
-    Each setting is a number or an (N,) tensor on the logits' device, one value per row, held as float32 (top_k: int32), as u is.  Runs give equal labels for equal inputs."""
+    Each setting is a number or an (N,) tensor on the logits' device, one value per row, held as float32 (top_k: int32), as u is.  Runs
+    give equal labels for equal inputs."""
     _refuse_recording()
     logits = _rows(logits, "logits")
     n, v = logits.shape
