@@ -10,11 +10,11 @@
 // bring back: the differences are taken at 2^-12 of their size, and T < 1 divides the weight.
 //
 // Bound by memory, short rows by the vector units (307,200 x 64: 0.90 busy): a row up to 256 KB is read once and stays in registers
-// until dz is written (longer ones are read twice).  The statistics are fp32, the sums in a fixed order (bit-reproducible).  Measured: loss of 307,200 x 64 fp32 24 us = 3.6 TB/s, loss and
-// gradient of 1,023 x 30,011 fp16 29 us = 4.2 TB/s and of 2,048 x 32,768 bf16 61 us = 4.4 TB/s (a copy of this card: 4.96).  The
-// gradient's k special columns are not looked up while the row is
-// written: the whole row is written as if p were 0, and behind a barrier the slots' own threads write their columns again.  The
-// first slot of an index owns its column and adds the shares of later slots with the same index in their order.
+// until dz is written (longer ones are read twice).  The statistics are fp32, the sums in a fixed order (bit-reproducible).  Measured:
+// loss of 307,200 x 64 fp32 24 us = 3.6 TB/s, loss and gradient of 1,023 x 30,011 fp16 29 us = 4.2 TB/s and of 2,048 x 32,768 bf16 61 us =
+// 4.4 TB/s (a copy of this card: 4.96).  The gradient's k special columns are not looked up while the row is written: the whole row is
+// written as if p were 0, and behind a barrier the slots' own threads write their columns again.  The first slot of an index owns its
+// column and adds the shares of later slots with the same index in their order.
 #include "host_api.h"
 #include "label_ops.h"
 #include <type_traits>
